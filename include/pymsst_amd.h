@@ -30,8 +30,9 @@ extern "C" {
 #endif
 
 enum { PMSST_F32 = 0, PMSST_F16 = 1, PMSST_BF16 = 2 };
-/* Activation codes (mask-MLP hidden layer: Linear -> tanh, fr.py:340,538). */
-enum { PMSST_ACT_NONE = 0, PMSST_ACT_TANH = 1 };
+/* Activation codes (mask-MLP hidden layer: Linear -> tanh, fr.py:340,538; PMSST_ACT_GELU: the
+ * dropout entry points only, the exact GELU). */
+enum { PMSST_ACT_NONE = 0, PMSST_ACT_TANH = 1, PMSST_ACT_GELU = 2 };
 enum {
   PMSST_OK = 0,
   PMSST_EINVAL = -1,     /* bad shape, size, pointer or alignment */
@@ -382,6 +383,50 @@ int pmsst_mask_apply_backward(const void* grad_est, const void* spec, const void
                               int64_t mask_stem_stride, int64_t batch, int64_t stems, int64_t channels, int64_t freqs,
                               int64_t frames, int zero_dc, void* grad_mask, void* grad_spec, int mask_dtype,
                               void* stream);
+
+/* ------------------------------------------------------------------ dropout
+ * No reference counterpart (the stock blocks run nn.GELU, nn.Dropout and the residual sum as separate
+ * passes that keep a mask).  n dense elements; p in [0, 1); rng: device int64[2] {seed, offset}, read when
+ * the kernel runs (NULL where round(65536 p) is 0).  Element e is kept where its 16 bits of Philox4x32-7
+ * (counter e / 8 and offset, key seed; csrc/philox.h) are at least round(65536 p), at most 65535, and is
+ * then multiplied by 65536 / (65536 - round(65536 p)).  The mask is never stored.
+ * activation PMSST_ACT_GELU applies the exact GELU first.
+ */
+
+/* out = dropout(act(x)) + residual; residual may be NULL.  out may be x or residual itself. */
+int pmsst_dropout_forward(const void* x, const void* residual, void* out, int64_t n, double p, const int64_t* rng,
+                          int activation, int dtype, void* stream);
+/* grad_x = keep / (1 - p) * grad_out * act'(x), with the forward's p and rng; x (the forward's input) may
+ * be NULL without an activation.  grad_x may be grad_out itself. */
+int pmsst_dropout_backward(const void* grad_out, const void* x, void* grad_x, int64_t n, double p, const int64_t* rng,
+                           int activation, int dtype, void* stream);
+
+/* ------------------------------------------------------------------ cross attention
+ * No reference counterpart (the stock blocks call SDPA).  Queries q[batch, queries, heads, head_dim] over
+ * keys and values k, v[batch, keys, kv_heads, head_dim]; kv_heads divides heads, query head h attends with
+ * key head h / (heads / kv_heads).  head_dim: a multiple of 8 in [8, 128].  *_strides: host int64[3] element
+ * strides of the batch, position and head axes (the last axis is dense), or NULL for dense; base pointers
+ * and strides must be whole 16 bytes (a broadcast axis has stride 0).
+ *   S = scale q k^T over the keys that are seen;  P = softmax(S);  out = (P o keep / (1 - p)) v
+ * A key is seen where key_mask[b * key_mask_stride + key] != 0 (NULL: all) and key < key_lengths[b] (device
+ * int32, cut to [0, keys]; NULL: keys).  What masked keys and values hold is not read into any result (NaN
+ * and infinities included).  A query that sees no key gets out = 0 and lse = -inf, and no gradient.
+ * Dropout: weight (b, h, query, key) is element ((b heads + h) queries + query) * pitch + key, pitch = keys
+ * rounded up to 8, of pmsst_dropout_forward's numbering, with its p and rng.
+ * 16-bit types: products of 16-bit operands with fp32 sums; the weights (and their gradient) are rounded
+ * once to 16 bits for the second product.  No atomics: results are the same bit for bit on every run.
+ */
+
+/* Bytes of workspace of the forward on the current device (0 unless few rows meet many keys). */
+size_t pmsst_cross_attention_forward_workspace_size(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                                    int64_t kv_heads, int64_t head_dim, int dtype);
+/* out[batch, queries, heads, head_dim] dense; lse[batch, heads, queries] = log sum exp(S), fp32, may be NULL. */
+int pmsst_cross_attention_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                  const void* v, const int64_t* v_strides, const uint8_t* key_mask,
+                                  int64_t key_mask_stride, const int32_t* key_lengths, void* out, float* lse,
+                                  int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
+                                  int64_t head_dim, double scale, double dropout_p, const int64_t* rng, int dtype,
+                                  void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

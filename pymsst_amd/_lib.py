@@ -25,6 +25,7 @@ _CTYPES = {
     "int": ctypes.c_int,
     "int64_t": ctypes.c_int64,
     "size_t": ctypes.c_size_t,
+    "double": ctypes.c_double,
     "void": None,
 }
 

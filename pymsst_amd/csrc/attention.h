@@ -1,0 +1,361 @@
+// Shared pieces of the cross attention kernels (cross_attention.hip, cross_attention_bwd.hip).
+//
+// Rows: the queries of one (batch, key head) pair, r = n * group + g for query n and query head
+// hk * group + g, so heads that share a key head share its tiles.  A wave owns 32 rows (or, where the
+// keys' gradients are summed, 32 keys) and multiplies 32 x 32 tiles on the matrix cores.
+//
+// Products run "transposed": a tile of scores is computed as K Q^T, keys down and rows across, because
+// lane l of a 32x32 result holds column l % 32 and rows 8 a + 4 (l / 32) + c (a, c = 0..3, register
+// 4 a + c).  Each lane then owns one query and 16 keys: the softmax reduces inside a lane and once across
+// the two halves, and its statistics are one register each.  With the K rows fed in the order key_row()
+// gives, those 16 keys are 8 + 8 consecutive ones in exactly the places the next product wants its second
+// operand (16-bit: column l % 32, k = 8 (l / 32) + 0..7 of each 16; fp32: any k per half), so P never leaves
+// its registers.
+//
+// LDS tiles hold whole rows of the head dimension (DB bytes, zero-filled past head_dim), their 16-byte
+// units XOR-swizzled by swz(row); see swz.
+#pragma once
+
+#include <algorithm>
+
+#include "common.h"
+#include "gemm.h"
+#include "mfma.h"
+#include "philox.h"
+
+namespace pmsst {
+namespace attn {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kInf = __builtin_inff();
+
+// Element strides {batch, position, head} of a [B, N, H, D] tensor whose last axis is dense.
+struct Strides {
+  int64_t b, n, h;
+};
+
+struct Shape {
+  int32_t B, N, M, H, Hk, D;
+  int32_t G;      // H / Hk
+  int32_t R;      // rows of one (batch, key head): N * G
+  FastDiv by_g;
+};
+
+struct KeyMask {
+  const uint8_t* mask;     // [B, M], 0 = not attended; NULL: all
+  int64_t stride;          // between batch rows
+  const int32_t* lengths;  // [B]; NULL: M
+};
+
+// The 16-byte unit u of LDS row r sits at unit u ^ swz(r).  A b128 fragment read takes one unit of 16 rows
+// that differ in r % 16 each cycle, a transpose read 64 bytes (an aligned group of 4 units) of rows
+// 4 i .. 4 i + 3; 64 banks hold 256 bytes, so rows that share r % (256 / DB) must differ in the swizzle, and
+// of four consecutive rows those that start on the same bank in its group bits (the upper ones).
+template <int DB>
+__device__ __forceinline__ constexpr int swz(int r) {
+  if constexpr (DB == 64) return (r >> 2) & 3;
+  else if constexpr (DB == 128) return (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 3) & 1);
+  else return ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+// Key (inside 32) that row `rho` of a score tile's first operand holds.  Result register r of half h is row
+// 8 (r / 4) + 4 h + r % 4, so a lane's registers 0-7 and 8-15 are the 8 consecutive keys 8 h + 0..7 of
+// either 16: one operand fragment of a 16-bit product, and one block of the dropout's bits.
+__device__ __forceinline__ constexpr int key_row(int rho) {
+  return (rho & 16) | ((rho & 4) << 1) | ((rho & 8) >> 1) | (rho & 3);
+}
+// Key of register r, without the half's 8 h.
+__device__ __forceinline__ constexpr int reg_key(int r) { return 16 * (r >> 3) + (r & 7); }
+
+// acc += A (32 rows) B^T (32 columns) over the 32 bytes of k that a 16-byte fragment per lane spans.
+template <typename T>
+__device__ __forceinline__ f32x16_t mma(const u32x4_t& a, const u32x4_t& b, f32x16_t acc) {
+  if constexpr (std::is_same<T, bf16>::value) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), acc,
+                                                   0, 0, 0);
+  } else if constexpr (std::is_same<T, f16>::value) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), acc, 0,
+                                                  0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t ai = a[i], bi = b[i];
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, ai), __builtin_bit_cast(float, bi), acc, 0, 0,
+                                                 0);
+    }
+    return acc;
+  }
+}
+
+// The other half's value (lane l ^ 32) combined with this lane's.
+__device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, kWave)); }
+__device__ __forceinline__ float half_sum(float v) { return v + __shfl_xor(v, 32, kWave); }
+
+// Two fp32 rounded to nearest into one register of 16-bit values.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  typedef T v2 __attribute__((ext_vector_type(2)));
+  const v2 v{static_cast<T>(lo), static_cast<T>(hi)};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// Eight score-tile registers (one 16-key step of a lane) as the second operand of the next product.
+template <typename T>
+__device__ __forceinline__ u32x4_t pack8(const f32x16_t& p, int step) {
+  return u32x4_t{pack2<T>(p[8 * step], p[8 * step + 1]), pack2<T>(p[8 * step + 2], p[8 * step + 3]),
+                 pack2<T>(p[8 * step + 4], p[8 * step + 5]), pack2<T>(p[8 * step + 6], p[8 * step + 7])};
+}
+
+// Eight elements (16-bit) or four (fp32) of a 16-byte unit.
+template <typename T>
+__device__ __forceinline__ void unpack(const u32x4_t& u, float (&o)[16 / sizeof(T)]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = u[i];
+    if constexpr (std::is_same<T, bf16>::value) {
+      o[2 * i] = __builtin_bit_cast(float, w << 16);
+      o[2 * i + 1] = __builtin_bit_cast(float, w & 0xFFFF0000u);
+    } else if constexpr (std::is_same<T, f16>::value) {
+      o[2 * i] = static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(w)));
+      o[2 * i + 1] = static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(w >> 16)));
+    } else {
+      o[i] = __builtin_bit_cast(float, w);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- LDS fragments
+
+// Fragment s (32 bytes of k) of tile row `row`: this lane's unit 2 s + h.
+template <int DB>
+__device__ __forceinline__ u32x4_t row_frag(const char* tile, int row, int s, int h) {
+  return *reinterpret_cast<const u32x4_t*>(tile + row * DB + 16 * ((2 * s + h) ^ swz<DB>(row)));
+}
+
+// Transposed tile as first operand (16-bit): the product's rows are the head-dimension columns 32 dt + 0..31,
+// its k the tile rows k0 + 8 h + 0..7 by two transpose reads; the columns of a 16-lane group come in the order
+// 0-3, 8-11, 4-7, 12-15, so that a result lane holds 8 consecutive ones.
+template <int DB>
+__device__ __forceinline__ u32x4_t col_frag(const char* tile, int k0, int dt, int lane) {
+  const int j = lane & 15, h = lane >> 5;
+  const int row = k0 + 8 * h + (j >> 2);
+  const int unit = 4 * dt + 2 * ((lane >> 4) & 1) + (j & 1);
+  const int byte = 8 * ((j >> 1) & 1);
+  typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+  const char* p0 = tile + row * DB + 16 * (unit ^ swz<DB>(row)) + byte;
+  const char* p1 = tile + (row + 4) * DB + 16 * (unit ^ swz<DB>(row + 4)) + byte;
+  const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0));
+  const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p1));
+  const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+  return u32x4_t{a.x, a.y, b.x, b.y};
+}
+
+// acc[dt] += (tile rows sub*32 .. + 31)^T * p, for every 32 columns of the head dimension: p is a score tile
+// whose k index is the tile's row.
+template <typename T, int DP>
+__device__ __forceinline__ void mma_cols(const char* tile, int sub, const f32x16_t& p, f32x16_t (&acc)[DP / 32], int lane) {
+  constexpr int DB = DP * sizeof(T);
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const u32x4_t b = pack8<T>(p, s);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = mma<T>(col_frag<DB>(tile, 32 * sub + 16 * s, dt, lane), b, acc[dt]);
+    }
+  } else {
+    const int h = lane >> 5, d = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 32 * sub + reg_key(r) + 8 * h;
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) {
+        const float a = *reinterpret_cast<const float*>(tile + row * DB + 16 * ((8 * dt + (d >> 2)) ^ swz<DB>(row)) +
+                                                        4 * (d & 3));
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[dt], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// score += (tile rows sub*32 + key_row(l % 32)) * frag^T
+template <typename T, int DP>
+__device__ __forceinline__ f32x16_t mma_rows(const char* tile, int sub, const u32x4_t (&frag)[DP * sizeof(T) / 32], int lane) {
+  constexpr int DB = DP * sizeof(T);
+  const int row = 32 * sub + key_row(lane & 31);
+  f32x16_t acc{};
+#pragma unroll
+  for (int s = 0; s < DB / 32; ++s) acc = mma<T>(row_frag<DB>(tile, row, s, lane >> 5), frag[s], acc);
+  return acc;
+}
+
+// ---------------------------------------------------------------- global access
+
+// A row's fragments from global memory: unit 2 s + h of each 32 bytes; zero past head_dim or where !valid.
+template <typename T, int DP>
+__device__ __forceinline__ void load_frags(const T* row, bool valid, int d_units, int h,
+                                           u32x4_t (&f)[DP * sizeof(T) / 32]) {
+  constexpr int NS = DP * sizeof(T) / 32;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    f[s] = u32x4_t{0, 0, 0, 0};
+    if (valid && 2 * s + h < d_units) f[s] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const char*>(row) + 32 * s + 16 * h);
+  }
+}
+
+// BK rows of a tile through registers: fetch() issues the loads (rows past the end are clamped, never
+// branched on), commit() zeroes what is not to be seen and writes the tile.
+template <typename T, int DP, int BK, int THREADS>
+struct Tile {
+  static constexpr int DB = DP * sizeof(T);
+  static constexpr int UNITS = DB / 16;
+  static constexpr int CH = BK * UNITS / THREADS;
+  static constexpr int STEP = THREADS / UNITS;  // rows between a thread's units
+  static_assert(CH >= 1 && CH * THREADS == BK * UNITS && THREADS % UNITS == 0, "whole units per thread");
+  u32x4_t reg[CH];
+
+  // at(i): element offset of tile row i's first element, for rows clamped below `rows` (> 0)
+  template <typename F>
+  __device__ __forceinline__ void fetch(const T* base, int row0, int rows, int d_units, F at) {
+    const int u = threadIdx.x % UNITS;
+    const int ub = u < d_units ? 16 * u : 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      int row = row0 + static_cast<int>(threadIdx.x) / UNITS + i * STEP;
+      row = row < rows ? row : rows - 1;
+      reg[i] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const char*>(base + at(row)) + ub);
+    }
+  }
+
+  __device__ __forceinline__ void commit(char* tile, uint64_t seen, int d_units) {
+    const int u = threadIdx.x % UNITS;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int row = static_cast<int>(threadIdx.x) / UNITS + i * STEP;
+      const bool ok = u < d_units && ((seen >> row) & 1);
+      const u32x4_t v = ok ? reg[i] : u32x4_t{0, 0, 0, 0};
+      *reinterpret_cast<u32x4_t*>(tile + row * DB + 16 * (u ^ swz<DB>(row))) = v;
+    }
+  }
+};
+
+// Bits of BK <= 64 rows from row0 that lie below `rows`.
+__device__ __forceinline__ uint64_t range_bits(int row0, int rows) {
+  const int left = rows - row0;
+  return left >= 64 ? ~uint64_t{0} : left <= 0 ? 0 : (uint64_t{1} << left) - 1;
+}
+
+// Keys of batch row b that count: its length (cut to [0, M]) and its row of the mask.
+__device__ __forceinline__ int key_count(const KeyMask& km, int b, int M) {
+  if (km.lengths == nullptr) return M;
+  const int len = km.lengths[b];
+  return len < 0 ? 0 : len > M ? M : len;
+}
+
+// The 64-bit word of a tile's seen keys, for this lane: bit reg_key(r) of the result is register r of
+// sub-tile `sub`.
+__device__ __forceinline__ uint32_t lane_bits(uint64_t seen, int sub, int h) {
+  return static_cast<uint32_t>(seen >> (32 * sub)) >> (8 * h);
+}
+
+// Stores a transposed accumulator (rows = head dimension, columns = positions): lane's position row at `row`.
+template <typename T, int DP>
+__device__ __forceinline__ void store_cols(T* row, const f32x16_t (&acc)[DP / 32], float scale, int d, int h) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int at = 32 * dt + 16 * j + 8 * h;
+        if (at < d) {
+          float o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = acc[dt][8 * j + i] * scale;
+          store_pack<T, 8>(row + at, o);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const int at = 32 * dt + 8 * a + 4 * h;
+        if (at < d) {
+          float o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = acc[dt][4 * a + i] * scale;
+          store_pack<T, 4>(row + at, o);
+        }
+      }
+    }
+  }
+}
+
+// The same, unrounded, into a partial sum's fp32 row; T is the type whose column order the accumulator has.
+template <typename T, int DP>
+__device__ __forceinline__ void store_cols_f32(float* row, const f32x16_t (&acc)[DP / 32], float scale, int d, int h) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt) {
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int at = 32 * dt + (sizeof(T) == 2 ? reg_key(4 * a) + 8 * h : 8 * a + 4 * h);
+      if (at < d) {
+        float o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = acc[dt][4 * a + i] * scale;
+        store_pack<float, 4>(row + at, o);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- block numbering
+// Blocks of one (batch, key head) share its keys: they run on one XCD (the hardware deals block i to XCD
+// i % 8) where the pairs fill the XCDs evenly; few pairs are spread block by block instead.
+struct Grid {
+  uint32_t pairs;  // batch * key heads
+  uint32_t per;    // blocks of a pair
+  uint32_t by_xcd;
+  FastDiv by_per;
+};
+
+inline Grid make_grid(int64_t pairs, int64_t per) {
+  Grid g;
+  g.pairs = static_cast<uint32_t>(pairs);
+  g.per = static_cast<uint32_t>(per);
+  g.by_xcd = pairs % 8 == 0 || pairs >= 64;
+  g.by_per = FastDiv(g.per);
+  return g;
+}
+inline int64_t grid_blocks(const Grid& g) {
+  return (g.by_xcd ? (int64_t{g.pairs} + 7) / 8 * 8 : int64_t{g.pairs}) * g.per;
+}
+// (pair, block of the pair); false: past the last pair.
+__device__ __forceinline__ bool locate(const Grid& g, uint32_t& pair, uint32_t& sub) {
+  const uint32_t x = blockIdx.x;
+  if (g.by_xcd) {
+    const uint32_t i = x >> 3, octet = g.by_per.div(i);
+    sub = i - octet * g.per;
+    pair = octet * 8 + (x & 7);
+  } else {
+    pair = g.by_per.div(x);
+    sub = x - pair * g.per;
+  }
+  return pair < g.pairs;
+}
+
+// ---------------------------------------------------------------- dropout of the weights
+// Weight (b, head, n, key) is element ((b H + head) N + n) * pitch + key of the dropout's numbering, pitch =
+// M rounded up to 8: a lane's 8 consecutive keys are one Philox block.
+__device__ __forceinline__ uint64_t drop_row(const Shape& s, int b, int head, int n) {
+  return ((static_cast<uint64_t>(b) * s.H + head) * s.N + n) * ((static_cast<uint32_t>(s.M) + 7) / 8);
+}
+
+// Host checks, in cross_attention.hip.
+int make_shape(const char* what, int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
+               int64_t head_dim, int dtype, Shape& s);
+int make_strides(const char* what, const void* p, const int64_t* strides, int64_t positions, int64_t heads, int64_t dim,
+                 int dtype, Strides& out);
+
+}  // namespace attn
+}  // namespace pmsst

@@ -548,6 +548,139 @@ class HipFusedExtension:
         _req(out_layout in ("bhnd", "bnhd"), f"unsupported out_layout {out_layout!r}")
         return list(self._gate_bwd(grad_out, attn, x, weight, gate, out_layout))
 
+    # ------------------------------------------------------------------ cross attention
+
+    def _attention_operand(self, t):
+        """``t`` with a dense last axis and whole 16 bytes between rows (else a dense copy), and its strides."""
+        unit = 16 // t.element_size()
+        st = t.stride()
+        if st[3] != 1 or st[0] % unit or st[1] % unit or st[2] % unit or t.data_ptr() % 16:
+            t = t.contiguous()
+            if t.data_ptr() % 16:
+                t = t.clone()
+            st = t.stride()
+        return t, (ctypes.c_int64 * 3)(*st[:3])
+
+    def _attention_check(self, q, k, v, key_mask, key_lengths, scale, dropout_p, rng):
+        _req(q.is_cuda and q.dim() == 4, "q must be a CUDA tensor of shape [B, N, H, D]")
+        _req(k.dim() == 4 and v.dim() == 4, "k and v must have shape [B, M, Hk, D]")
+        _req(k.device == q.device and v.device == q.device, "q, k and v must be on one device")
+        _req(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one dtype")
+        b, n, h, d = q.shape
+        m, hk = k.shape[1], k.shape[2]
+        _req(v.shape == k.shape and k.shape[0] == b and k.shape[3] == d, "k and v must have shape [B, M, Hk, D]")
+        _req(hk > 0 and h % hk == 0, "the key heads must divide the query heads")
+        _req(d % 8 == 0 and 8 <= d <= 128, "the head dimension must be a multiple of 8 in [8, 128]")
+        stride = 0
+        if key_mask is not None:
+            _req(key_mask.device == q.device and key_mask.dtype in (torch.bool, torch.uint8) and key_mask.shape == (b, m),
+                 "key_mask must be a bool tensor of shape [B, M] on q's device")
+            if key_mask.stride(1) != 1:
+                key_mask = key_mask.contiguous()
+            stride = key_mask.stride(0)
+        if key_lengths is not None:
+            _req(key_lengths.device == q.device and key_lengths.dtype == torch.int32 and key_lengths.shape == (b,),
+                 "key_lengths must be an int32 tensor of shape [B] on q's device")
+            key_lengths = key_lengths.contiguous()
+        scale = d**-0.5 if scale is None else float(scale)
+        _req(0.0 < scale < 1e30, "scale must be positive")
+        self._dropout_check(dropout_p, rng, q.device)
+        return key_mask, stride, key_lengths, scale
+
+    def cross_attention_forward(self, q, k, v, key_mask=None, key_lengths=None, scale=None, dropout_p: float = 0.0,
+                                rng=None, need_lse: bool = False):
+        """Build addition: ``softmax(scale q k^T) v`` of ``q[B, N, H, D]`` over ``k`` / ``v[B, M, Hk, D]`` (another
+        stream of any length, or the same one), returned as ``[out[B, N, H, D]]``, or ``[out, lse]`` with
+        ``need_lse`` (``lse[B, H, N]`` fp32, what the backward takes).
+
+        ``Hk`` divides ``H``: consecutive query heads share a key head.  Any strides (views of a fused
+        projection, expanded batches) are read in place if their rows are dense and whole 16 bytes apart.
+        ``key_mask``: bool ``[B, M]``, true where a key is attended to; ``key_lengths``: int32 ``[B]``; both may
+        be given.  What masked keys hold never reaches a result; a query without any key gets zeros.
+        ``scale``: ``D ** -0.5`` unless given.  ``dropout_p`` drops weights with the bits of
+        :meth:`dropout_forward` on a ``[B, H, N, M rounded up to 8]`` tensor and the same ``rng``.
+        Few rows (single queries) over many keys are split over the keys."""
+        key_mask, mask_stride, key_lengths, scale = self._attention_check(q, k, v, key_mask, key_lengths, scale, dropout_p,
+                                                                          rng)
+        code = dtype_code(q.dtype)
+        (q, qs), (k, ks), (v, vs) = self._attention_operand(q), self._attention_operand(k), self._attention_operand(v)
+        b, n, h, d = q.shape
+        m, hk = k.shape[1], k.shape[2]
+        out = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
+        lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device) if need_lse else None
+        with _DeviceGuard(q.device):
+            size = self._lib.pmsst_cross_attention_forward_workspace_size(b, n, m, h, hk, d, code)
+            ws = _workspace(size, q.device) if size else None
+            rc = self._lib.pmsst_cross_attention_forward(
+                _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(key_mask), mask_stride, _ptr(key_lengths), _ptr(out),
+                _ptr(lse), b, n, m, h, hk, d, scale, dropout_p, _ptr(rng), code, _ptr(ws), size, _stream(q.device),
+            )
+        check(rc, "pmsst_cross_attention_forward")
+        return [out, lse] if need_lse else [out]
+
+    # ------------------------------------------------------------------ dropout
+
+    @staticmethod
+    def _dropout_check(p, rng, device) -> None:
+        _req(0.0 <= p < 1.0, "the dropout probability must lie in [0, 1)")
+        if rng is None:
+            _req(p == 0.0, "rng must be given where the dropout probability is not 0")
+        else:
+            _req(rng.is_cuda and rng.device == device and rng.dtype == torch.int64 and rng.shape == (2,)
+                 and rng.is_contiguous(), "rng must be an int64 CUDA tensor {seed, offset} on the input's device")
+
+    @staticmethod
+    def _dropout_activation(name) -> int:
+        if name is None or name == "none":
+            return 0  # PMSST_ACT_NONE
+        if name == "gelu":
+            return 2  # PMSST_ACT_GELU
+        raise ValueError(f"unsupported activation {name!r}")
+
+    def dropout_forward(self, x, p: float, rng, activation=None, residual=None):
+        """Build addition: ``dropout(act(x)) + residual`` in one pass, without a stored mask.
+
+        ``rng``: int64 CUDA tensor ``{seed, offset}``, read when the kernel runs; the same values give the
+        same mask, element ``e`` of ``x`` in row-major order being kept where its 16 bits of Philox4x32-7
+        are at least ``round(65536 p)`` (so a probability is held to 2^-16).  What is kept is divided by
+        the exact share of values that keep.  ``activation``: ``None`` or ``"gelu"`` (the exact one);
+        ``residual``: ``x``'s shape and dtype, or ``None``.  Arithmetic is fp32, rounded once."""
+        act = self._dropout_activation(activation)
+        _req(x.is_cuda, "x must be a CUDA tensor")
+        self._dropout_check(p, rng, x.device)
+        if residual is not None:
+            _req(residual.device == x.device and residual.shape == x.shape and residual.dtype == x.dtype,
+                 "residual must have x's shape, dtype and device")
+            residual = residual.contiguous()
+        x = x.contiguous()
+        out = torch.empty_like(x)
+        with _DeviceGuard(x.device):
+            rc = self._lib.pmsst_dropout_forward(_ptr(x), _ptr(residual), _ptr(out), x.numel(), p, _ptr(rng), act,
+                                                 dtype_code(x.dtype), _stream(x.device))
+        check(rc, "pmsst_dropout_forward")
+        return out
+
+    def dropout_backward(self, grad_out, p: float, rng, x=None, activation=None):
+        """Gradient of :meth:`dropout_forward`'s ``x`` (its mask drawn again from the same ``p`` and ``rng``
+        values; the residual's gradient is ``grad_out`` itself).  ``x``: the forward's input, needed with an
+        activation."""
+        act = self._dropout_activation(activation)
+        _req(grad_out.is_cuda, "grad_out must be a CUDA tensor")
+        self._dropout_check(p, rng, grad_out.device)
+        if act:
+            _req(x is not None and x.device == grad_out.device and x.shape == grad_out.shape
+                 and x.dtype == grad_out.dtype, "x must be the forward's input, in grad_out's shape, dtype and device")
+            x = x.contiguous()
+        else:
+            x = None
+        grad_out = grad_out.contiguous()
+        grad_x = torch.empty_like(grad_out)
+        with _DeviceGuard(grad_out.device):
+            rc = self._lib.pmsst_dropout_backward(_ptr(grad_out), _ptr(x), _ptr(grad_x), grad_out.numel(), p, _ptr(rng),
+                                                  act, dtype_code(grad_out.dtype), _stream(grad_out.device))
+        check(rc, "pmsst_dropout_backward")
+        return grad_x
+
     # ------------------------------------------------------------------ mel band rows
 
     @staticmethod
