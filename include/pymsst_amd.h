@@ -428,6 +428,20 @@ int pmsst_cross_attention_forward(const void* q, const int64_t* q_strides, const
                                   int64_t head_dim, double scale, double dropout_p, const int64_t* rng, int dtype,
                                   void* workspace, size_t workspace_bytes, void* stream);
 
+/* Bytes of workspace of the backward on the current device. */
+size_t pmsst_cross_attention_backward_workspace_size(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                                     int64_t kv_heads, int64_t head_dim, int dtype);
+/* Gradients of the forward (same masks, scale, dropout_p and rng values) from its dense out and its lse:
+ * grad_q[batch, queries, heads, head_dim], grad_k and grad_v[batch, keys, kv_heads, head_dim], dense, fully
+ * written (zeros for keys that are not seen; heads that share a key head are summed). */
+int pmsst_cross_attention_backward(const void* grad_out, const int64_t* grad_out_strides, const void* q,
+                                   const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                   const int64_t* v_strides, const void* out, const float* lse, const uint8_t* key_mask,
+                                   int64_t key_mask_stride, const int32_t* key_lengths, void* grad_q, void* grad_k,
+                                   void* grad_v, int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                   int64_t kv_heads, int64_t head_dim, double scale, double dropout_p, const int64_t* rng,
+                                   int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -153,6 +153,12 @@ __device__ __forceinline__ u32x4_t col_frag(const char* tile, int k0, int dt, in
   return u32x4_t{a.x, a.y, b.x, b.y};
 }
 
+// fp32 tiles are read by as many instructions as the matrix cores run: nothing is scheduled across this, or
+// the reads of a whole tile would be hoisted and spill.
+__device__ __forceinline__ void hold(bool here) {
+  if (here) __builtin_amdgcn_sched_barrier(0);
+}
+
 // acc[dt] += (tile rows sub*32 .. + 31)^T * p, for every 32 columns of the head dimension: p is a score tile
 // whose k index is the tile's row.
 template <typename T, int DP>
@@ -176,6 +182,7 @@ __device__ __forceinline__ void mma_cols(const char* tile, int sub, const f32x16
                                                         4 * (d & 3));
         acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[dt], 0, 0, 0);
       }
+      hold(r % 2 == 1);
     }
   }
 }
@@ -187,7 +194,10 @@ __device__ __forceinline__ f32x16_t mma_rows(const char* tile, int sub, const u3
   const int row = 32 * sub + key_row(lane & 31);
   f32x16_t acc{};
 #pragma unroll
-  for (int s = 0; s < DB / 32; ++s) acc = mma<T>(row_frag<DB>(tile, row, s, lane >> 5), frag[s], acc);
+  for (int s = 0; s < DB / 32; ++s) {
+    acc = mma<T>(row_frag<DB>(tile, row, s, lane >> 5), frag[s], acc);
+    if constexpr (sizeof(T) == 4) hold(s % 2 == 1);
+  }
   return acc;
 }
 
@@ -350,6 +360,9 @@ __device__ __forceinline__ bool locate(const Grid& g, uint32_t& pair, uint32_t& 
 __device__ __forceinline__ uint64_t drop_row(const Shape& s, int b, int head, int n) {
   return ((static_cast<uint64_t>(b) * s.H + head) * s.N + n) * ((static_cast<uint32_t>(s.M) + 7) / 8);
 }
+
+// Head dimension a kernel is built for.
+inline int padded_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 // Host checks, in cross_attention.hip.
 int make_shape(const char* what, int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,

@@ -211,13 +211,14 @@ struct FwdPlan {
   int64_t row_tiles, splits, tiles_per_split;
 };
 
-// Waves of a block: 2 where that covers the rows (a block of 4 would idle), else 4.  Splits: as many as give
+// Waves of a block: 2 where that covers the rows (half a block of 4 would idle; fp32 rows of 512 bytes keep 4,
+// whose lanes hold half as much of a tile on its way), else 4.  Splits: as many as give
 // every CU two blocks, of at least 256 keys each.
 FwdPlan plan_forward(const Shape& s, int dtype) {
   FwdPlan p;
-  p.nw = s.R <= 64 ? 2 : 4;
-  const int dp = s.D <= 32 ? 32 : s.D <= 64 ? 64 : 128;
-  p.bk = dp * static_cast<int>(dtype_size(dtype)) == 512 ? 32 : 64;
+  const bool wide = padded_dim(s.D) * static_cast<int>(dtype_size(dtype)) == 512;
+  p.nw = s.R <= 64 && !wide ? 2 : 4;
+  p.bk = wide ? 32 : 64;
   p.row_tiles = (int64_t{s.R} + 32 * p.nw - 1) / (32 * p.nw);
   const int64_t tiles = std::max<int64_t>(1, (int64_t{s.M} + p.bk - 1) / p.bk);
   const int64_t blocks = int64_t{s.B} * s.Hk * p.row_tiles, want = 2 * num_cus();
@@ -238,7 +239,10 @@ int launch_fwd(const FwdArgs& a, bool drop, hipStream_t stream) {
 
 template <typename T, int DP>
 int launch_fwd(const FwdArgs& a, const FwdPlan& p, bool drop, hipStream_t stream) {
-  return p.nw == 2 ? launch_fwd<T, DP, 2>(a, drop, stream) : launch_fwd<T, DP, 4>(a, drop, stream);
+  if constexpr (DP * sizeof(T) != 512) {
+    if (p.nw == 2) return launch_fwd<T, DP, 2>(a, drop, stream);
+  }
+  return launch_fwd<T, DP, 4>(a, drop, stream);
 }
 
 template <typename T>

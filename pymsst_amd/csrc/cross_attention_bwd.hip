@@ -1,0 +1,608 @@
+// Cross attention backward.  With P the weights, recomputed from the saved lse, f the dropout's factor of each
+// weight (keep / (1 - p)) and dO the output's gradient:
+//   D  = rowsum(dO o O)              dV = (P o f)^T dO
+//   dS = P o ((dO V^T) o f - D)      dQ = scale dS K,   dK = scale dS^T Q
+//
+// Two kernels, so that every sum has one owner and no atomic is needed:
+//  * attn_dq_kernel: a wave owns 32 rows (its Q and dO in registers) and passes over the key tiles; it also
+//    writes D, which it forms from O and dO;
+//  * attn_dkv_kernel: a wave owns 32 keys (its K and V in registers) and passes over the row tiles of every
+//    query head that shares the key head.
+// Both recompute S and dO V^T (7 products in all; one kernel would need 5 and atomics, or dQ partials, to sum dQ).
+// Few owners over a long axis are split over it: fp32 partial sums in the workspace, added in a fixed order.
+//
+// fp16 only: P and dS are rounded to 16 bits as operands, and fp16 loses digits below 2^-14.  Both are scaled by
+// powers of two that cannot overflow, from the bound |dO V^T o f - D| <= 2 max|V| |dO row|_1 / (1 - p); a small
+// kernel before the others takes the maxima.
+#include "attention.h"
+
+namespace pmsst {
+namespace {
+
+using namespace attn;
+
+struct BwdArgs {
+  const void *q, *k, *v, *out, *dout;
+  Strides qs, ks, vs, os, gs;
+  KeyMask km;
+  const float* lse;  // [B, H, N]
+  void *dq, *dk, *dv;
+  float* delta;                // [pairs, R]
+  float *vmax, *l1;            // fp16: [pairs, kParts] maxima of |V| over the seen keys and of |dO row|_1
+  float *part_q, *part_k, *part_v;  // partial sums [splits, pairs, R or M, D], NULL: not split
+  Shape s;
+  Grid grid;
+  uint32_t tiles;              // owner tiles (rows or keys) of a pair; grid.per = tiles * splits
+  int32_t tiles_per_split;
+  float scale, scale_log2;
+  Dropout drop;
+};
+
+constexpr int kParts = 16;
+
+// Rows of a passing tile: 64, or 32 where its two LDS tiles, twice, would pass 64 KB.
+template <typename T, int DP>
+constexpr int bwd_tile() { return DP * sizeof(T) == 512 ? 32 : 64; }
+
+// Largest power of two that keeps bound * 2^e <= 2^top (0 where the bound says nothing).
+__device__ __forceinline__ int scale_exponent(float bound, int top) {
+  if (!(bound > 0.f) || bound > 3e38f) return 0;
+  int x;
+  frexpf(bound, &x);
+  const int e = top - x;
+  return e < -100 ? -100 : e > 100 ? 100 : e;
+}
+
+__device__ __forceinline__ float parts_max(const float* parts) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) m = fmaxf(m, parts[i]);
+  return m;
+}
+
+// ---------------------------------------------------------------- fp16 bounds
+
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bound_kernel(BwdArgs a) {
+  __shared__ float red[2][4];
+  const uint32_t pair = blockIdx.x / kParts;
+  const int part = static_cast<int>(blockIdx.x % kParts);
+  const Shape& s = a.s;
+  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
+  const int units = s.D / 8, lane_u = threadIdx.x & 15, row_u = threadIdx.x >> 4;  // 16 lanes a row
+  const int count = key_count(a.km, b, s.M);
+  const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
+  const T* gb = static_cast<const T*>(a.dout) + b * a.gs.b;
+  float vm = 0.f, lm = 0.f;
+  for (int64_t m = part * 16 + row_u; m < count; m += 16 * kParts) {
+    if (a.km.mask && a.km.mask[b * a.km.stride + m] == 0) continue;
+    if (lane_u < units) {
+      float x[8];
+      load_pack<T, 8>(vb + m * a.vs.n + 8 * lane_u, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vm = fmaxf(vm, fabsf(x[i]));
+    }
+  }
+  for (int64_t r = part * 16 + row_u; r < s.R; r += 16 * kParts) {
+    const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(r))), head = hk * s.G + static_cast<int>(r) - n * s.G;
+    float sum = 0.f;
+    if (lane_u < units) {
+      float x[8];
+      load_pack<T, 8>(gb + n * a.gs.n + head * a.gs.h + 8 * lane_u, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += fabsf(x[i]);
+    }
+    lm = fmaxf(lm, group_sum(sum, 16));
+  }
+  for (int off = 32; off > 0; off >>= 1) {
+    vm = fmaxf(vm, __shfl_xor(vm, off, kWave));
+    lm = fmaxf(lm, __shfl_xor(lm, off, kWave));
+  }
+  if ((threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = vm;
+    red[1][threadIdx.x >> 6] = lm;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    a.vmax[pair * kParts + part] = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    a.l1[pair * kParts + part] = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+  }
+}
+
+// ---------------------------------------------------------------- dQ
+
+template <typename T, int DP, int NW, bool DROP>
+__global__ __launch_bounds__(64 * NW) void attn_dq_kernel(BwdArgs a) {
+  constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
+  constexpr int BK = bwd_tile<T, DP>(), SUBS = BK / 32;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][BK * DB];
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+  uint32_t pair, sub_block;
+  if (!locate(a.grid, pair, sub_block)) return;
+  const uint32_t split = sub_block / a.tiles, row_tile = sub_block - split * a.tiles;
+  const Shape& s = a.s;
+  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
+  const int d_units = s.D * static_cast<int>(sizeof(T)) / 16;
+
+  const int r = static_cast<int>(row_tile) * 32 * NW + wave * 32 + (lane & 31);
+  const bool row_ok = r < s.R;
+  const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(r))), head = hk * s.G + (r - n * s.G);
+  u32x4_t qf[NS], gf[NS];
+  float delta = 0.f, l1 = 0.f;
+  load_frags<T, DP>(static_cast<const T*>(a.q) + b * a.qs.b + (row_ok ? n * a.qs.n + head * a.qs.h : 0), row_ok, d_units,
+                    h, qf);
+  load_frags<T, DP>(static_cast<const T*>(a.dout) + b * a.gs.b + (row_ok ? n * a.gs.n + head * a.gs.h : 0), row_ok,
+                    d_units, h, gf);
+  {
+    u32x4_t of[NS];
+    load_frags<T, DP>(static_cast<const T*>(a.out) + b * a.os.b + (row_ok ? n * a.os.n + head * a.os.h : 0), row_ok,
+                      d_units, h, of);
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      float x[E], y[E];
+      unpack<T>(of[i], x);
+      unpack<T>(gf[i], y);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        delta = fmaf(x[j], y[j], delta);
+        if constexpr (std::is_same<T, f16>::value) l1 += fabsf(y[j]);
+      }
+    }
+    delta = half_sum(delta);
+  }
+  if (row_ok && h == 0 && split == 0) a.delta[static_cast<int64_t>(pair) * s.R + r] = delta;
+  // -lse in log2 units: a row that sees no key (and one past the end) has no weight
+  float base = -kInf;
+  if (row_ok) {
+    const float lse = a.lse[(static_cast<int64_t>(b) * s.H + head) * s.N + n];
+    base = lse == -kInf ? -kInf : -lse * kLog2e;
+  }
+  int e = 0;
+  if constexpr (std::is_same<T, f16>::value) {
+    e = scale_exponent(2.f * half_sum(l1) * parts_max(a.vmax + pair * kParts) * a.drop.factor, 15);
+    base += static_cast<float>(e);
+  }
+
+  const int count = key_count(a.km, b, s.M);
+  const int all_tiles = (count + BK - 1) / BK;
+  const int t0 = static_cast<int>(split) * a.tiles_per_split;
+  const int t1 = min(all_tiles, t0 + a.tiles_per_split);
+  const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
+  const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
+  const uint8_t* mask = a.km.mask ? a.km.mask + b * a.km.stride : nullptr;
+  PhiloxKey key{};
+  uint64_t drop0 = 0;
+  if constexpr (DROP) {
+    key = philox_key(a.drop.rng);
+    drop0 = drop_row(s, b, head, n);
+  }
+
+  f32x16_t acc[DT]{};
+  Tile<T, DP, BK, 64 * NW> kt, vt;
+  uint8_t seen_byte = 1;
+  auto fetch = [&](int t) {
+    const int key0 = t * BK;
+    if (mask) seen_byte = mask[min(key0 + lane, count - 1)];
+    kt.fetch(kb, key0, count, d_units, [&](int i) { return i * a.ks.n; });
+    vt.fetch(vb, key0, count, d_units, [&](int i) { return i * a.vs.n; });
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
+    char* kl = lds[t & 1][0];
+    char* vl = lds[t & 1][1];
+    uint64_t seen = range_bits(t * BK, count);
+    if (mask) seen &= __ballot(seen_byte != 0);
+    if constexpr (BK == 32) seen &= 0xFFFFFFFFu;
+    constexpr uint64_t kAll = BK == 64 ? ~uint64_t{0} : 0xFFFFFFFFu;
+    kt.commit(kl, seen, d_units);
+    vt.commit(vl, seen, d_units);
+    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
+    if (seen == 0) continue;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      f32x16_t p = mma_rows<T, DP>(kl, u, qf, lane);
+      f32x16_t dp = mma_rows<T, DP>(vl, u, gf, lane);
+      if constexpr (DROP) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t w[4];
+          philox7(key, drop0 + static_cast<uint32_t>(t * (BK / 8) + 4 * u + 2 * j + h), w);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dp[8 * j + i] = philox_keep(w, i, a.drop.limit << 16) ? dp[8 * j + i] * a.drop.factor : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.scale_log2, base)) * (dp[i] - delta);
+      }
+      if (seen != kAll) {
+        const uint32_t bits = lane_bits(seen, u, h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = (bits >> reg_key(i)) & 1 ? p[i] : 0.f;
+      }
+      mma_cols<T, DP>(kl, u, p, acc, lane);
+    }
+  }
+  if (!row_ok) return;
+  const float out_scale = std::is_same<T, f16>::value ? ldexpf(a.scale, -e) : a.scale;
+  if (a.part_q) {
+    const int64_t at = (static_cast<int64_t>(split) * a.grid.pairs + pair) * s.R + r;
+    store_cols_f32<T, DP>(a.part_q + at * s.D, acc, out_scale, s.D, h);
+  } else {
+    const int64_t at = (static_cast<int64_t>(b) * s.N + n) * s.H + head;
+    store_cols<T, DP>(static_cast<T*>(a.dq) + at * s.D, acc, out_scale, s.D, h);
+  }
+}
+
+// ---------------------------------------------------------------- dK, dV
+
+template <typename T, int DP, int NW, bool DROP>
+__global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(BwdArgs a) {
+  constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
+  constexpr int BQ = bwd_tile<T, DP>(), SUBS = BQ / 32;
+  constexpr bool kHalf = std::is_same<T, f16>::value;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][BQ * DB];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][BQ];  // -lse (log2 units), D
+  __shared__ __attribute__((aligned(16))) uint32_t kept[DROP ? NW : 1][DROP ? 32 : 4];
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+  uint32_t pair, sub_block;
+  if (!locate(a.grid, pair, sub_block)) return;
+  const uint32_t split = sub_block / a.tiles, key_tile = sub_block - split * a.tiles;
+  const Shape& s = a.s;
+  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
+  const int d_units = s.D * static_cast<int>(sizeof(T)) / 16;
+  const int count = key_count(a.km, b, s.M);
+  const int block_key0 = static_cast<int>(key_tile) * 32 * NW;
+  const int key0 = block_key0 + wave * 32, ki = key0 + (lane & 31);
+  const bool seen = ki < count && (a.km.mask == nullptr || a.km.mask[b * a.km.stride + ki] != 0);
+
+  f32x16_t dk[DT]{}, dv[DT]{};
+  float k_scale = a.scale, v_scale = DROP ? a.drop.factor : 1.f;
+  if (block_key0 < count) {
+    u32x4_t kf[NS], vf[NS];
+    load_frags<T, DP>(static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h + (seen ? ki * a.ks.n : 0), seen, d_units, h, kf);
+    load_frags<T, DP>(static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h + (seen ? ki * a.vs.n : 0), seen, d_units, h, vf);
+    // P' = 2^shift P, dS' = P' 2^e (...): see the head of this file
+    constexpr float kShift = kHalf ? 14.f : 0.f;
+    float power = 1.f;
+    if constexpr (kHalf) {
+      const int e = scale_exponent(2.f * parts_max(a.l1 + pair * kParts) * parts_max(a.vmax + pair * kParts) * a.drop.factor,
+                                   1);
+      power = ldexpf(1.f, e);
+      k_scale = ldexpf(a.scale, -e - 14);
+      v_scale = ldexpf(v_scale, -14);
+    }
+    const float dp_scale = DROP ? a.drop.factor * power : power;
+
+    const int tiles = (s.R + BQ - 1) / BQ;
+    const int t0 = static_cast<int>(split) * a.tiles_per_split;
+    const int t1 = min(tiles, t0 + a.tiles_per_split);
+    const T* qb = static_cast<const T*>(a.q) + b * a.qs.b;
+    const T* gb = static_cast<const T*>(a.dout) + b * a.gs.b;
+    PhiloxKey key{};
+    if constexpr (DROP) key = philox_key(a.drop.rng);
+
+    Tile<T, DP, BQ, 64 * NW> qt, gt;
+    float stat_lse = 0.f, stat_delta = 0.f;
+    auto at = [&](int i, const Strides& st) {
+      const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(i)));
+      return n * st.n + (hk * s.G + (i - n * s.G)) * st.h;
+    };
+    auto fetch = [&](int t) {
+      const int row0 = t * BQ;
+      qt.fetch(qb, row0, s.R, d_units, [&](int i) { return at(i, a.qs); });
+      gt.fetch(gb, row0, s.R, d_units, [&](int i) { return at(i, a.gs); });
+      if (threadIdx.x < BQ) {
+        const int i = min(row0 + static_cast<int>(threadIdx.x), s.R - 1);
+        const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(i)));
+        stat_lse = a.lse[(static_cast<int64_t>(b) * s.H + hk * s.G + (i - n * s.G)) * s.N + n];
+        stat_delta = a.delta[static_cast<int64_t>(pair) * s.R + i];
+      }
+    };
+    // fp32 rows of 512 bytes leave no registers for the tile after this one (its products take 10 times as long
+    // as its loads)
+    constexpr bool kAhead = DB < 512;
+    if (kAhead && t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+      if (!kAhead) fetch(t);
+      char* ql = lds[t & 1][0];
+      char* gl = lds[t & 1][1];
+      float* base = stat[t & 1][0];
+      float* delta = stat[t & 1][1];
+      const uint64_t rows = range_bits(t * BQ, s.R);
+      qt.commit(ql, rows, d_units);
+      gt.commit(gl, rows, d_units);
+      if (threadIdx.x < BQ) {
+        const bool ok = ((rows >> threadIdx.x) & 1) && stat_lse != -kInf;
+        base[threadIdx.x] = ok ? kShift - stat_lse * kLog2e : -kInf;
+        delta[threadIdx.x] = ok ? stat_delta * power : 0.f;
+      }
+      __syncthreads();
+      if (kAhead && t + 1 < t1) fetch(t + 1);
+#pragma unroll
+      for (int u = 0; u < SUBS; ++u) {
+        if constexpr (DROP) {
+          // 32 rows x 4 blocks of 8 keys: a lane draws 2 of them, one byte of kept bits each
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int idx = lane + 64 * j, row = idx >> 2, blk = idx & 3;
+            const int i = min(t * BQ + 32 * u + row, s.R - 1);
+            const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(i)));
+            uint32_t w[4];
+            philox7(key, drop_row(s, b, hk * s.G + (i - n * s.G), n) + static_cast<uint32_t>(key0 / 8 + blk), w);
+            uint32_t bits = 0;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) bits |= philox_keep(w, c, a.drop.limit << 16) ? 1u << c : 0u;
+            reinterpret_cast<uint8_t*>(kept[wave])[idx] = static_cast<uint8_t>(bits);
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        hold(sizeof(T) == 4);
+        f32x16_t p = mma_rows<T, DP>(ql, u, kf, lane);
+        f32x16_t ds = mma_rows<T, DP>(gl, u, vf, lane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int row = reg_key(i) + 8 * h;
+          p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.scale_log2, base[32 * u + row]));
+          if constexpr (DROP) {
+            const bool keep = (kept[wave][row] >> (lane & 31)) & 1;
+            ds[i] = p[i] * ((keep ? ds[i] * dp_scale : 0.f) - delta[32 * u + row]);
+            p[i] = keep ? p[i] : 0.f;
+          } else {
+            ds[i] = p[i] * fmaf(ds[i], dp_scale, -delta[32 * u + row]);
+          }
+        }
+        if constexpr (DROP) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        hold(sizeof(T) == 4);
+        mma_cols<T, DP>(gl, u, p, dv, lane);
+        mma_cols<T, DP>(ql, u, ds, dk, lane);
+      }
+    }
+  }
+  if (ki >= s.M) return;
+  if (!seen) {
+    // nothing was learnt about a key that is not seen, whatever its columns of the tiles hold
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      dk[dt] = f32x16_t{};
+      dv[dt] = f32x16_t{};
+    }
+  }
+  if (a.part_k) {
+    const int64_t at = ((static_cast<int64_t>(split) * a.grid.pairs + pair) * s.M + ki) * s.D;
+    store_cols_f32<T, DP>(a.part_k + at, dk, k_scale, s.D, h);
+    store_cols_f32<T, DP>(a.part_v + at, dv, v_scale, s.D, h);
+  } else {
+    const int64_t at = ((static_cast<int64_t>(b) * s.M + ki) * s.Hk + hk) * s.D;
+    store_cols<T, DP>(static_cast<T*>(a.dk) + at, dk, k_scale, s.D, h);
+    store_cols<T, DP>(static_cast<T*>(a.dv) + at, dv, v_scale, s.D, h);
+  }
+}
+
+// ---------------------------------------------------------------- partial sums
+
+// out[b, position, head, d] = sum over splits of part[split, pair, row, d]; positions x group rows per pair
+// (group 1 for the keys).  A thread takes 4 columns.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, void* out, int splits, int64_t pairs,
+                                                       int32_t heads, int32_t kv_heads, int32_t group, int32_t positions,
+                                                       int32_t dim) {
+  const int64_t quads = dim / 4, rows = static_cast<int64_t>(positions) * group, total = pairs * rows * quads;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = i / quads, quad = i - row * quads, pair = row / rows, r = row - pair * rows;
+  const int64_t b = pair / kv_heads, hk = pair - b * kv_heads, n = r / group, head = hk * group + (r - n * group);
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < splits; ++k) {
+    float x[4];
+    load_pack<float, 4>(part + ((k * pairs * rows + row) * quads + quad) * 4, x);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] += x[c];
+  }
+  store_pack<T, 4>(static_cast<T*>(out) + ((b * positions + n) * heads + head) * dim + 4 * quad, o);
+}
+
+// ---------------------------------------------------------------- host
+
+struct BwdPlan {
+  int nw_q, nw_k;
+  int64_t q_tiles, q_splits, q_per, k_tiles, k_splits, k_per;
+};
+
+// Splits as in the forward: as many as give every CU two blocks, of at least 256 keys (rows) each.
+BwdPlan plan_backward(const Shape& s, int dtype) {
+  const bool wide = padded_dim(s.D) * static_cast<int>(dtype_size(dtype)) == 512;
+  const int64_t bk = wide ? 32 : 64;
+  const int64_t pairs = int64_t{s.B} * s.Hk, want = 2 * num_cus();
+  auto split = [&](int64_t owners, int64_t along, int64_t& splits, int64_t& per) {
+    const int64_t tiles = std::max<int64_t>(1, (along + bk - 1) / bk);
+    splits = 1;
+    if (owners < want) splits = std::max<int64_t>(1, std::min(want / owners, along / 256));
+    per = (tiles + splits - 1) / splits;
+    splits = (tiles + per - 1) / per;
+  };
+  BwdPlan p;
+  p.nw_q = s.R <= 64 && !wide ? 2 : 4;
+  p.nw_k = s.M <= 64 && !wide ? 2 : 4;
+  p.q_tiles = (int64_t{s.R} + 32 * p.nw_q - 1) / (32 * p.nw_q);
+  p.k_tiles = (int64_t{s.M} + 32 * p.nw_k - 1) / (32 * p.nw_k);
+  split(pairs * p.q_tiles, s.M, p.q_splits, p.q_per);
+  split(std::max<int64_t>(1, pairs * p.k_tiles), s.R, p.k_splits, p.k_per);
+  return p;
+}
+
+struct BwdSpace {
+  size_t delta, bound, part_q, part_k, total;
+};
+
+BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int dtype) {
+  const size_t pairs = static_cast<size_t>(s.B) * s.Hk;
+  BwdSpace w;
+  w.delta = align_up(pairs * s.R * 4, 256);
+  w.bound = dtype == PMSST_F16 ? align_up(pairs * kParts * 4, 256) : 0;
+  w.part_q = p.q_splits > 1 ? align_up(static_cast<size_t>(p.q_splits) * pairs * s.R * s.D * 4, 256) : 0;
+  w.part_k = p.k_splits > 1 ? align_up(static_cast<size_t>(p.k_splits) * pairs * s.M * s.D * 4, 256) : 0;
+  w.total = w.delta + 2 * w.bound + w.part_q + 2 * w.part_k;
+  return w;
+}
+
+template <typename T, int DP, int NW>
+int launch_dq(const BwdArgs& a, bool drop, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
+  if (drop) attn_dq_kernel<T, DP, NW, true><<<grid, 64 * NW, 0, stream>>>(a);
+  else attn_dq_kernel<T, DP, NW, false><<<grid, 64 * NW, 0, stream>>>(a);
+  return check_launch("attn_dq_kernel");
+}
+
+template <typename T, int DP>
+int launch_dq(const BwdArgs& a, int nw, bool drop, hipStream_t stream) {
+  if constexpr (DP * sizeof(T) != 512) {
+    if (nw == 2) return launch_dq<T, DP, 2>(a, drop, stream);
+  }
+  return launch_dq<T, DP, 4>(a, drop, stream);
+}
+
+template <typename T, int DP, int NW>
+int launch_dkv(const BwdArgs& a, bool drop, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
+  if (drop) attn_dkv_kernel<T, DP, NW, true><<<grid, 64 * NW, 0, stream>>>(a);
+  else attn_dkv_kernel<T, DP, NW, false><<<grid, 64 * NW, 0, stream>>>(a);
+  return check_launch("attn_dkv_kernel");
+}
+
+template <typename T, int DP>
+int launch_dkv(const BwdArgs& a, int nw, bool drop, hipStream_t stream) {
+  if constexpr (DP * sizeof(T) != 512) {
+    if (nw == 2) return launch_dkv<T, DP, 2>(a, drop, stream);
+  }
+  return launch_dkv<T, DP, 4>(a, drop, stream);
+}
+
+template <typename T>
+int launch_sum(const float* part, void* out, int64_t splits, const Shape& s, bool keys, hipStream_t stream) {
+  const int64_t pairs = int64_t{s.B} * s.Hk, rows = keys ? s.M : s.R;
+  const int64_t blocks = (pairs * rows * (s.D / 4) + 255) / 256;
+  attn_sum_kernel<T><<<dim3(static_cast<uint32_t>(blocks)), 256, 0, stream>>>(
+      part, out, static_cast<int>(splits), pairs, keys ? s.Hk : s.H, s.Hk, keys ? 1 : s.G, keys ? s.M : s.N, s.D);
+  return check_launch("attn_sum_kernel");
+}
+
+template <typename T, int DP>
+int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+  const bool drop = a.drop.limit != 0;
+  const int64_t pairs = int64_t{a.s.B} * a.s.Hk;
+  if constexpr (std::is_same<T, f16>::value) {
+    attn_bound_kernel<T><<<dim3(static_cast<uint32_t>(pairs * kParts)), 256, 0, stream>>>(a);
+    const int rc = check_launch("attn_bound_kernel");
+    if (rc != PMSST_OK) return rc;
+  }
+  a.tiles = static_cast<uint32_t>(p.q_tiles);
+  a.tiles_per_split = static_cast<int32_t>(p.q_per);
+  a.grid = make_grid(pairs, p.q_tiles * p.q_splits);
+  int rc = launch_dq<T, DP>(a, p.nw_q, drop, stream);
+  if (rc == PMSST_OK && a.part_q) rc = launch_sum<T>(a.part_q, a.dq, p.q_splits, a.s, false, stream);
+  if (rc != PMSST_OK || a.s.M == 0) return rc;
+  a.tiles = static_cast<uint32_t>(p.k_tiles);
+  a.tiles_per_split = static_cast<int32_t>(p.k_per);
+  a.grid = make_grid(pairs, p.k_tiles * p.k_splits);
+  rc = launch_dkv<T, DP>(a, p.nw_k, drop, stream);
+  if (rc != PMSST_OK || !a.part_k) return rc;
+  rc = launch_sum<T>(a.part_k, a.dk, p.k_splits, a.s, true, stream);
+  return rc != PMSST_OK ? rc : launch_sum<T>(a.part_v, a.dv, p.k_splits, a.s, true, stream);
+}
+
+template <typename T>
+int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+  return a.s.D <= 32 ? run_bwd<T, 32>(a, p, stream) : a.s.D <= 64 ? run_bwd<T, 64>(a, p, stream) : run_bwd<T, 128>(a, p, stream);
+}
+
+}  // namespace
+}  // namespace pmsst
+
+extern "C" {
+
+size_t pmsst_cross_attention_backward_workspace_size(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                                     int64_t kv_heads, int64_t head_dim, int dtype) {
+  pmsst::attn::Shape s;
+  if (pmsst::attn::make_shape("pmsst_cross_attention_backward", batch, queries, keys, heads, kv_heads, head_dim, dtype,
+                              s) != PMSST_OK ||
+      s.B == 0 || s.N == 0)
+    return 0;
+  return pmsst::bwd_space(s, pmsst::plan_backward(s, dtype), dtype).total;
+}
+
+int pmsst_cross_attention_backward(const void* grad_out, const int64_t* grad_out_strides, const void* q,
+                                   const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                   const int64_t* v_strides, const void* out, const float* lse, const uint8_t* key_mask,
+                                   int64_t key_mask_stride, const int32_t* key_lengths, void* grad_q, void* grad_k,
+                                   void* grad_v, int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                   int64_t kv_heads, int64_t head_dim, double scale, double dropout_p, const int64_t* rng,
+                                   int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace pmsst;
+  using namespace pmsst::attn;
+  const char* what = "pmsst_cross_attention_backward";
+  BwdArgs a{};
+  int rc = make_shape(what, batch, queries, keys, heads, kv_heads, head_dim, dtype, a.s);
+  if (rc != PMSST_OK) return rc;
+  PMSST_REQUIRE(scale > 0.0 && scale < 1e30, "%s: scale must be positive", what);
+  PMSST_REQUIRE(dropout_p >= 0.0 && dropout_p < 1.0, "%s: the dropout probability must lie in [0, 1)", what);
+  if (batch == 0) return PMSST_OK;
+  PMSST_REQUIRE(queries > 0, "%s: queries must be positive (the keys' gradients are zero without any)", what);
+  PMSST_REQUIRE(grad_out && q && out && lse && grad_q && (keys == 0 || (k && v && grad_k && grad_v)), "%s: null pointer",
+                what);
+  if ((rc = make_strides(what, grad_out, grad_out_strides, queries, heads, head_dim, dtype, a.gs)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, out, nullptr, queries, heads, head_dim, dtype, a.os)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, q, q_strides, queries, heads, head_dim, dtype, a.qs)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, k, k_strides, keys, kv_heads, head_dim, dtype, a.ks)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, v, v_strides, keys, kv_heads, head_dim, dtype, a.vs)) != PMSST_OK) return rc;
+  PMSST_REQUIRE(((reinterpret_cast<uintptr_t>(grad_q) | reinterpret_cast<uintptr_t>(grad_k) |
+                  reinterpret_cast<uintptr_t>(grad_v)) & 15) == 0,
+                "%s: gradients must be 16-byte aligned", what);
+  a.drop = make_dropout(dropout_p, rng);
+  PMSST_REQUIRE(rng || a.drop.limit == 0, "%s: null pointer (rng)", what);
+  const BwdPlan p = plan_backward(a.s, dtype);
+  const BwdSpace w = bwd_space(a.s, p, dtype);
+  if (workspace == nullptr || workspace_bytes < w.total)
+    return fail(PMSST_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, w.total, workspace_bytes);
+  PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: workspace must be 16-byte aligned", what);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.dout = grad_out;
+  a.km = {key_mask, key_mask_stride, key_lengths};
+  a.lse = lse;
+  a.dq = grad_q;
+  a.dk = grad_k;
+  a.dv = grad_v;
+  char* at = static_cast<char*>(workspace);
+  a.delta = reinterpret_cast<float*>(at);
+  at += w.delta;
+  a.vmax = reinterpret_cast<float*>(at);
+  at += w.bound;
+  a.l1 = reinterpret_cast<float*>(at);
+  at += w.bound;
+  if (w.part_q) a.part_q = reinterpret_cast<float*>(at);
+  at += w.part_q;
+  if (w.part_k) {
+    a.part_k = reinterpret_cast<float*>(at);
+    a.part_v = reinterpret_cast<float*>(at + w.part_k);
+  }
+  const int64_t pairs = batch * kv_heads, per = std::max(p.q_tiles * p.q_splits, p.k_tiles * p.k_splits);
+  constexpr int64_t kGrid = int64_t{1} << 31;
+  PMSST_REQUIRE(per < kGrid / (pairs + 8) && pairs < kGrid / kParts, "%s: too many rows for one call", what);
+  a.scale = static_cast<float>(scale);
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case PMSST_F32: return run_bwd<float>(a, p, st);
+    case PMSST_F16: return run_bwd<f16>(a, p, st);
+    default: return run_bwd<bf16>(a, p, st);
+  }
+}
+
+}  // extern "C"

@@ -618,6 +618,40 @@ class HipFusedExtension:
         check(rc, "pmsst_cross_attention_forward")
         return [out, lse] if need_lse else [out]
 
+    def cross_attention_backward(self, grad_out, q, k, v, out, lse, key_mask=None, key_lengths=None, scale=None,
+                                 dropout_p: float = 0.0, rng=None):
+        """Gradients ``[grad_q, grad_k, grad_v]`` of :meth:`cross_attention_forward` (dense, in the inputs'
+        shapes) from its ``out`` and ``lse`` and the same masks, scale, ``dropout_p`` and ``rng`` values.  The
+        weights are computed again; query heads that share a key head are summed in a fixed order."""
+        key_mask, mask_stride, key_lengths, scale = self._attention_check(q, k, v, key_mask, key_lengths, scale, dropout_p,
+                                                                          rng)
+        b, n, h, d = q.shape
+        m, hk = k.shape[1], k.shape[2]
+        for t, name in ((grad_out, "grad_out"), (out, "out")):
+            _req(t.device == q.device and t.shape == q.shape and t.dtype == q.dtype,
+                 f"{name} must have q's shape, dtype and device")
+        _req(lse.device == q.device and lse.dtype == torch.float32 and lse.shape == (b, h, n),
+             "lse must be the forward's, float32 [B, H, N]")
+        code = dtype_code(q.dtype)
+        grad_q = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
+        grad_k = torch.empty((b, m, hk, d), dtype=q.dtype, device=q.device)
+        grad_v = torch.empty((b, m, hk, d), dtype=q.dtype, device=q.device)
+        if n == 0:
+            return [grad_q, grad_k.zero_(), grad_v.zero_()]
+        (q, qs), (k, ks), (v, vs) = self._attention_operand(q), self._attention_operand(k), self._attention_operand(v)
+        grad_out, gs = self._attention_operand(grad_out)
+        out, lse = out.contiguous(), lse.contiguous()
+        with _DeviceGuard(q.device):
+            size = self._lib.pmsst_cross_attention_backward_workspace_size(b, n, m, h, hk, d, code)
+            ws = _workspace(size, q.device)
+            rc = self._lib.pmsst_cross_attention_backward(
+                _ptr(grad_out), gs, _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(out), _ptr(lse), _ptr(key_mask), mask_stride,
+                _ptr(key_lengths), _ptr(grad_q), _ptr(grad_k), _ptr(grad_v), b, n, m, h, hk, d, scale, dropout_p,
+                _ptr(rng), code, _ptr(ws), size, _stream(q.device),
+            )
+        check(rc, "pmsst_cross_attention_backward")
+        return [grad_q, grad_k, grad_v]
+
     # ------------------------------------------------------------------ dropout
 
     @staticmethod
