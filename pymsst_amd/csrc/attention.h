@@ -22,6 +22,7 @@
 #include "gemm.h"
 #include "mfma.h"
 #include "philox.h"
+#include "ring.h"
 
 namespace pmsst {
 namespace attn {
@@ -90,9 +91,24 @@ __device__ __forceinline__ f32x16_t mma(const u32x4_t& a, const u32x4_t& b, f32x
   }
 }
 
-// The other half's value (lane l ^ 32) combined with this lane's.
-__device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, kWave)); }
-__device__ __forceinline__ float half_sum(float v) { return v + __shfl_xor(v, 32, kWave); }
+// This lane's value and that of lane l ^ 32 combined, the lower lane's first: one exchange of register halves.
+__device__ __forceinline__ void halves(float v, float& lo, float& hi) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t a = r[0], b = r[1];
+  lo = __builtin_bit_cast(float, a);
+  hi = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float half_max(float v) {
+  float lo, hi;
+  halves(v, lo, hi);
+  return fmaxf(lo, hi);
+}
+__device__ __forceinline__ float half_sum(float v) {
+  float lo, hi;
+  halves(v, lo, hi);
+  return lo + hi;
+}
 
 // Two fp32 rounded to nearest into one register of 16-bit values.
 template <typename T>
@@ -159,6 +175,14 @@ __device__ __forceinline__ void hold(bool here) {
   if (here) __builtin_amdgcn_sched_barrier(0);
 }
 
+// The lane index, unknown to the compiler for rows of 256 bytes and more: the up to 80 swizzled addresses of a tile, which do not
+// change from tile to tile, would be kept in registers that those kernels do not have.
+template <int DB>
+__device__ __forceinline__ int fresh(int lane) {
+  if constexpr (DB >= 256) asm volatile("" : "+v"(lane));
+  return lane;
+}
+
 // acc[dt] += (tile rows sub*32 .. + 31)^T * p, for every 32 columns of the head dimension: p is a score tile
 // whose k index is the tile's row.
 template <typename T, int DP>
@@ -187,7 +211,7 @@ __device__ __forceinline__ void mma_cols(const char* tile, int sub, const f32x16
   }
 }
 
-// score += (tile rows sub*32 + key_row(l % 32)) * frag^T
+// (tile rows sub*32 + key_row(l % 32)) * frag^T
 template <typename T, int DP>
 __device__ __forceinline__ f32x16_t mma_rows(const char* tile, int sub, const u32x4_t (&frag)[DP * sizeof(T) / 32], int lane) {
   constexpr int DB = DP * sizeof(T);
@@ -215,41 +239,83 @@ __device__ __forceinline__ void load_frags(const T* row, bool valid, int d_units
   }
 }
 
-// BK rows of a tile through registers: fetch() issues the loads (rows past the end are clamped, never
-// branched on), commit() zeroes what is not to be seen and writes the tile.
-template <typename T, int DP, int BK, int THREADS>
+// BK rows of a tile, moved from global memory straight into LDS (16 bytes a lane to a wave's base + 16 * lane:
+// the lane that fills unit p of row r fetches unit p ^ swz(r)).  Whole tiles step a pointer per unit by a
+// constant; a cut one (and rows whose heads do not divide the tile, and fp32 rows of 512 bytes, which leave no
+// registers for pointers) computes its addresses, rows past the end
+// clamped to the last, and what is not to be seen is zeroed afterwards by the lanes that moved it.
+template <typename T, int DP, int BK, int NW>
 struct Tile {
   static constexpr int DB = DP * sizeof(T);
   static constexpr int UNITS = DB / 16;
-  static constexpr int CH = BK * UNITS / THREADS;
-  static constexpr int STEP = THREADS / UNITS;  // rows between a thread's units
-  static_assert(CH >= 1 && CH * THREADS == BK * UNITS && THREADS % UNITS == 0, "whole units per thread");
-  u32x4_t reg[CH];
+  static constexpr int CH = BK * UNITS / (64 * NW);  // moves of a wave
+  static constexpr int STEP = 64 * NW / UNITS;       // rows between them
+  static constexpr int BYTES = BK * DB;
+  static_assert(CH >= 1 && CH * 64 * NW == BK * UNITS && 64 % UNITS == 0, "whole rows per move");
+  const char* ptr[CH];
 
-  // at(i): element offset of tile row i's first element, for rows clamped below `rows` (> 0)
-  template <typename F>
-  __device__ __forceinline__ void fetch(const T* base, int row0, int rows, int d_units, F at) {
-    const int u = threadIdx.x % UNITS;
-    const int ub = u < d_units ? 16 * u : 0;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      int row = row0 + static_cast<int>(threadIdx.x) / UNITS + i * STEP;
-      row = row < rows ? row : rows - 1;
-      reg[i] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const char*>(base + at(row)) + ub);
-    }
+  static __device__ __forceinline__ int row_of(int i) { return static_cast<int>(threadIdx.x) / UNITS + i * STEP; }
+
+  // The unit this lane moves of its row (unit 0 in place of those past head_dim).
+  static __device__ __forceinline__ int unit_of(int i) {
+    return (static_cast<int>(threadIdx.x) % UNITS) ^ swz<DB>(row_of(i));
+  }
+  static __device__ __forceinline__ int byte_of(int i, int d_units) {
+    const int u = unit_of(i);
+    return u < d_units ? 16 * u : 0;
   }
 
-  __device__ __forceinline__ void commit(char* tile, uint64_t seen, int d_units) {
-    const int u = threadIdx.x % UNITS;
+  // at(row): element offset of a row from `base`
+  template <typename F>
+  __device__ __forceinline__ void start(const T* base, int row0, int d_units, F at) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int row = static_cast<int>(threadIdx.x) / UNITS + i * STEP;
-      const bool ok = u < d_units && ((seen >> row) & 1);
-      const u32x4_t v = ok ? reg[i] : u32x4_t{0, 0, 0, 0};
-      *reinterpret_cast<u32x4_t*>(tile + row * DB + 16 * (u ^ swz<DB>(row))) = v;
+      ptr[i] = reinterpret_cast<const char*>(base + at(row0 + row_of(i))) + byte_of(i, d_units);
+    }
+  }
+  static __device__ __forceinline__ uint32_t target(const char* tile, int i) {
+    return lds_addr(tile) + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64) * 1024 + i * NW * 1024;
+  }
+  // Starts a whole tile's move; the pointers go on by `step` bytes.
+  __device__ __forceinline__ void fetch(const char* tile, int64_t step) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      dma16_m0(ptr[i], target(tile, i));
+      ptr[i] += step;
+    }
+  }
+  // The tile at row0, of which only rows below `rows` (> 0) are there.
+  template <typename F>
+  __device__ __forceinline__ void fetch_cut(const char* tile, const T* base, int row0, int rows, int d_units, F at) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int row = min(row0 + row_of(i), rows - 1);
+      dma16_m0(reinterpret_cast<const char*>(base + at(row)) + byte_of(i, d_units), target(tile, i));
+    }
+  }
+  // Zeroes this lane's units of rows whose bit is 0, and those past head_dim; the moves must have arrived.
+  __device__ __forceinline__ void clear(char* tile, uint64_t seen, int d_units) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      if (unit_of(i) >= d_units || !((seen >> row_of(i)) & 1)) {
+        *reinterpret_cast<u32x4_t*>(tile + (i * 64 * NW + static_cast<int>(threadIdx.x)) * 16) = u32x4_t{0, 0, 0, 0};
+      }
     }
   }
 };
+
+// Two tiles a stage; a stage is filled STAGES - 1 tiles ahead.  Rows of up to 128 bytes have three stages (48 KB,
+// three blocks of 4 waves a CU); longer ones, and blocks of 2 waves, which LDS would keep from sharing a CU, two.
+template <int DB, int NW>
+constexpr int stages() { return DB <= 128 && NW == 4 ? 3 : 2; }
+
+// Uses a loaded register here, so that the compiler waits for the load here and not (for every load in flight)
+// inside the loop.
+template <int N>
+__device__ __forceinline__ void arrive(u32x4_t (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
 
 // Bits of BK <= 64 rows from row0 that lie below `rows`.
 __device__ __forceinline__ uint64_t range_bits(int row0, int rows) {
@@ -264,10 +330,10 @@ __device__ __forceinline__ int key_count(const KeyMask& km, int b, int M) {
   return len < 0 ? 0 : len > M ? M : len;
 }
 
-// The 64-bit word of a tile's seen keys, for this lane: bit reg_key(r) of the result is register r of
-// sub-tile `sub`.
-__device__ __forceinline__ uint32_t lane_bits(uint64_t seen, int sub, int h) {
-  return static_cast<uint32_t>(seen >> (32 * sub)) >> (8 * h);
+// `v` where bit k of `bits` is set, else `other`: a sign-extended bit and a bit select.
+__device__ __forceinline__ float where_bit(uint32_t bits, int k, float v, float other) {
+  const uint32_t m = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), k, 1));
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) & m) | (__builtin_bit_cast(uint32_t, other) & ~m));
 }
 
 // Stores a transposed accumulator (rows = head dimension, columns = positions): lane's position row at `row`.

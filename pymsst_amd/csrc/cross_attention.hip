@@ -43,10 +43,11 @@ template <typename T>
 constexpr float p_shift() { return std::is_same<T, f16>::value ? 6.f : 0.f; }
 
 template <typename T, int DP, int NW, bool DROP>
-__global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 ? 1 : 2))) void attn_fwd_kernel(FwdArgs a) {
   constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
   constexpr int BK = fwd_keys<T, DP>(), SUBS = BK / 32;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][BK * DB];
+  constexpr int S = stages<DB, NW>();
+  __shared__ __attribute__((aligned(16))) char lds[S][2][BK * DB];
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
   uint32_t pair, sub_block;
   if (!locate(a.grid, pair, sub_block)) return;
@@ -57,6 +58,7 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(FwdArgs a) {
 
   const int r = static_cast<int>(row_tile) * 32 * NW + wave * 32 + (lane & 31);
   const bool row_ok = r < s.R;
+  const bool idle = __builtin_amdgcn_readfirstlane(r) >= s.R;  // no row of this wave is there: it only moves tiles
   const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(r))), head = hk * s.G + (r - n * s.G);
   u32x4_t qf[NS];
   load_frags<T, DP>(static_cast<const T*>(a.q) + b * a.qs.b + (row_ok ? n * a.qs.n + head * a.qs.h : 0), row_ok, d_units,
@@ -78,66 +80,89 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(FwdArgs a) {
   }
 
   f32x16_t o[DT]{};
-  float ref = -kInf, l = 0.f;  // the maximum (in log2 units) P is taken against, this lane's part of the sum
+  float ref = -kInf;           // the maximum (in log2 units) P is taken against
+  float l[2] = {0.f, 0.f};     // this lane's part of the sum
 
-  Tile<T, DP, BK, 64 * NW> kt, vt;
-  uint8_t seen_byte = 1;
-  auto fetch = [&](int t) {
+  Tile<T, DP, BK, NW> kt, vt;
+  auto k_at = [&](int i) { return i * a.ks.n; };
+  auto v_at = [&](int i) { return i * a.vs.n; };
+  kt.start(kb, t0 * BK, d_units, k_at);
+  vt.start(vb, t0 * BK, d_units, v_at);
+  uint8_t byte_now = 1, byte_next = 1;  // this lane's key of the mask
+  auto mask_byte = [&](int t) { return mask[min(t * BK + lane, count - 1)]; };
+  auto fetch = [&](int t, int stage) {
     const int key0 = t * BK;
-    if (mask) seen_byte = mask[min(key0 + lane, count - 1)];
-    kt.fetch(kb, key0, count, d_units, [&](int i) { return i * a.ks.n; });
-    vt.fetch(vb, key0, count, d_units, [&](int i) { return i * a.vs.n; });
+    if (DB < 512 && key0 + BK <= count) {
+      kt.fetch(lds[stage][0], BK * static_cast<int64_t>(sizeof(T)) * a.ks.n);
+      vt.fetch(lds[stage][1], BK * static_cast<int64_t>(sizeof(T)) * a.vs.n);
+    } else {
+      kt.fetch_cut(lds[stage][0], kb, key0, count, d_units, k_at);
+      vt.fetch_cut(lds[stage][1], vb, key0, count, d_units, v_at);
+    }
   };
-  if (t0 < t1) fetch(t0);
+  arrive(qf);
+  if (mask && t0 < t1) byte_next = mask_byte(t0);
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) {
+    if (t0 + i < t1) fetch(t0 + i, i);
+  }
+  int stage = 0;
   for (int t = t0; t < t1; ++t) {
-    char* kl = lds[t & 1][0];
-    char* vl = lds[t & 1][1];
+    char* kl = lds[stage][0];
+    char* vl = lds[stage][1];
     uint64_t seen = range_bits(t * BK, count);
-    if (mask) seen &= __ballot(seen_byte != 0);
+    if (mask) {
+      byte_now = byte_next;
+      seen &= __ballot(byte_now != 0);
+      if (t + 1 < t1) byte_next = mask_byte(t + 1);
+    }
     if constexpr (BK == 32) seen &= 0xFFFFFFFFu;
     constexpr uint64_t kAll = BK == 64 ? ~uint64_t{0} : 0xFFFFFFFFu;
-    kt.commit(kl, seen, d_units);
-    vt.commit(vl, seen, d_units);
+    // this tile has arrived once only the next ones' moves are in flight
+    if (S == 3 && !mask && t + 1 < t1) vm_wait<2 * kt.CH>();
+    else vm_wait<0>();
+    if (seen != kAll || d_units != kt.UNITS) {
+      kt.clear(kl, seen, d_units);
+      vt.clear(vl, seen, d_units);
+    }
     __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
-    if (seen == 0) continue;
-
-    f32x16_t p[SUBS];
-#pragma unroll
-    for (int u = 0; u < SUBS; ++u) p[u] = mma_rows<T, DP>(kl, u, qf, lane);
-    if (seen != kAll) {
-#pragma unroll
-      for (int u = 0; u < SUBS; ++u) {
-        const uint32_t bits = lane_bits(seen, u, h);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[u][i] = (bits >> reg_key(i)) & 1 ? p[u][i] : -kInf;
-      }
-    }
-    float top = p[0][0];
+    if (t + S - 1 < t1) fetch(t + S - 1, stage == 0 ? S - 1 : stage - 1);
+    stage = stage == S - 1 ? 0 : stage + 1;
+    if (idle) continue;
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
+      const uint32_t sub_seen = static_cast<uint32_t>(seen >> (32 * u));
+      if (sub_seen == 0) continue;
+      const int at_lane = fresh<DB>(lane);
+      f32x16_t p = mma_rows<T, DP>(kl, u, qf, at_lane);
+      if (sub_seen != 0xFFFFFFFFu) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, p[u][i]);
-    }
-    top = half_max(top) * a.scale_log2;
-    if (__any(top > ref + kLag)) {
-      const float next = fmaxf(ref, top);
-      const float alpha = next == -kInf ? 1.f : __builtin_amdgcn_exp2f(ref - next);
-      ref = next;
-      l *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+        for (int i = 0; i < 16; ++i) p[i] = where_bit(sub_seen >> (8 * h), reg_key(i), p[i], -kInf);
       }
-    }
-    const float base = ref == -kInf ? 0.f : p_shift<T>() - ref;
+      float top = fmaxf(p[0], p[1]), top2 = fmaxf(p[2], p[3]);
 #pragma unroll
-    for (int u = 0; u < SUBS; ++u) {
+      for (int i = 4; i < 16; i += 4) {
+        top = fmaxf(fmaxf(top, p[i]), p[i + 1]);
+        top2 = fmaxf(fmaxf(top2, p[i + 2]), p[i + 3]);
+      }
+      top = half_max(fmaxf(top, top2)) * a.scale_log2;
+      if (__any(top > ref + kLag)) {
+        const float next = fmaxf(ref, top);
+        const float alpha = next == -kInf ? 1.f : __builtin_amdgcn_exp2f(ref - next);
+        ref = next;
+        l[0] *= alpha;
+        l[1] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+        }
+      }
+      const float base = ref == -kInf ? 0.f : p_shift<T>() - ref;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        p[u][i] = __builtin_amdgcn_exp2f(fmaf(p[u][i], a.scale_log2, base));
-        l += p[u][i];
+        p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.scale_log2, base));
+        l[i & 1] += p[i];
       }
       if constexpr (DROP) {
 #pragma unroll
@@ -145,17 +170,17 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(FwdArgs a) {
           uint32_t w[4];
           philox7(key, drop0 + static_cast<uint32_t>(t * (BK / 8) + 4 * u + 2 * j + h), w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) p[u][8 * j + i] = philox_keep(w, i, a.drop.limit << 16) ? p[u][8 * j + i] : 0.f;
+          for (int i = 0; i < 8; ++i) p[8 * j + i] = philox_keep(w, i, a.drop.limit << 16) ? p[8 * j + i] : 0.f;
         }
       }
-      mma_cols<T, DP>(vl, u, p[u], o, lane);
+      mma_cols<T, DP>(vl, u, p, o, at_lane);
     }
   }
 
-  l = half_sum(l);
-  const float inv = l == 0.f ? 0.f : (DROP ? a.drop.factor : 1.f) / l;
+  const float sum = half_sum(l[0] + l[1]);
+  const float inv = sum == 0.f ? 0.f : (DROP ? a.drop.factor : 1.f) / sum;
   if (!row_ok) return;
-  const float lse = l == 0.f ? -kInf : (ref - p_shift<T>() + __log2f(l)) * kLn2;
+  const float lse = sum == 0.f ? -kInf : (ref - p_shift<T>() + __log2f(sum)) * kLn2;
   if (a.part_o) {
     const int64_t at = (static_cast<int64_t>(split) * a.grid.pairs + pair) * s.R + r;
     store_cols_f32<T, DP>(a.part_o + at * s.D, o, inv, s.D, h);
@@ -212,8 +237,10 @@ struct FwdPlan {
 };
 
 // Waves of a block: 2 where that covers the rows (half a block of 4 would idle; fp32 rows of 512 bytes keep 4,
-// whose lanes hold half as much of a tile on its way), else 4.  Splits: as many as give
-// every CU two blocks, of at least 256 keys each.
+// whose lanes hold half as much of a tile on its way), else 4.  Splits, of at least 256 keys each: up to 4 blocks
+// of 4 waves a CU, whose products bound them and whose ragged ends so even out (2760 queries over up to 8192 keys,
+// heads of 128: 235 us; with 2 blocks a CU 266, with 8 253), or 2 blocks of 2 waves, which the keys' bytes bound
+// (16 single queries over up to 16500 keys: 89 us; with 4 blocks 102).
 FwdPlan plan_forward(const Shape& s, int dtype) {
   FwdPlan p;
   const bool wide = padded_dim(s.D) * static_cast<int>(dtype_size(dtype)) == 512;
@@ -221,9 +248,9 @@ FwdPlan plan_forward(const Shape& s, int dtype) {
   p.bk = wide ? 32 : 64;
   p.row_tiles = (int64_t{s.R} + 32 * p.nw - 1) / (32 * p.nw);
   const int64_t tiles = std::max<int64_t>(1, (int64_t{s.M} + p.bk - 1) / p.bk);
-  const int64_t blocks = int64_t{s.B} * s.Hk * p.row_tiles, want = 2 * num_cus();
+  const int64_t blocks = int64_t{s.B} * s.Hk * p.row_tiles, want = (p.nw == 4 ? 4 : 2) * num_cus();
   p.splits = 1;
-  if (blocks < want) p.splits = std::max<int64_t>(1, std::min(want / blocks, int64_t{s.M} / 256));
+  if (blocks < want) p.splits = std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, int64_t{s.M} / 256));
   p.tiles_per_split = (tiles + p.splits - 1) / p.splits;
   p.splits = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
   return p;

@@ -27,7 +27,8 @@ struct BwdArgs {
   KeyMask km;
   const float* lse;  // [B, H, N]
   void *dq, *dk, *dv;
-  float* delta;                // [pairs, R]
+  float *base, *delta;         // [pairs, rows_pad]: -lse in log2 units (- inf: no weight), D
+  int32_t rows_pad;            // R rounded up to 64
   float *vmax, *l1;            // fp16: [pairs, kParts] maxima of |V| over the seen keys and of |dO row|_1
   float *part_q, *part_k, *part_v;  // partial sums [splits, pairs, R or M, D], NULL: not split
   Shape s;
@@ -58,6 +59,11 @@ __device__ __forceinline__ float parts_max(const float* parts) {
 #pragma unroll
   for (int i = 0; i < kParts; ++i) m = fmaxf(m, parts[i]);
   return m;
+}
+
+// fp16: dK's power of two, of a pair (P is held at 2^14 there, so dS at 2^(14 + this)).
+__device__ __forceinline__ int pair_exponent(const BwdArgs& a, uint32_t pair) {
+  return scale_exponent(2.f * parts_max(a.l1 + pair * kParts) * parts_max(a.vmax + pair * kParts) * a.drop.factor, 1);
 }
 
 // ---------------------------------------------------------------- fp16 bounds
@@ -112,10 +118,11 @@ __global__ __launch_bounds__(256) void attn_bound_kernel(BwdArgs a) {
 // ---------------------------------------------------------------- dQ
 
 template <typename T, int DP, int NW, bool DROP>
-__global__ __launch_bounds__(64 * NW) void attn_dq_kernel(BwdArgs a) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 ? 1 : 2))) void attn_dq_kernel(BwdArgs a) {
   constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
   constexpr int BK = bwd_tile<T, DP>(), SUBS = BK / 32;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][BK * DB];
+  constexpr int S = stages<DB, NW>();
+  __shared__ __attribute__((aligned(16))) char lds[S][2][BK * DB];
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
   uint32_t pair, sub_block;
   if (!locate(a.grid, pair, sub_block)) return;
@@ -126,11 +133,10 @@ __global__ __launch_bounds__(64 * NW) void attn_dq_kernel(BwdArgs a) {
 
   const int r = static_cast<int>(row_tile) * 32 * NW + wave * 32 + (lane & 31);
   const bool row_ok = r < s.R;
+  const bool idle = __builtin_amdgcn_readfirstlane(r) >= s.R;  // no row of this wave is there: it only moves tiles
   const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(r))), head = hk * s.G + (r - n * s.G);
   u32x4_t qf[NS], gf[NS];
   float delta = 0.f, l1 = 0.f;
-  load_frags<T, DP>(static_cast<const T*>(a.q) + b * a.qs.b + (row_ok ? n * a.qs.n + head * a.qs.h : 0), row_ok, d_units,
-                    h, qf);
   load_frags<T, DP>(static_cast<const T*>(a.dout) + b * a.gs.b + (row_ok ? n * a.gs.n + head * a.gs.h : 0), row_ok,
                     d_units, h, gf);
   {
@@ -151,12 +157,22 @@ __global__ __launch_bounds__(64 * NW) void attn_dq_kernel(BwdArgs a) {
     }
     delta = half_sum(delta);
   }
-  if (row_ok && h == 0 && split == 0) a.delta[static_cast<int64_t>(pair) * s.R + r] = delta;
+  hold(true);
+  load_frags<T, DP>(static_cast<const T*>(a.q) + b * a.qs.b + (row_ok ? n * a.qs.n + head * a.qs.h : 0), row_ok, d_units,
+                    h, qf);
   // -lse in log2 units: a row that sees no key (and one past the end) has no weight
   float base = -kInf;
   if (row_ok) {
     const float lse = a.lse[(static_cast<int64_t>(b) * s.H + head) * s.N + n];
     base = lse == -kInf ? -kInf : -lse * kLog2e;
+  }
+  if (h == 0 && split == 0 && r < a.rows_pad) {
+    // for the other kernel, in the order and form it takes them; rows past the end have no weight
+    float d = delta;
+    if constexpr (std::is_same<T, f16>::value) d = ldexpf(d, pair_exponent(a, pair));
+    const int64_t at = static_cast<int64_t>(pair) * a.rows_pad + r;
+    a.base[at] = base + (std::is_same<T, f16>::value ? 14.f : 0.f);
+    a.delta[at] = d;
   }
   int e = 0;
   if constexpr (std::is_same<T, f16>::value) {
@@ -179,31 +195,61 @@ __global__ __launch_bounds__(64 * NW) void attn_dq_kernel(BwdArgs a) {
   }
 
   f32x16_t acc[DT]{};
-  Tile<T, DP, BK, 64 * NW> kt, vt;
-  uint8_t seen_byte = 1;
-  auto fetch = [&](int t) {
+  Tile<T, DP, BK, NW> kt, vt;
+  auto k_at = [&](int i) { return i * a.ks.n; };
+  auto v_at = [&](int i) { return i * a.vs.n; };
+  kt.start(kb, t0 * BK, d_units, k_at);
+  vt.start(vb, t0 * BK, d_units, v_at);
+  uint8_t byte_now = 1, byte_next = 1;  // this lane's key of the mask
+  auto mask_byte = [&](int t) { return mask[min(t * BK + lane, count - 1)]; };
+  auto fetch = [&](int t, int stage) {
     const int key0 = t * BK;
-    if (mask) seen_byte = mask[min(key0 + lane, count - 1)];
-    kt.fetch(kb, key0, count, d_units, [&](int i) { return i * a.ks.n; });
-    vt.fetch(vb, key0, count, d_units, [&](int i) { return i * a.vs.n; });
+    if (DB < 512 && key0 + BK <= count) {
+      kt.fetch(lds[stage][0], BK * static_cast<int64_t>(sizeof(T)) * a.ks.n);
+      vt.fetch(lds[stage][1], BK * static_cast<int64_t>(sizeof(T)) * a.vs.n);
+    } else {
+      kt.fetch_cut(lds[stage][0], kb, key0, count, d_units, k_at);
+      vt.fetch_cut(lds[stage][1], vb, key0, count, d_units, v_at);
+    }
   };
-  if (t0 < t1) fetch(t0);
+  arrive(qf);
+  arrive(gf);
+  asm volatile("" : "+v"(base), "+v"(delta));
+  if (mask && t0 < t1) byte_next = mask_byte(t0);
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) {
+    if (t0 + i < t1) fetch(t0 + i, i);
+  }
+  int stage = 0;
   for (int t = t0; t < t1; ++t) {
-    char* kl = lds[t & 1][0];
-    char* vl = lds[t & 1][1];
+    char* kl = lds[stage][0];
+    char* vl = lds[stage][1];
     uint64_t seen = range_bits(t * BK, count);
-    if (mask) seen &= __ballot(seen_byte != 0);
+    if (mask) {
+      byte_now = byte_next;
+      seen &= __ballot(byte_now != 0);
+      if (t + 1 < t1) byte_next = mask_byte(t + 1);
+    }
     if constexpr (BK == 32) seen &= 0xFFFFFFFFu;
     constexpr uint64_t kAll = BK == 64 ? ~uint64_t{0} : 0xFFFFFFFFu;
-    kt.commit(kl, seen, d_units);
-    vt.commit(vl, seen, d_units);
+    // this tile has arrived once only the next ones' moves are in flight
+    if (S == 3 && !mask && t + 1 < t1) vm_wait<2 * kt.CH>();
+    else vm_wait<0>();
+    if (seen != kAll || d_units != kt.UNITS) {
+      kt.clear(kl, seen, d_units);
+      vt.clear(vl, seen, d_units);
+    }
     __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
-    if (seen == 0) continue;
+    if (t + S - 1 < t1) fetch(t + S - 1, stage == 0 ? S - 1 : stage - 1);
+    stage = stage == S - 1 ? 0 : stage + 1;
+    if (idle) continue;
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
-      f32x16_t p = mma_rows<T, DP>(kl, u, qf, lane);
-      f32x16_t dp = mma_rows<T, DP>(vl, u, gf, lane);
+      const uint32_t sub_seen = static_cast<uint32_t>(seen >> (32 * u));
+      if (sub_seen == 0) continue;
+      const int at_lane = fresh<DB>(lane);
+      f32x16_t p = mma_rows<T, DP>(kl, u, qf, at_lane);
+      f32x16_t dp = mma_rows<T, DP>(vl, u, gf, at_lane);
       if constexpr (DROP) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -219,12 +265,11 @@ __global__ __launch_bounds__(64 * NW) void attn_dq_kernel(BwdArgs a) {
       for (int i = 0; i < 16; ++i) {
         p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.scale_log2, base)) * (dp[i] - delta);
       }
-      if (seen != kAll) {
-        const uint32_t bits = lane_bits(seen, u, h);
+      if (sub_seen != 0xFFFFFFFFu) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = (bits >> reg_key(i)) & 1 ? p[i] : 0.f;
+        for (int i = 0; i < 16; ++i) p[i] = where_bit(sub_seen >> (8 * h), reg_key(i), p[i], 0.f);
       }
-      mma_cols<T, DP>(kl, u, p, acc, lane);
+      mma_cols<T, DP>(kl, u, p, acc, at_lane);
     }
   }
   if (!row_ok) return;
@@ -241,12 +286,13 @@ __global__ __launch_bounds__(64 * NW) void attn_dq_kernel(BwdArgs a) {
 // ---------------------------------------------------------------- dK, dV
 
 template <typename T, int DP, int NW, bool DROP>
-__global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 ? 1 : 2))) void attn_dkv_kernel(BwdArgs a) {
   constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
   constexpr int BQ = bwd_tile<T, DP>(), SUBS = BQ / 32;
   constexpr bool kHalf = std::is_same<T, f16>::value;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][BQ * DB];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][BQ];  // -lse (log2 units), D
+  constexpr int S = stages<DB, NW>();
+  __shared__ __attribute__((aligned(16))) char lds[S][2][BQ * DB];
+  __shared__ __attribute__((aligned(16))) float stat[S][2][64];  // -lse (log2 units), D
   __shared__ __attribute__((aligned(16))) uint32_t kept[DROP ? NW : 1][DROP ? 32 : 4];
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
   uint32_t pair, sub_block;
@@ -260,23 +306,22 @@ __global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(BwdArgs a) {
   const int key0 = block_key0 + wave * 32, ki = key0 + (lane & 31);
   const bool seen = ki < count && (a.km.mask == nullptr || a.km.mask[b * a.km.stride + ki] != 0);
 
+  const bool idle = __builtin_amdgcn_readfirstlane(key0) >= count;  // no key of this wave counts: it only moves tiles
+
   f32x16_t dk[DT]{}, dv[DT]{};
   float k_scale = a.scale, v_scale = DROP ? a.drop.factor : 1.f;
   if (block_key0 < count) {
     u32x4_t kf[NS], vf[NS];
     load_frags<T, DP>(static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h + (seen ? ki * a.ks.n : 0), seen, d_units, h, kf);
     load_frags<T, DP>(static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h + (seen ? ki * a.vs.n : 0), seen, d_units, h, vf);
-    // P' = 2^shift P, dS' = P' 2^e (...): see the head of this file
-    constexpr float kShift = kHalf ? 14.f : 0.f;
-    float power = 1.f;
+    // P' = 2^14 P (in base), dS' = P' 2^e (...): see the head of this file
+    float dp_scale = DROP ? a.drop.factor : 1.f;
     if constexpr (kHalf) {
-      const int e = scale_exponent(2.f * parts_max(a.l1 + pair * kParts) * parts_max(a.vmax + pair * kParts) * a.drop.factor,
-                                   1);
-      power = ldexpf(1.f, e);
+      const int e = pair_exponent(a, pair);
+      dp_scale = ldexpf(dp_scale, e);
       k_scale = ldexpf(a.scale, -e - 14);
       v_scale = ldexpf(v_scale, -14);
     }
-    const float dp_scale = DROP ? a.drop.factor * power : power;
 
     const int tiles = (s.R + BQ - 1) / BQ;
     const int t0 = static_cast<int>(split) * a.tiles_per_split;
@@ -286,45 +331,61 @@ __global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(BwdArgs a) {
     PhiloxKey key{};
     if constexpr (DROP) key = philox_key(a.drop.rng);
 
-    Tile<T, DP, BQ, 64 * NW> qt, gt;
-    float stat_lse = 0.f, stat_delta = 0.f;
+    Tile<T, DP, BQ, NW> qt, gt;
     auto at = [&](int i, const Strides& st) {
       const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(i)));
       return n * st.n + (hk * s.G + (i - n * s.G)) * st.h;
     };
-    auto fetch = [&](int t) {
+    auto q_at = [&](int i) { return at(i, a.qs); };
+    auto g_at = [&](int i) { return at(i, a.gs); };
+    const bool steps = BQ % s.G == 0;  // a tile further on is the same head again
+    const int64_t q_step = BQ / s.G * static_cast<int64_t>(sizeof(T)) * a.qs.n;
+    const int64_t g_step = BQ / s.G * static_cast<int64_t>(sizeof(T)) * a.gs.n;
+    qt.start(qb, t0 * BQ, d_units, q_at);
+    gt.start(gb, t0 * BQ, d_units, g_at);
+    // waves 0 and 1 also move a tile's 64 (32) pairs of statistics, 4 bytes a lane
+    const int wave0 = __builtin_amdgcn_readfirstlane(wave);
+    const float* stat_src = (wave0 == 0 ? a.base : a.delta) + static_cast<int64_t>(pair) * a.rows_pad + lane;
+    auto fetch = [&](int t, int stage) {
       const int row0 = t * BQ;
-      qt.fetch(qb, row0, s.R, d_units, [&](int i) { return at(i, a.qs); });
-      gt.fetch(gb, row0, s.R, d_units, [&](int i) { return at(i, a.gs); });
-      if (threadIdx.x < BQ) {
-        const int i = min(row0 + static_cast<int>(threadIdx.x), s.R - 1);
-        const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(i)));
-        stat_lse = a.lse[(static_cast<int64_t>(b) * s.H + hk * s.G + (i - n * s.G)) * s.N + n];
-        stat_delta = a.delta[static_cast<int64_t>(pair) * s.R + i];
+      if (DB < 512 && steps && row0 + BQ <= s.R) {
+        qt.fetch(lds[stage][0], q_step);
+        gt.fetch(lds[stage][1], g_step);
+      } else {
+        qt.fetch_cut(lds[stage][0], qb, row0, s.R, d_units, q_at);
+        gt.fetch_cut(lds[stage][1], gb, row0, s.R, d_units, g_at);
       }
+      if (wave0 < 2 && (BQ == 64 || lane < BQ)) dma4_m0(stat_src + row0, lds_addr(stat[stage]) + 256 * wave0);
     };
-    // fp32 rows of 512 bytes leave no registers for the tile after this one (its products take 10 times as long
-    // as its loads)
-    constexpr bool kAhead = DB < 512;
-    if (kAhead && t0 < t1) fetch(t0);
+    arrive(kf);
+    arrive(vf);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) {
+      if (t0 + i < t1) fetch(t0 + i, i);
+    }
+    int stage = 0;
     for (int t = t0; t < t1; ++t) {
-      if (!kAhead) fetch(t);
-      char* ql = lds[t & 1][0];
-      char* gl = lds[t & 1][1];
-      float* base = stat[t & 1][0];
-      float* delta = stat[t & 1][1];
-      const uint64_t rows = range_bits(t * BQ, s.R);
-      qt.commit(ql, rows, d_units);
-      gt.commit(gl, rows, d_units);
-      if (threadIdx.x < BQ) {
-        const bool ok = ((rows >> threadIdx.x) & 1) && stat_lse != -kInf;
-        base[threadIdx.x] = ok ? kShift - stat_lse * kLog2e : -kInf;
-        delta[threadIdx.x] = ok ? stat_delta * power : 0.f;
+      char* ql = lds[stage][0];
+      char* gl = lds[stage][1];
+      const float* base = stat[stage][0];
+      const float* delta = stat[stage][1];
+      if (S == 3 && t + 1 < t1) {
+        if (wave0 < 2) vm_wait<2 * qt.CH + 1>();
+        else vm_wait<2 * qt.CH>();
+      } else {
+        vm_wait<0>();
+      }
+      if (d_units != qt.UNITS) {
+        qt.clear(ql, ~uint64_t{0}, d_units);
+        gt.clear(gl, ~uint64_t{0}, d_units);
       }
       __syncthreads();
-      if (kAhead && t + 1 < t1) fetch(t + 1);
+      if (t + S - 1 < t1) fetch(t + S - 1, stage == 0 ? S - 1 : stage - 1);
+      stage = stage == S - 1 ? 0 : stage + 1;
+      if (idle) continue;
 #pragma unroll
       for (int u = 0; u < SUBS; ++u) {
+        if (t * BQ + 32 * u >= s.R) continue;
         if constexpr (DROP) {
           // 32 rows x 4 blocks of 8 keys: a lane draws 2 of them, one byte of kept bits each
 #pragma unroll
@@ -342,8 +403,9 @@ __global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(BwdArgs a) {
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         hold(sizeof(T) == 4);
-        f32x16_t p = mma_rows<T, DP>(ql, u, kf, lane);
-        f32x16_t ds = mma_rows<T, DP>(gl, u, vf, lane);
+        const int at_lane = fresh<DB>(lane);
+        f32x16_t p = mma_rows<T, DP>(ql, u, kf, at_lane);
+        f32x16_t ds = mma_rows<T, DP>(gl, u, vf, at_lane);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int row = reg_key(i) + 8 * h;
@@ -358,8 +420,8 @@ __global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(BwdArgs a) {
         }
         if constexpr (DROP) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         hold(sizeof(T) == 4);
-        mma_cols<T, DP>(gl, u, p, dv, lane);
-        mma_cols<T, DP>(ql, u, ds, dk, lane);
+        mma_cols<T, DP>(gl, u, p, dv, at_lane);
+        mma_cols<T, DP>(ql, u, ds, dk, at_lane);
       }
     }
   }
@@ -421,7 +483,7 @@ BwdPlan plan_backward(const Shape& s, int dtype) {
   auto split = [&](int64_t owners, int64_t along, int64_t& splits, int64_t& per) {
     const int64_t tiles = std::max<int64_t>(1, (along + bk - 1) / bk);
     splits = 1;
-    if (owners < want) splits = std::max<int64_t>(1, std::min(want / owners, along / 256));
+    if (owners < want) splits = std::max<int64_t>(1, std::min((want + owners - 1) / owners, along / 256));
     per = (tiles + splits - 1) / splits;
     splits = (tiles + per - 1) / per;
   };
@@ -442,11 +504,11 @@ struct BwdSpace {
 BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int dtype) {
   const size_t pairs = static_cast<size_t>(s.B) * s.Hk;
   BwdSpace w;
-  w.delta = align_up(pairs * s.R * 4, 256);
+  w.delta = align_up(pairs * align_up(s.R, 64) * 4, 256);
   w.bound = dtype == PMSST_F16 ? align_up(pairs * kParts * 4, 256) : 0;
   w.part_q = p.q_splits > 1 ? align_up(static_cast<size_t>(p.q_splits) * pairs * s.R * s.D * 4, 256) : 0;
   w.part_k = p.k_splits > 1 ? align_up(static_cast<size_t>(p.k_splits) * pairs * s.M * s.D * 4, 256) : 0;
-  w.total = w.delta + 2 * w.bound + w.part_q + 2 * w.part_k;
+  w.total = 2 * w.delta + 2 * w.bound + w.part_q + 2 * w.part_k;
   return w;
 }
 
@@ -580,6 +642,9 @@ int pmsst_cross_attention_backward(const void* grad_out, const int64_t* grad_out
   a.dk = grad_k;
   a.dv = grad_v;
   char* at = static_cast<char*>(workspace);
+  a.rows_pad = static_cast<int32_t>(align_up(a.s.R, 64));
+  a.base = reinterpret_cast<float*>(at);
+  at += w.delta;
   a.delta = reinterpret_cast<float*>(at);
   at += w.delta;
   a.vmax = reinterpret_cast<float*>(at);

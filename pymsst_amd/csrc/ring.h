@@ -26,6 +26,20 @@ __device__ __forceinline__ void dma16_m0(const void* g, uint32_t lds) {
       : "memory");
 }
 
+// The same with 4 bytes per lane (lane l writes LDS byte lds + 4 l).
+__device__ __forceinline__ void dma4_m0(const void* g, uint32_t lds) {
+  uint32_t save;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(save)
+      : "v"(g), "s"(lds)
+      : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void ring_vm_wait(int n) {
   // s_waitcnt vmcnt(n) for a wave-uniform n <= N
