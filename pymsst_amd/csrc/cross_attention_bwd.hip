@@ -445,6 +445,204 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
   }
 }
 
+// ---------------------------------------------------------------- up to 64 keys, 16 bits
+
+// All gradients in one pass where a tile holds every key: a block of 2 waves keeps K and V in LDS and passes over
+// the row tiles of its pair.  A wave takes 32 rows: its whole row of P and dP is in registers, so D is summed from
+// them (unrounded, and O is not read: with few keys a rounded O would cost dQ and dK half a rounding more).  P and dS then go through LDS, rows down and keys across, to be the other
+// operand of dV and dK, of which each wave owns 32 keys.  5 products instead of 7, and every tensor is moved once:
+// 1032 x 62 queries over 62 keys, bf16, 8 heads of 64 take 128 us, of which the bytes need 88.
+// fp16: P is held at 2^14; dS at a power of two from its own largest magnitude in the row tile, and dK's sum is
+// brought to a tile's power when that is the smaller one.
+// Waves that share a SIMD: fp16's scaling and the dropped bits together pass the registers of two.
+template <typename T, int DP, bool DROP>
+constexpr int few_waves() { return DP == 128 || (DP == 64 && DROP && std::is_same<T, f16>::value) ? 1 : 2; }
+
+template <typename T, int DP, bool DROP>
+__global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T, DP, DROP>()))) void attn_bwd_few_kernel(BwdArgs a) {
+  constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32, PB = 64 * sizeof(T);
+  constexpr bool kHalf = std::is_same<T, f16>::value;
+  __shared__ __attribute__((aligned(16))) char kv[2][64 * DB];
+  __shared__ __attribute__((aligned(16))) char rows[2][64 * DB];
+  __shared__ __attribute__((aligned(16))) char ps[2][64 * PB];
+  __shared__ float most[2];
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t pair, split;
+  if (!locate(a.grid, pair, split)) return;
+  const Shape& s = a.s;
+  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
+  const int d_units = s.D * static_cast<int>(sizeof(T)) / 16;
+  const int count = key_count(a.km, b, s.M);
+  uint64_t seen = range_bits(0, count);
+  if (a.km.mask) seen &= __ballot(a.km.mask[b * a.km.stride + min(lane, s.M - 1)] != 0);
+  const int tiles = (s.R + 63) / 64;
+  const int t0 = static_cast<int>(split) * a.tiles_per_split;
+  const int t1 = min(tiles, t0 + a.tiles_per_split);
+  PhiloxKey key{};
+  if constexpr (DROP) key = philox_key(a.drop.rng);
+  const float factor = DROP ? a.drop.factor : 1.f;
+
+  Tile<T, DP, 64, 2> tile;  // no state: every move computes its addresses
+  tile.fetch_cut(kv[0], static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h, 0, s.M, d_units, [&](int i) { return i * a.ks.n; });
+  tile.fetch_cut(kv[1], static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h, 0, s.M, d_units, [&](int i) { return i * a.vs.n; });
+
+  f32x16_t dk[DT]{}, dv[DT]{};
+  constexpr int kNoSum = 100;  // above every exponent: nothing but zeros so far
+  int e_sum = kNoSum;          // dk is held at 2^e_sum
+  for (int t = t0; t < t1; ++t) {
+    if (t > t0) __syncthreads();  // the tiles of the rows before these have been read
+    auto at = [&](int i, const Strides& st) {
+      const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(i)));
+      return n * st.n + (hk * s.G + (i - n * s.G)) * st.h;
+    };
+    tile.fetch_cut(rows[0], static_cast<const T*>(a.q) + b * a.qs.b, t * 64, s.R, d_units, [&](int i) { return at(i, a.qs); });
+    tile.fetch_cut(rows[1], static_cast<const T*>(a.dout) + b * a.gs.b, t * 64, s.R, d_units, [&](int i) { return at(i, a.gs); });
+    const int r = t * 64 + 32 * wave + (lane & 31);
+    const bool row_ok = r < s.R;
+    const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(r))), head = hk * s.G + (r - n * s.G);
+    float base = -kInf;  // -lse in log2 units: a row that sees no key (and one past the end) has no weight
+    if (row_ok) {
+      const float lse = a.lse[(static_cast<int64_t>(b) * s.H + head) * s.N + n];
+      base = lse == -kInf ? -kInf : -lse * kLog2e;
+    }
+    vm_wait<0>();
+    if (t == t0 && (seen != ~uint64_t{0} || d_units != tile.UNITS)) {
+      tile.clear(kv[0], seen, d_units);
+      tile.clear(kv[1], seen, d_units);
+    }
+    if (d_units != tile.UNITS) {
+      tile.clear(rows[0], ~uint64_t{0}, d_units);
+      tile.clear(rows[1], ~uint64_t{0}, d_units);
+    }
+    __syncthreads();
+
+    const int at_lane = fresh<256>(lane);  // whatever DB: this kernel has no registers for addresses
+    uint32_t kept[2] = {0, 0};  // bit i: register i of the sub-tile
+    if constexpr (DROP) {
+      const uint64_t drop0 = drop_row(s, b, head, n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t w[4];
+        philox7(key, drop0 + static_cast<uint32_t>(2 * j + h), w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kept[j >> 1] |= philox_keep(w, i, a.drop.limit << 16) ? 1u << (8 * (j & 1) + i) : 0u;
+      }
+      hold(true);
+    }
+    f32x16_t p[2], ds[2];
+    {
+      u32x4_t f[NS];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) f[i] = row_frag<DB>(rows[0], 32 * wave + (at_lane & 31), i, h);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) p[u] = mma_rows<T, DP>(kv[0], u, f, at_lane);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) f[i] = row_frag<DB>(rows[1], 32 * wave + (at_lane & 31), i, h);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) ds[u] = mma_rows<T, DP>(kv[1], u, f, at_lane);
+    }
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t bits = static_cast<uint32_t>(seen >> (32 * u)) >> (8 * h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float w = where_bit(bits, reg_key(i), __builtin_amdgcn_exp2f(fmaf(p[u][i], a.scale_log2, base)), 0.f);
+        const float dw = DROP ? where_bit(kept[u], i, ds[u][i] * factor, 0.f) : ds[u][i];
+        sum[i & 1] = fmaf(w, dw, sum[i & 1]);
+        ds[u][i] = dw;
+        p[u][i] = w;
+      }
+    }
+    const float delta = half_sum(sum[0] + sum[1]);
+    float top = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        ds[u][i] = p[u][i] * (ds[u][i] - delta);
+        if constexpr (DROP) p[u][i] = where_bit(kept[u], i, p[u][i], 0.f);
+        if constexpr (kHalf) top = fmaxf(top, fabsf(ds[u][i]));
+      }
+    }
+    int e = 0;
+    if constexpr (kHalf) {
+      for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+      if (lane == 0) most[wave] = top;
+      __syncthreads();
+      top = fmaxf(most[0], most[1]);
+      e = top == 0.f ? kNoSum : scale_exponent(top, 15);
+      const float power = ldexpf(1.f, e);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          ds[u][i] *= power;
+          p[u][i] *= 16384.f;
+        }
+      }
+      // dk stays at the smaller power of two; this tile's dS are stored at it below
+      if (e < e_sum) {
+        const float down = e_sum == kNoSum ? 0.f : ldexpf(1.f, e - e_sum);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dk[dt][i] *= down;
+        }
+        e_sum = e;
+      }
+    }
+
+    f32x16_t dq[DT]{};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) mma_cols<T, DP>(kv[0], u, ds[u], dq, at_lane);
+    const int row = 32 * wave + (at_lane & 31);
+    if (row_ok) {
+      const int64_t to = (static_cast<int64_t>(b) * s.N + n) * s.H + head;
+      store_cols<T, DP>(static_cast<T*>(a.dq) + to * s.D, dq, kHalf ? ldexpf(a.scale, -e) : a.scale, s.D, h);
+    }
+
+    // [row][key] tiles: a lane writes its row's keys, 8 consecutive ones a unit
+    const float shift = kHalf ? ldexpf(1.f, e_sum - e) : 1.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (kHalf) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[u][i] *= shift;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int to = row * PB + 16 * ((4 * u + 2 * j + h) ^ swz<PB>(row));
+        *reinterpret_cast<u32x4_t*>(ps[0] + to) = pack8<T>(p[u], j);
+        *reinterpret_cast<u32x4_t*>(ps[1] + to) = pack8<T>(ds[u], j);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const u32x4_t pf = col_frag<PB>(ps[0], 16 * k, wave, at_lane), sf = col_frag<PB>(ps[1], 16 * k, wave, at_lane);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        dv[dt] = mma<T>(col_frag<DB>(rows[1], 16 * k, dt, at_lane), pf, dv[dt]);
+        dk[dt] = mma<T>(col_frag<DB>(rows[0], 16 * k, dt, at_lane), sf, dk[dt]);
+      }
+    }
+  }
+  // a transposed read hands lane l the key key_row(l % 32)
+  const int ki = 32 * wave + key_row(lane & 31);
+  if (ki >= s.M) return;
+  const float k_scale = kHalf ? ldexpf(a.scale, -e_sum) : a.scale, v_scale = kHalf ? factor / 16384.f : factor;
+  if (a.part_k) {
+    const int64_t to = ((static_cast<int64_t>(split) * a.grid.pairs + pair) * s.M + ki) * s.D;
+    store_cols_f32<T, DP>(a.part_k + to, dk, k_scale, s.D, h);
+    store_cols_f32<T, DP>(a.part_v + to, dv, v_scale, s.D, h);
+  } else {
+    const int64_t to = ((static_cast<int64_t>(b) * s.M + ki) * s.Hk + hk) * s.D;
+    store_cols<T, DP>(static_cast<T*>(a.dk) + to, dk, k_scale, s.D, h);
+    store_cols<T, DP>(static_cast<T*>(a.dv) + to, dv, v_scale, s.D, h);
+  }
+}
+
 // ---------------------------------------------------------------- partial sums
 
 // out[b, position, head, d] = sum over splits of part[split, pair, row, d]; positions x group rows per pair
@@ -471,6 +669,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, void* 
 // ---------------------------------------------------------------- host
 
 struct BwdPlan {
+  bool few;  // up to 64 keys of 16-bit types: attn_bwd_few_kernel (fp32's tiles would leave a CU one block of 2 waves)
   int nw_q, nw_k;
   int64_t q_tiles, q_splits, q_per, k_tiles, k_splits, k_per;
 };
@@ -492,8 +691,9 @@ BwdPlan plan_backward(const Shape& s, int dtype) {
   p.nw_k = s.M <= 64 && !wide ? 2 : 4;
   p.q_tiles = (int64_t{s.R} + 32 * p.nw_q - 1) / (32 * p.nw_q);
   p.k_tiles = (int64_t{s.M} + 32 * p.nw_k - 1) / (32 * p.nw_k);
+  p.few = s.M > 0 && s.M <= 64 && dtype != PMSST_F32;
   split(pairs * p.q_tiles, s.M, p.q_splits, p.q_per);
-  split(std::max<int64_t>(1, pairs * p.k_tiles), s.R, p.k_splits, p.k_per);
+  split(std::max<int64_t>(1, pairs * (p.few ? 1 : p.k_tiles)), s.R, p.k_splits, p.k_per);
   return p;
 }
 
@@ -504,8 +704,8 @@ struct BwdSpace {
 BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int dtype) {
   const size_t pairs = static_cast<size_t>(s.B) * s.Hk;
   BwdSpace w;
-  w.delta = align_up(pairs * align_up(s.R, 64) * 4, 256);
-  w.bound = dtype == PMSST_F16 ? align_up(pairs * kParts * 4, 256) : 0;
+  w.delta = p.few ? 0 : align_up(pairs * align_up(s.R, 64) * 4, 256);
+  w.bound = dtype == PMSST_F16 && !p.few ? align_up(pairs * kParts * 4, 256) : 0;
   w.part_q = p.q_splits > 1 ? align_up(static_cast<size_t>(p.q_splits) * pairs * s.R * s.D * 4, 256) : 0;
   w.part_k = p.k_splits > 1 ? align_up(static_cast<size_t>(p.k_splits) * pairs * s.M * s.D * 4, 256) : 0;
   w.total = 2 * w.delta + 2 * w.bound + w.part_q + 2 * w.part_k;
@@ -553,10 +753,27 @@ int launch_sum(const float* part, void* out, int64_t splits, const Shape& s, boo
   return check_launch("attn_sum_kernel");
 }
 
+template <typename T>
+int sum_keys(const BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+  const int rc = launch_sum<T>(a.part_k, a.dk, p.k_splits, a.s, true, stream);
+  return rc != PMSST_OK ? rc : launch_sum<T>(a.part_v, a.dv, p.k_splits, a.s, true, stream);
+}
+
 template <typename T, int DP>
 int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
   const bool drop = a.drop.limit != 0;
   const int64_t pairs = int64_t{a.s.B} * a.s.Hk;
+  if constexpr (sizeof(T) == 2) {
+    if (p.few) {
+      a.tiles_per_split = static_cast<int32_t>(p.k_per);
+      a.grid = make_grid(pairs, p.k_splits);
+      const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
+      if (drop) attn_bwd_few_kernel<T, DP, true><<<grid, 128, 0, stream>>>(a);
+      else attn_bwd_few_kernel<T, DP, false><<<grid, 128, 0, stream>>>(a);
+      const int rc = check_launch("attn_bwd_few_kernel");
+      return rc == PMSST_OK && a.part_k ? sum_keys<T>(a, p, stream) : rc;
+    }
+  }
   if constexpr (std::is_same<T, f16>::value) {
     attn_bound_kernel<T><<<dim3(static_cast<uint32_t>(pairs * kParts)), 256, 0, stream>>>(a);
     const int rc = check_launch("attn_bound_kernel");
@@ -572,9 +789,7 @@ int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
   a.tiles_per_split = static_cast<int32_t>(p.k_per);
   a.grid = make_grid(pairs, p.k_tiles * p.k_splits);
   rc = launch_dkv<T, DP>(a, p.nw_k, drop, stream);
-  if (rc != PMSST_OK || !a.part_k) return rc;
-  rc = launch_sum<T>(a.part_k, a.dk, p.k_splits, a.s, true, stream);
-  return rc != PMSST_OK ? rc : launch_sum<T>(a.part_v, a.dv, p.k_splits, a.s, true, stream);
+  return rc == PMSST_OK && a.part_k ? sum_keys<T>(a, p, stream) : rc;
 }
 
 template <typename T>
@@ -628,7 +843,7 @@ int pmsst_cross_attention_backward(const void* grad_out, const int64_t* grad_out
   PMSST_REQUIRE(rng || a.drop.limit == 0, "%s: null pointer (rng)", what);
   const BwdPlan p = plan_backward(a.s, dtype);
   const BwdSpace w = bwd_space(a.s, p, dtype);
-  if (workspace == nullptr || workspace_bytes < w.total)
+  if (w.total > 0 && (workspace == nullptr || workspace_bytes < w.total))
     return fail(PMSST_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, w.total, workspace_bytes);
   PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: workspace must be 16-byte aligned", what);
   a.q = q;

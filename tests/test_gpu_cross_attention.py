@@ -115,7 +115,7 @@ def test_c_abi_refusals():
     for bad in (dict(n=0), dict(n=-1), dict(d=12), dict(p=0.5), dict(p=1.5), dict(grad=None), dict(out=None), dict(lse=None),
                 dict(dq=None), dict(dq=odd), dict(grad=odd)):
         assert bwd(**bad) == -1, bad
-    assert bwd(ws=None) == -4 and bwd(size=16) == -4
+    assert bwd(m=300, ws=None) == -4 and bwd(m=300, size=16) == -4
     need = lib.pmsst_cross_attention_forward_workspace_size(1, 1, 20000, 8, 8, 64, 2)
     assert need > 0 and fwd(n=1, m=20000, h=8, hk=8, ws=one, size=need - 1) == -4
     assert lib.pmsst_cross_attention_forward_workspace_size(1, 1, 20000, 8, 3, 64, 2) == 0  # no such call
