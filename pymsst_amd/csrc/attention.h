@@ -206,7 +206,7 @@ __device__ __forceinline__ void mma_cols(const char* tile, int sub, const f32x16
                                                         4 * (d & 3));
         acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[dt], 0, 0, 0);
       }
-      hold(r % 2 == 1);
+      hold(DB == 512 ? r % 2 == 1 : r % 4 == 3);
     }
   }
 }
@@ -220,7 +220,7 @@ __device__ __forceinline__ f32x16_t mma_rows(const char* tile, int sub, const u3
 #pragma unroll
   for (int s = 0; s < DB / 32; ++s) {
     acc = mma<T>(row_frag<DB>(tile, row, s, lane >> 5), frag[s], acc);
-    if constexpr (sizeof(T) == 4) hold(s % 2 == 1);
+    if constexpr (sizeof(T) == 4) hold(DB == 512 ? s % 2 == 1 : s % 4 == 3);
   }
   return acc;
 }

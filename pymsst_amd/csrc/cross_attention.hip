@@ -237,10 +237,11 @@ struct FwdPlan {
 };
 
 // Waves of a block: 2 where that covers the rows (half a block of 4 would idle; fp32 rows of 512 bytes keep 4,
-// whose lanes hold half as much of a tile on its way), else 4.  Splits, of at least 256 keys each: up to 4 blocks
-// of 4 waves a CU, whose products bound them and whose ragged ends so even out (2760 queries over up to 8192 keys,
-// heads of 128: 235 us; with 2 blocks a CU 266, with 8 253), or 2 blocks of 2 waves, which the keys' bytes bound
-// (16 single queries over up to 16500 keys: 89 us; with 4 blocks 102).
+// whose lanes hold half as much of a tile on its way), else 4.  Splits: of at least 128 keys, up to 4 blocks of 4
+// waves a CU, whose products bound them and whose ragged ends so even out (2760 queries over up to 8192 keys,
+// heads of 128: 235 us; with 2 blocks a CU 266, with 8 253), or of at least 512 keys, up to 2 blocks of 2 waves, which the
+// keys' bytes bound (16 single queries over up to 16500 keys: 89 us; with 4 blocks 102; a tile of 64 keys takes about
+// 1 us and the second kernel 5).
 FwdPlan plan_forward(const Shape& s, int dtype) {
   FwdPlan p;
   const bool wide = padded_dim(s.D) * static_cast<int>(dtype_size(dtype)) == 512;
@@ -250,7 +251,7 @@ FwdPlan plan_forward(const Shape& s, int dtype) {
   const int64_t tiles = std::max<int64_t>(1, (int64_t{s.M} + p.bk - 1) / p.bk);
   const int64_t blocks = int64_t{s.B} * s.Hk * p.row_tiles, want = (p.nw == 4 ? 4 : 2) * num_cus();
   p.splits = 1;
-  if (blocks < want) p.splits = std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, int64_t{s.M} / 256));
+  if (blocks < want) p.splits = std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, int64_t{s.M} / (p.nw == 4 ? 128 : 512)));
   p.tiles_per_split = (tiles + p.splits - 1) / p.splits;
   p.splits = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
   return p;

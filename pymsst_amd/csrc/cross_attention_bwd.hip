@@ -674,7 +674,7 @@ struct BwdPlan {
   int64_t q_tiles, q_splits, q_per, k_tiles, k_splits, k_per;
 };
 
-// Splits as in the forward: as many as give every CU two blocks, of at least 256 keys (rows) each.
+// Splits as in the forward: as many as give every CU two blocks, of at least 128 keys (rows) each.
 BwdPlan plan_backward(const Shape& s, int dtype) {
   const bool wide = padded_dim(s.D) * static_cast<int>(dtype_size(dtype)) == 512;
   const int64_t bk = wide ? 32 : 64;
@@ -682,7 +682,7 @@ BwdPlan plan_backward(const Shape& s, int dtype) {
   auto split = [&](int64_t owners, int64_t along, int64_t& splits, int64_t& per) {
     const int64_t tiles = std::max<int64_t>(1, (along + bk - 1) / bk);
     splits = 1;
-    if (owners < want) splits = std::max<int64_t>(1, std::min((want + owners - 1) / owners, along / 256));
+    if (owners < want) splits = std::max<int64_t>(1, std::min((want + owners - 1) / owners, along / 128));
     per = (tiles + splits - 1) / splits;
     splits = (tiles + per - 1) / per;
   };

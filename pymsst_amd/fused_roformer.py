@@ -65,6 +65,13 @@ EXPERIMENTAL_FUSED_MEL_BANDS_ENV = "PYMSST_EXPERIMENTAL_FUSED_MEL_BANDS"
 # fill) of the BS-RoFormer output in one HIP pass each way.
 EXPERIMENTAL_FUSED_MASK_APPLY_ENV = "PYMSST_EXPERIMENTAL_FUSED_MASK_APPLY"
 
+# This build's addition: attention itself on the HIP cross attention kernels in place of SDPA (its dropout drawn
+# by counter instead of torch's generator stream), in training and evaluation.
+EXPERIMENTAL_FUSED_ATTENTION_ENV = "PYMSST_EXPERIMENTAL_FUSED_ATTENTION"
+# This build's addition: the blocks' dropouts without stored masks, the feed-forward's behind its GELU, the last of
+# each block before its residual sum (training with attn_dropout / ff_dropout above 0).
+EXPERIMENTAL_FUSED_DROPOUT_ENV = "PYMSST_EXPERIMENTAL_FUSED_DROPOUT"
+
 _TRUE = {"1", "true", "yes", "on"}
 _FLOAT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 
@@ -129,6 +136,8 @@ class FusedTrainingStatus:
     patched_mask_mlp: bool = False  # this build's addition (hidden Linear + tanh fused as well)
     patched_mel_bands: bool = False  # this build's addition (Mel-band gather / mask scatter)
     patched_mask_apply: bool = False  # this build's addition (mask product in the iSTFT layout)
+    patched_attention: bool = False  # this build's addition (attention in place of SDPA)
+    patched_dropout: bool = False  # this build's addition (dropouts without stored masks)
 
 
 # ---------------------------------------------------------------------- switchboard
@@ -263,9 +272,11 @@ def apply_roformer_fused_training_backend(
     mask_mlp = final and _mask_mlp_enabled(ext)
     mel_bands = _patch_mel_bands(ext) if _flag(EXPERIMENTAL_FUSED_MEL_BANDS_ENV) else False
     mask_apply = _patch_mask_apply(ext) if _flag(EXPERIMENTAL_FUSED_MASK_APPLY_ENV) else False
+    attention = _patch_core_attention(ext) if _flag(EXPERIMENTAL_FUSED_ATTENTION_ENV) else False
+    dropouts = _patch_core_dropout(ext) if _flag(EXPERIMENTAL_FUSED_DROPOUT_ENV) else False
 
     if not any((n_band_splits, single_stem, rotary, rms, gates, grouped_linear, layout, pack_autograd, final_autograd,
-                final, mel_bands, mask_apply)):
+                final, mel_bands, mask_apply, attention, dropouts)):
         reason = "no compatible BandSplit modules were found"
         warnings.warn(reason, RuntimeWarning, stacklevel=2)
         return FusedTrainingStatus(requested=normalized, active="off", reason=reason)
@@ -295,6 +306,8 @@ def apply_roformer_fused_training_backend(
         patched_mask_mlp=mask_mlp,
         patched_mel_bands=mel_bands,
         patched_mask_apply=mask_apply,
+        patched_attention=attention,
+        patched_dropout=dropouts,
     )
 
 
@@ -462,6 +475,79 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
     attention_forward_cuda_ext._pymsst_fused_attention_gate_mode = mode
     attention_forward_cuda_ext._pymsst_original_forward = original
     transformer.Attention.forward = attention_forward_cuda_ext
+    return True
+
+
+def _patch_core_attention(ext: Any) -> bool:
+    """Module-level ``_sdpa`` replacement (no reference counterpart: the stock and the gate-patched ``Attention``
+    both call PyTorch's SDPA).  What the kernels do not take (CPU, fp64, mixed dtypes, other head dimensions) goes
+    to the original."""
+    if any(not hasattr(ext, n) for n in ("cross_attention_forward", "cross_attention_backward")):
+        return False
+    _, transformer, _ = _core()
+    if getattr(transformer._sdpa, "_pymsst_fused_attention", False):
+        return True
+    original = transformer._sdpa
+
+    def sdpa_cuda_ext(q, k, v, dropout_p):
+        d = q.shape[-1]
+        if (not q.is_cuda or q.dtype not in _FLOAT_TYPES or k.dtype != q.dtype or v.dtype != q.dtype or d % 8
+                or not 8 <= d <= 128):
+            return original(q, k, v, dropout_p)
+        out = cross_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), dropout_p=dropout_p, extension=ext)
+        return out.transpose(1, 2)
+
+    sdpa_cuda_ext._pymsst_fused_attention = True
+    sdpa_cuda_ext._pymsst_original_sdpa = original
+    transformer._sdpa = sdpa_cuda_ext
+    return True
+
+
+def _patch_core_dropout(ext: Any) -> bool:
+    """Class-level ``FeedForward.forward`` and ``Transformer.forward`` replacement (no reference counterpart): the
+    hidden layer's GELU and dropout in one pass, each block's last dropout in one with its residual sum."""
+    if any(not hasattr(ext, n) for n in ("dropout_forward", "dropout_backward")):
+        return False
+    _, transformer, _ = _core()
+    if getattr(transformer.Transformer.forward, "_pymsst_fused_dropout", False):
+        return True
+    original_ff, original = transformer.FeedForward.forward, transformer.Transformer.forward
+
+    def feed_forward_cuda_ext(self, x):
+        norm, up, act, drop, down, last = self.net
+        if not self.training or not x.is_cuda or drop.p <= 0 or drop.p >= 1 or act.approximate != "none":
+            return original_ff(self, x)
+        h = up(norm(x))
+        if h.dtype not in _FLOAT_TYPES:
+            return last(down(drop(act(h))))
+        return last(down(dropout(h, drop.p, activation="gelu", extension=ext)))
+
+    def residual_block(block, last, x):
+        p = last.p
+        if not block.training or not x.is_cuda or p <= 0 or p >= 1:
+            return block(x) + x
+        last.p = 0.0  # the block's own call of its last dropout: passes its input on
+        try:
+            y = block(x)
+        finally:
+            last.p = p
+        if y.dtype not in _FLOAT_TYPES:
+            return F.dropout(y, p) + x
+        if y.dtype != x.dtype:
+            return dropout(y, p, extension=ext) + x
+        return dropout(y, p, residual=x, extension=ext)
+
+    def transformer_cuda_ext(self, x):
+        for attn, ff in self.layers:
+            x = residual_block(attn, attn.to_out[1], x)
+            x = residual_block(ff, ff.net[5], x)
+        return self.norm(x)
+
+    feed_forward_cuda_ext._pymsst_original_forward = original_ff
+    transformer_cuda_ext._pymsst_fused_dropout = True
+    transformer_cuda_ext._pymsst_original_forward = original
+    transformer.FeedForward.forward = feed_forward_cuda_ext
+    transformer.Transformer.forward = transformer_cuda_ext
     return True
 
 
@@ -1390,6 +1476,74 @@ class _FusedAttentionGate(torch.autograd.Function):
         return grad_attn.reshape(ctx.attn_shape), grad_x.reshape(ctx.x_shape), grad_weight, grad_bias, None
 
 
+class _FusedCrossAttention(torch.autograd.Function):
+    """Attention of ``q[B,N,H,D]`` over ``k`` / ``v[B,M,Hk,D]`` (this build's addition); saves the output and the
+    rows' log-sums, no weights and no mask."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, key_mask, key_lengths, scale, dropout_p, rng, extension):
+        kw = dict(key_mask=key_mask, key_lengths=key_lengths, scale=scale, dropout_p=dropout_p, rng=rng)
+        if not any(ctx.needs_input_grad[:3]):
+            return extension.cross_attention_forward(q, k, v, **kw)[0]
+        out, lse = extension.cross_attention_forward(q, k, v, need_lse=True, **kw)
+        ctx.save_for_backward(q, k, v, out, lse, key_mask, key_lengths, rng)
+        ctx.scale, ctx.dropout_p, ctx.extension = scale, dropout_p, extension
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, key_mask, key_lengths, rng = ctx.saved_tensors
+        grads = ctx.extension.cross_attention_backward(grad_out, q, k, v, out, lse, key_mask, key_lengths, ctx.scale,
+                                                       ctx.dropout_p, rng)
+        return (*grads, None, None, None, None, None, None)
+
+
+class _FusedDropout(torch.autograd.Function):
+    """``dropout(act(x)) + residual`` (this build's addition); saves the seed and offset, and ``x`` for a GELU."""
+
+    @staticmethod
+    def forward(ctx, x, residual, p, rng, activation, extension):
+        ctx.save_for_backward(x if activation else None, rng)
+        ctx.p, ctx.activation, ctx.extension = p, activation, extension
+        return extension.dropout_forward(x, p, rng, activation=activation, residual=residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        x, rng = ctx.saved_tensors
+        grad_x = None
+        if ctx.needs_input_grad[0]:
+            grad_x = ctx.extension.dropout_backward(grad_out, ctx.p, rng, x=x, activation=ctx.activation)
+        return grad_x, grad_out if ctx.needs_input_grad[1] else None, None, None, None, None
+
+
+def draw_rng(device) -> torch.Tensor:
+    """A seed and offset for one dropout call, from torch's generator of ``device``: ``torch.manual_seed`` repeats
+    them, activation checkpointing draws them again, and a captured graph draws new ones on every replay."""
+    return torch.empty(2, dtype=torch.int64, device=device).random_()
+
+
+def cross_attention(q, k, v, *, key_mask=None, key_lengths=None, scale=None, dropout_p: float = 0.0, rng=None,
+                    extension=None) -> torch.Tensor:
+    """Differentiable ``softmax(scale q k^T) v`` of ``q[B, N, H, D]`` over another stream's ``k`` / ``v[B, M, Hk, D]``
+    (see ``HipFusedExtension.cross_attention_forward`` for masks, shared heads and layouts).  ``rng`` is drawn from
+    torch's generator where ``dropout_p`` needs one and none is given."""
+    ext = extension if extension is not None else load_fused_band_split_extension()
+    if dropout_p > 0.0 and rng is None:
+        rng = draw_rng(q.device)
+    return _FusedCrossAttention.apply(q, k, v, key_mask, key_lengths, scale, float(dropout_p), rng, ext)
+
+
+def dropout(x, p: float, *, activation=None, residual=None, rng=None, extension=None) -> torch.Tensor:
+    """Differentiable ``dropout(act(x)) + residual`` without a stored mask (``activation``: ``None`` or ``"gelu"``).
+    ``rng`` is drawn from torch's generator where ``p`` needs one and none is given."""
+    ext = extension if extension is not None else load_fused_band_split_extension()
+    if p > 0.0 and rng is None:
+        rng = draw_rng(x.device)
+    return _FusedDropout.apply(x, residual, float(p), rng, activation, ext)
+
+
 class _FusedRotary(torch.autograd.Function):
     """fr.py:1154-1166; ``cos``/``sin`` are the ``[..., ::2]`` views (no copy is made)."""
 
@@ -1496,6 +1650,9 @@ _CORE_PATCH_POINTS = (
     ("transformer", None, "apply_rotary_emb_fast", "_pymsst_original_apply_rotary"),
     ("transformer", "RMSNorm", "forward", "_pymsst_original_forward"),
     ("transformer", "Attention", "forward", "_pymsst_original_forward"),
+    ("transformer", "FeedForward", "forward", "_pymsst_original_forward"),
+    ("transformer", "Transformer", "forward", "_pymsst_original_forward"),
+    ("transformer", None, "_sdpa", "_pymsst_original_sdpa"),
     ("bands", None, "grouped_linear", "_pymsst_original_grouped_linear"),
     ("bands", "MaskEstimator", "_forward_layer_grouped_mlp", "_pymsst_original_forward_layer_grouped_mlp"),
     ("bands", "MaskEstimator", "_get_layer_group_params", "_pymsst_original_get_layer_group_params"),
@@ -1549,6 +1706,9 @@ __all__ = [
     "RUNTIME_PRESETS",
     "apply_roformer_fused_training_backend",
     "apply_runtime_preset",
+    "cross_attention",
+    "draw_rng",
+    "dropout",
     "load_fused_band_split_extension",
     "normalize_fused_kernel_backend",
     "normalize_fused_rms_norm_mode",
