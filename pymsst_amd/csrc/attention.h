@@ -183,18 +183,26 @@ __device__ __forceinline__ int fresh(int lane) {
   return lane;
 }
 
+// acc[dt] += (tile rows sub*32 .. + 31)^T * b, b the two 16-row fragments of a score tile (16-bit types).
+template <typename T, int DP>
+__device__ __forceinline__ void mma_cols(const char* tile, int sub, const u32x4_t (&b)[2], f32x16_t (&acc)[DP / 32], int lane) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) {
+      acc[dt] = mma<T>(col_frag<DP * sizeof(T)>(tile, 32 * sub + 16 * s, dt, lane), b[s], acc[dt]);
+    }
+  }
+}
+
 // acc[dt] += (tile rows sub*32 .. + 31)^T * p, for every 32 columns of the head dimension: p is a score tile
 // whose k index is the tile's row.
 template <typename T, int DP>
 __device__ __forceinline__ void mma_cols(const char* tile, int sub, const f32x16_t& p, f32x16_t (&acc)[DP / 32], int lane) {
   constexpr int DB = DP * sizeof(T);
   if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const u32x4_t b = pack8<T>(p, s);
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = mma<T>(col_frag<DB>(tile, 32 * sub + 16 * s, dt, lane), b, acc[dt]);
-    }
+    const u32x4_t b[2] = {pack8<T>(p, 0), pack8<T>(p, 1)};
+    mma_cols<T, DP>(tile, sub, b, acc, lane);
   } else {
     const int h = lane >> 5, d = lane & 31;
 #pragma unroll

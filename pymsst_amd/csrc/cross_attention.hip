@@ -164,13 +164,27 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
         p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.scale_log2, base));
         l[i & 1] += p[i];
       }
+      if constexpr (DROP && sizeof(T) == 2) {
+        // a word of random bits is two elements, as a word of the packed weights is
+        u32x4_t pb[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t w[4];
+          philox7(key, drop0 + static_cast<uint32_t>(t * (BK / 8) + 4 * u + 2 * j + h), w);
+          pb[j] = pack8<T>(p, j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pb[j][i] &= ~philox_dropped(w[i], a.drop.limit);
+        }
+        mma_cols<T, DP>(vl, u, pb, o, at_lane);
+        continue;
+      }
       if constexpr (DROP) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint32_t w[4];
           philox7(key, drop0 + static_cast<uint32_t>(t * (BK / 8) + 4 * u + 2 * j + h), w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) p[8 * j + i] = philox_keep(w, i, a.drop.limit << 16) ? p[8 * j + i] : 0.f;
+          for (int i = 0; i < 8; ++i) p[8 * j + i] = philox_keep(w, i, a.drop.limit) ? p[8 * j + i] : 0.f;
         }
       }
       mma_cols<T, DP>(vl, u, p, o, at_lane);

@@ -257,7 +257,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
           philox7(key, drop0 + static_cast<uint32_t>(t * (BK / 8) + 4 * u + 2 * j + h), w);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            dp[8 * j + i] = philox_keep(w, i, a.drop.limit << 16) ? dp[8 * j + i] * a.drop.factor : 0.f;
+            dp[8 * j + i] = philox_keep(w, i, a.drop.limit) ? dp[8 * j + i] * a.drop.factor : 0.f;
           }
         }
       }
@@ -395,10 +395,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(i)));
             uint32_t w[4];
             philox7(key, drop_row(s, b, hk * s.G + (i - n * s.G), n) + static_cast<uint32_t>(key0 / 8 + blk), w);
-            uint32_t bits = 0;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) bits |= philox_keep(w, c, a.drop.limit << 16) ? 1u << c : 0u;
-            reinterpret_cast<uint8_t*>(kept[wave])[idx] = static_cast<uint8_t>(bits);
+            reinterpret_cast<uint8_t*>(kept[wave])[idx] = static_cast<uint8_t>(philox_kept8(w, a.drop.limit));
           }
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
@@ -411,9 +408,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
           const int row = reg_key(i) + 8 * h;
           p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.scale_log2, base[32 * u + row]));
           if constexpr (DROP) {
-            const bool keep = (kept[wave][row] >> (lane & 31)) & 1;
-            ds[i] = p[i] * ((keep ? ds[i] * dp_scale : 0.f) - delta[32 * u + row]);
-            p[i] = keep ? p[i] : 0.f;
+            const uint32_t keep = kept[wave][row];
+            ds[i] = p[i] * (where_bit(keep, lane & 31, ds[i] * dp_scale, 0.f) - delta[32 * u + row]);
+            p[i] = where_bit(keep, lane & 31, p[i], 0.f);
           } else {
             ds[i] = p[i] * fmaf(ds[i], dp_scale, -delta[32 * u + row]);
           }
@@ -524,8 +521,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
       for (int j = 0; j < 4; ++j) {
         uint32_t w[4];
         philox7(key, drop0 + static_cast<uint32_t>(2 * j + h), w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) kept[j >> 1] |= philox_keep(w, i, a.drop.limit << 16) ? 1u << (8 * (j & 1) + i) : 0u;
+        kept[j >> 1] |= philox_kept8(w, a.drop.limit) << (8 * (j & 1));
       }
       hold(true);
     }

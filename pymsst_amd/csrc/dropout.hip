@@ -112,7 +112,7 @@ __device__ __forceinline__ void drop8(float (&v)[8], const float (&u)[8], uint64
     uint32_t w[4];
     philox7(key, block, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = philox_keep(w, i, d.limit << 16) ? v[i] * d.factor : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = philox_keep(w, i, d.limit) ? v[i] * d.factor : 0.f;
   }
   if constexpr (SECOND && !BACK) {
 #pragma unroll

@@ -37,9 +37,9 @@ __device__ __forceinline__ void philox7(const PhiloxKey& key, uint64_t block, ui
   for (int r = 0; r < 7; ++r) {
     const uint64_t p0 = static_cast<uint64_t>(c0) * 0xD2511F53u;
     const uint64_t p1 = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-    c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k0;
+    c0 = __builtin_amdgcn_bitop3_b32(static_cast<uint32_t>(p1 >> 32), c1, k0, 0x96);  // a ^ b ^ c
     c1 = static_cast<uint32_t>(p1);
-    c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k1;
+    c2 = __builtin_amdgcn_bitop3_b32(static_cast<uint32_t>(p0 >> 32), c3, k1, 0x96);
     c3 = static_cast<uint32_t>(p0);
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
@@ -50,10 +50,25 @@ __device__ __forceinline__ void philox7(const PhiloxKey& key, uint64_t block, ui
   w[3] = c3;
 }
 
-// Whether element `e` (0..7) of the block is kept; `limit16` = limit << 16.  A high half is compared in
-// place: its word is at least limit16 exactly where its high half is at least limit.
-__device__ __forceinline__ bool philox_keep(const uint32_t (&w)[4], int e, uint32_t limit16) {
-  return ((e & 1) ? w[e >> 1] : w[e >> 1] << 16) >= limit16;
+// Whether element `e` (0..7) of the block is kept.
+__device__ __forceinline__ bool philox_keep(const uint32_t (&w)[4], int e, uint32_t limit) {
+  return static_cast<uint16_t>((e & 1) ? w[e >> 1] >> 16 : w[e >> 1]) >= static_cast<uint16_t>(limit);
+}
+
+// The same of both elements of a word: all ones in the half of one that is dropped.  A saturating difference of
+// the halves, taken as signed numbers (both less 2^15), has the sign of the comparison.
+__device__ __forceinline__ uint32_t philox_dropped(uint32_t w, uint32_t limit) {
+  typedef short v2 __attribute__((ext_vector_type(2)));
+  const v2 r = __builtin_bit_cast(v2, w ^ 0x80008000u), l = __builtin_bit_cast(v2, (limit ^ 0x8000u) * 0x10001u);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(r, l) >> static_cast<short>(15));
+}
+
+// The kept elements of a block as a byte, element e in bit e.
+__device__ __forceinline__ uint32_t philox_kept8(const uint32_t (&w)[4], uint32_t limit) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bits |= ~philox_dropped(w[i], limit) & ((1u << (2 * i)) | (1u << (17 + 2 * i)));
+  return (bits | bits >> 16) & 0xFFu;
 }
 
 // Host: limit and factor of a probability in [0, 1).
