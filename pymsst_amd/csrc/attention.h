@@ -282,7 +282,7 @@ struct Tile {
     }
   }
   static __device__ __forceinline__ uint32_t target(const char* tile, int i) {
-    return lds_addr(tile) + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64) * 1024 + i * NW * 1024;
+    return __builtin_amdgcn_readfirstlane(lds_addr(tile) + static_cast<uint32_t>(threadIdx.x) / 64 * 1024) + i * NW * 1024;
   }
   // Starts a whole tile's move; the pointers go on by `step` bytes.
   __device__ __forceinline__ void fetch(const char* tile, int64_t step) {
@@ -312,10 +312,9 @@ struct Tile {
   }
 };
 
-// Two tiles a stage; a stage is filled STAGES - 1 tiles ahead.  Rows of up to 128 bytes have three stages (48 KB,
-// three blocks of 4 waves a CU); longer ones, and blocks of 2 waves, which LDS would keep from sharing a CU, two.
-template <int DB, int NW>
-constexpr int stages() { return DB <= 128 && NW == 4 ? 3 : 2; }
+// Tiles lie in two stages: while one is multiplied, the next one's move fills the other.  (Three stages hold more
+// LDS than the wait they save is worth: 124 x 948 queries, forward 365 us, with two 330.)
+constexpr int kStages = 2;
 
 // Uses a loaded register here, so that the compiler waits for the load here and not (for every load in flight)
 // inside the loop.

@@ -46,9 +46,8 @@ template <typename T, int DP, int NW, bool DROP>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 ? 1 : 2))) void attn_fwd_kernel(FwdArgs a) {
   constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
   constexpr int BK = fwd_keys<T, DP>(), SUBS = BK / 32;
-  constexpr int S = stages<DB, NW>();
-  __shared__ __attribute__((aligned(16))) char lds[S][2][BK * DB];
-  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+  __shared__ __attribute__((aligned(16))) char lds[kStages][2][BK * DB];
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t pair, sub_block;
   if (!locate(a.grid, pair, sub_block)) return;
   const uint32_t split = sub_block / a.row_tiles, row_tile = sub_block - split * a.row_tiles;
@@ -102,10 +101,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
   };
   arrive(qf);
   if (mask && t0 < t1) byte_next = mask_byte(t0);
-#pragma unroll
-  for (int i = 0; i < S - 1; ++i) {
-    if (t0 + i < t1) fetch(t0 + i, i);
-  }
+  if (t0 < t1) fetch(t0, 0);
   int stage = 0;
   for (int t = t0; t < t1; ++t) {
     char* kl = lds[stage][0];
@@ -118,16 +114,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
     }
     if constexpr (BK == 32) seen &= 0xFFFFFFFFu;
     constexpr uint64_t kAll = BK == 64 ? ~uint64_t{0} : 0xFFFFFFFFu;
-    // this tile has arrived once only the next ones' moves are in flight
-    if (S == 3 && !mask && t + 1 < t1) vm_wait<2 * kt.CH>();
-    else vm_wait<0>();
+    vm_wait<0>();  // this wave's moves of the tile have arrived
     if (seen != kAll || d_units != kt.UNITS) {
       kt.clear(kl, seen, d_units);
       vt.clear(vl, seen, d_units);
     }
     __syncthreads();
-    if (t + S - 1 < t1) fetch(t + S - 1, stage == 0 ? S - 1 : stage - 1);
-    stage = stage == S - 1 ? 0 : stage + 1;
+    if (t + 1 < t1) fetch(t + 1, stage ^ 1);
+    stage ^= 1;
     if (idle) continue;
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {

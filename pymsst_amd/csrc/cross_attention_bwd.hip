@@ -75,12 +75,15 @@ __global__ __launch_bounds__(256) void attn_bound_kernel(BwdArgs a) {
   const int part = static_cast<int>(blockIdx.x % kParts);
   const Shape& s = a.s;
   const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
-  const int units = s.D / 8, lane_u = threadIdx.x & 15, row_u = threadIdx.x >> 4;  // 16 lanes a row
+  // 4, 8 or 16 lanes a row, 16 bytes each
+  const int units = s.D / 8, log_lanes = units <= 4 ? 2 : units <= 8 ? 3 : 4;
+  const int lane_u = threadIdx.x & ((1 << log_lanes) - 1), row_u = threadIdx.x >> log_lanes, step = 256 >> log_lanes;
   const int count = key_count(a.km, b, s.M);
   const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
   const T* gb = static_cast<const T*>(a.dout) + b * a.gs.b;
   float vm = 0.f, lm = 0.f;
-  for (int64_t m = part * 16 + row_u; m < count; m += 16 * kParts) {
+#pragma unroll 4
+  for (int64_t m = part * step + row_u; m < count; m += step * kParts) {
     if (a.km.mask && a.km.mask[b * a.km.stride + m] == 0) continue;
     if (lane_u < units) {
       float x[8];
@@ -89,7 +92,8 @@ __global__ __launch_bounds__(256) void attn_bound_kernel(BwdArgs a) {
       for (int i = 0; i < 8; ++i) vm = fmaxf(vm, fabsf(x[i]));
     }
   }
-  for (int64_t r = part * 16 + row_u; r < s.R; r += 16 * kParts) {
+#pragma unroll 4
+  for (int64_t r = part * step + row_u; r < s.R; r += step * kParts) {
     const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(r))), head = hk * s.G + static_cast<int>(r) - n * s.G;
     float sum = 0.f;
     if (lane_u < units) {
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(256) void attn_bound_kernel(BwdArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum += fabsf(x[i]);
     }
-    lm = fmaxf(lm, group_sum(sum, 16));
+    lm = fmaxf(lm, group_sum(sum, 1 << log_lanes));
   }
   for (int off = 32; off > 0; off >>= 1) {
     vm = fmaxf(vm, __shfl_xor(vm, off, kWave));
@@ -121,8 +125,7 @@ template <typename T, int DP, int NW, bool DROP>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 ? 1 : 2))) void attn_dq_kernel(BwdArgs a) {
   constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
   constexpr int BK = bwd_tile<T, DP>(), SUBS = BK / 32;
-  constexpr int S = stages<DB, NW>();
-  __shared__ __attribute__((aligned(16))) char lds[S][2][BK * DB];
+  __shared__ __attribute__((aligned(16))) char lds[kStages][2][BK * DB];
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
   uint32_t pair, sub_block;
   if (!locate(a.grid, pair, sub_block)) return;
@@ -216,10 +219,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
   arrive(gf);
   asm volatile("" : "+v"(base), "+v"(delta));
   if (mask && t0 < t1) byte_next = mask_byte(t0);
-#pragma unroll
-  for (int i = 0; i < S - 1; ++i) {
-    if (t0 + i < t1) fetch(t0 + i, i);
-  }
+  if (t0 < t1) fetch(t0, 0);
   int stage = 0;
   for (int t = t0; t < t1; ++t) {
     char* kl = lds[stage][0];
@@ -232,16 +232,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
     }
     if constexpr (BK == 32) seen &= 0xFFFFFFFFu;
     constexpr uint64_t kAll = BK == 64 ? ~uint64_t{0} : 0xFFFFFFFFu;
-    // this tile has arrived once only the next ones' moves are in flight
-    if (S == 3 && !mask && t + 1 < t1) vm_wait<2 * kt.CH>();
-    else vm_wait<0>();
+    vm_wait<0>();  // this wave's moves of the tile have arrived
     if (seen != kAll || d_units != kt.UNITS) {
       kt.clear(kl, seen, d_units);
       vt.clear(vl, seen, d_units);
     }
     __syncthreads();
-    if (t + S - 1 < t1) fetch(t + S - 1, stage == 0 ? S - 1 : stage - 1);
-    stage = stage == S - 1 ? 0 : stage + 1;
+    if (t + 1 < t1) fetch(t + 1, stage ^ 1);
+    stage ^= 1;
     if (idle) continue;
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
@@ -290,9 +288,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
   constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
   constexpr int BQ = bwd_tile<T, DP>(), SUBS = BQ / 32;
   constexpr bool kHalf = std::is_same<T, f16>::value;
-  constexpr int S = stages<DB, NW>();
-  __shared__ __attribute__((aligned(16))) char lds[S][2][BQ * DB];
-  __shared__ __attribute__((aligned(16))) float stat[S][2][64];  // -lse (log2 units), D
+  __shared__ __attribute__((aligned(16))) char lds[kStages][2][BQ * DB];
+  __shared__ __attribute__((aligned(16))) float stat[kStages][2][64];  // -lse (log2 units), D
   __shared__ __attribute__((aligned(16))) uint32_t kept[DROP ? NW : 1][DROP ? 32 : 4];
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
   uint32_t pair, sub_block;
@@ -355,33 +352,25 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         qt.fetch_cut(lds[stage][0], qb, row0, s.R, d_units, q_at);
         gt.fetch_cut(lds[stage][1], gb, row0, s.R, d_units, g_at);
       }
-      if (wave0 < 2 && (BQ == 64 || lane < BQ)) dma4_m0(stat_src + row0, lds_addr(stat[stage]) + 256 * wave0);
+      if (wave0 < 2 && (BQ == 64 || lane < BQ)) dma4_m0(stat_src + row0, __builtin_amdgcn_readfirstlane(lds_addr(stat[stage]) + 256 * wave0));
     };
     arrive(kf);
     arrive(vf);
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i) {
-      if (t0 + i < t1) fetch(t0 + i, i);
-    }
+    if (t0 < t1) fetch(t0, 0);
     int stage = 0;
     for (int t = t0; t < t1; ++t) {
       char* ql = lds[stage][0];
       char* gl = lds[stage][1];
       const float* base = stat[stage][0];
       const float* delta = stat[stage][1];
-      if (S == 3 && t + 1 < t1) {
-        if (wave0 < 2) vm_wait<2 * qt.CH + 1>();
-        else vm_wait<2 * qt.CH>();
-      } else {
-        vm_wait<0>();
-      }
+      vm_wait<0>();  // this wave's moves of the tile have arrived
       if (d_units != qt.UNITS) {
         qt.clear(ql, ~uint64_t{0}, d_units);
         gt.clear(gl, ~uint64_t{0}, d_units);
       }
       __syncthreads();
-      if (t + S - 1 < t1) fetch(t + S - 1, stage == 0 ? S - 1 : stage - 1);
-      stage = stage == S - 1 ? 0 : stage + 1;
+      if (t + 1 < t1) fetch(t + 1, stage ^ 1);
+      stage ^= 1;
       if (idle) continue;
 #pragma unroll
       for (int u = 0; u < SUBS; ++u) {
@@ -642,11 +631,15 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
 // ---------------------------------------------------------------- partial sums
 
 // out[b, position, head, d] = sum over splits of part[split, pair, row, d]; positions x group rows per pair
-// (group 1 for the keys).  A thread takes 4 columns.
+// (group 1 for the keys, whose two gradients are the grid's y).  A thread takes 4 columns.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, void* out, int splits, int64_t pairs,
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, void* out, const float* part1, void* out1, int splits, int64_t pairs,
                                                        int32_t heads, int32_t kv_heads, int32_t group, int32_t positions,
                                                        int32_t dim) {
+  if (blockIdx.y != 0) {
+    part = part1;
+    out = out1;
+  }
   const int64_t quads = dim / 4, rows = static_cast<int64_t>(positions) * group, total = pairs * rows * quads;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= total) return;
@@ -741,18 +734,21 @@ int launch_dkv(const BwdArgs& a, int nw, bool drop, hipStream_t stream) {
 }
 
 template <typename T>
-int launch_sum(const float* part, void* out, int64_t splits, const Shape& s, bool keys, hipStream_t stream) {
-  const int64_t pairs = int64_t{s.B} * s.Hk, rows = keys ? s.M : s.R;
-  const int64_t blocks = (pairs * rows * (s.D / 4) + 255) / 256;
+int sum_rows(const BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+  const Shape& s = a.s;
+  const int64_t pairs = int64_t{s.B} * s.Hk, blocks = (pairs * s.R * (s.D / 4) + 255) / 256;
   attn_sum_kernel<T><<<dim3(static_cast<uint32_t>(blocks)), 256, 0, stream>>>(
-      part, out, static_cast<int>(splits), pairs, keys ? s.Hk : s.H, s.Hk, keys ? 1 : s.G, keys ? s.M : s.N, s.D);
+      a.part_q, a.dq, nullptr, nullptr, static_cast<int>(p.q_splits), pairs, s.H, s.Hk, s.G, s.N, s.D);
   return check_launch("attn_sum_kernel");
 }
 
 template <typename T>
 int sum_keys(const BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
-  const int rc = launch_sum<T>(a.part_k, a.dk, p.k_splits, a.s, true, stream);
-  return rc != PMSST_OK ? rc : launch_sum<T>(a.part_v, a.dv, p.k_splits, a.s, true, stream);
+  const Shape& s = a.s;
+  const int64_t pairs = int64_t{s.B} * s.Hk, blocks = (pairs * s.M * (s.D / 4) + 255) / 256;
+  attn_sum_kernel<T><<<dim3(static_cast<uint32_t>(blocks), 2), 256, 0, stream>>>(
+      a.part_k, a.dk, a.part_v, a.dv, static_cast<int>(p.k_splits), pairs, s.Hk, s.Hk, 1, s.M, s.D);
+  return check_launch("attn_sum_kernel");
 }
 
 template <typename T, int DP>
@@ -779,7 +775,7 @@ int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
   a.tiles_per_split = static_cast<int32_t>(p.q_per);
   a.grid = make_grid(pairs, p.q_tiles * p.q_splits);
   int rc = launch_dq<T, DP>(a, p.nw_q, drop, stream);
-  if (rc == PMSST_OK && a.part_q) rc = launch_sum<T>(a.part_q, a.dq, p.q_splits, a.s, false, stream);
+  if (rc == PMSST_OK && a.part_q) rc = sum_rows<T>(a, p, stream);
   if (rc != PMSST_OK || a.s.M == 0) return rc;
   a.tiles = static_cast<uint32_t>(p.k_tiles);
   a.tiles_per_split = static_cast<int32_t>(p.k_per);
