@@ -9,7 +9,8 @@
 // tail keeps its digits.  The derivative Phi(x) + x phi(x) shares the exponential.
 //
 // A thread takes whole blocks of 8 elements (one Philox block, 16 bytes of a 16-bit type).  Bound: HBM
-// (x and y, or dy, x and dx, once each).
+// (x and y, or dy, x and dx, once each): 63984 x 768 bf16 with a GELU 37 us forward (5.3 TB/s; without the random
+// numbers 38, so they are hidden) and 48 us backward (6.1 TB/s); 63984 x 192 with a residual 12.5 us (5.9 TB/s).
 #include "common.h"
 #include "philox.h"
 

@@ -11,8 +11,10 @@ import torch
 
 import oracle.attention as oa
 from pymsst_amd import _lib
+from pymsst_amd import extension as ext_mod
 from tests import attention_bars as bars
 from tests.conftest import dt_name, to_np
+from tests.test_gpu_guard_writes import _GuardedTorch
 
 _F = [torch.float32, torch.bfloat16, torch.float16]
 _SEED, _OFFSET = 0x1234567_89ABCDEF, 0x7000000_00000005
@@ -375,6 +377,27 @@ def test_streams_and_repeated_calls(hip_ext):
     torch.cuda.synchronize()
     for res in got:
         assert all(torch.equal(x, y) for x, y in zip(res, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", _F)
+def test_no_write_outside_the_outputs(hip_ext, monkeypatch, dtype):
+    """Outputs and workspaces between guard patterns, at odd shapes of every route (split forward and backward, few
+    keys, wide rows, cut head dimensions)."""
+    guard = _GuardedTorch(torch)
+    monkeypatch.setattr(ext_mod, "torch", guard)
+    for shape in ((2, 70, 150, 4, 2, 64), (1, 1, 3000, 4, 2, 72), (1, 900, 33, 3, 1, 40), (2, 33, 200, 2, 2, 128),
+                  (1, 5, 1500, 2, 1, 128), (2, 129, 65, 6, 2, 24)):
+        for p in (0.0, 0.2):
+            q, k, v, do, km, kl = _inputs(shape, dtype, "lengths", seed=1)
+            kw = dict(key_lengths=kl, dropout_p=p, rng=_rng() if p else None)
+            out, lse = hip_ext.cross_attention_forward(q, k, v, need_lse=True, **kw)
+            hip_ext.cross_attention_backward(do, q, k, v, out, lse, **kw)
+            assert not guard.damaged(), shape
+    x = torch.randn(4099, device="cuda").to(dtype)
+    hip_ext.dropout_forward(x, 0.3, _rng(), activation="gelu", residual=x)
+    hip_ext.dropout_backward(x, 0.3, _rng(), x=x, activation="gelu")
+    assert not guard.damaged()
 
 
 @pytest.mark.gpu
