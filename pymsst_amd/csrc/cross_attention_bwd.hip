@@ -439,7 +439,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
 // the row tiles of its pair.  A wave takes 32 rows: its whole row of P and dP is in registers, so D is summed from
 // them (unrounded, and O is not read: with few keys a rounded O would cost dQ and dK half a rounding more).  P and dS then go through LDS, rows down and keys across, to be the other
 // operand of dV and dK, of which each wave owns 32 keys.  5 products instead of 7, and every tensor is moved once:
-// 1032 x 62 queries over 62 keys, bf16, 8 heads of 64 take 128 us, of which the bytes need 88.
+// 1032 x 62 queries over 62 keys, bf16, 8 heads of 64 take 113 us, of which
+// the bytes need 88.
 // fp16: P is held at 2^14; dS at a power of two from its own largest magnitude in the row tile, and dK's sum is
 // brought to a tile's power when that is the smaller one.
 // Waves that share a SIMD: fp16's scaling and the dropped bits together pass the registers of two.
@@ -868,7 +869,7 @@ int pmsst_cross_attention_backward(const void* grad_out, const int64_t* grad_out
   }
   const int64_t pairs = batch * kv_heads, per = std::max(p.q_tiles * p.q_splits, p.k_tiles * p.k_splits);
   constexpr int64_t kGrid = int64_t{1} << 31;
-  PMSST_REQUIRE(per < kGrid / (pairs + 8) && pairs < kGrid / kParts, "%s: too many rows for one call", what);
+  PMSST_REQUIRE(per < kGrid / (pairs + 64) && pairs < kGrid / kParts, "%s: too many rows for one call", what);
   a.scale = static_cast<float>(scale);
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   hipStream_t st = static_cast<hipStream_t>(stream);

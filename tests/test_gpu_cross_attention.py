@@ -124,6 +124,22 @@ def test_c_abi_refusals():
     assert fwd(b=0) == 0 and fwd(n=0) == 0  # nothing to do
 
 
+@pytest.mark.parametrize("pairs", [1, 7, 8, 16, 63, 65, 100, 512, 513, 576, 992, 2047, 2048, 2049, 8256])
+@pytest.mark.parametrize("per", [1, 3, 8])
+def test_block_numbering_visits_every_tile_once(pairs, per):
+    """The numbering of ``attention.h`` (blocks of a pair on one XCD, many pairs eight at a time), restated."""
+    by_xcd, by_eight = pairs % 8 == 0 or pairs >= 64, pairs >= 2048 or (pairs >= 512 and pairs % 64 == 0)
+    step = 64 if by_eight else 8 if by_xcd else 1
+    seen = []
+    for x in range(-(-pairs // step) * step * per):
+        i, xcd = divmod(x, 8)
+        local, sub = divmod(i, per) if by_xcd else divmod(x, per)
+        pair = ((local // 8) * 8 + xcd) * 8 + local % 8 if by_eight else local * 8 + xcd if by_xcd else local
+        if pair < pairs:
+            seen.append((pair, sub))
+    assert len(seen) == pairs * per == len(set(seen))
+
+
 # ---------------------------------------------------------------------- GPU
 
 _SHAPES = [
