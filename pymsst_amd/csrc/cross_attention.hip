@@ -3,7 +3,7 @@
 // One pass over the keys with a running maximum and sum (per row, fp32): with s the scores of a tile,
 //   m' = max(m, max s),  l' = l exp(m - m') + sum exp(s - m'),  O' = O exp(m - m') + exp(s - m') V,
 // and O / l at the end.  attention.h describes the tiles.  A block is NW waves of 32 rows; K and V tiles of BK
-// keys pass through registers into two LDS buffers in turn, so that a tile's loads are in flight while the one
+// keys are moved from memory straight into two LDS stages in turn, so that a tile is on its way while the one
 // before it is multiplied.
 //
 // Bound: with many rows the matrix cores and the vector unit together (exponentials, sums and conversions of a tile take

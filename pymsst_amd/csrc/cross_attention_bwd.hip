@@ -437,10 +437,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
 
 // All gradients in one pass where a tile holds every key: a block of 2 waves keeps K and V in LDS and passes over
 // the row tiles of its pair.  A wave takes 32 rows: its whole row of P and dP is in registers, so D is summed from
-// them (unrounded, and O is not read: with few keys a rounded O would cost dQ and dK half a rounding more).  P and dS then go through LDS, rows down and keys across, to be the other
-// operand of dV and dK, of which each wave owns 32 keys.  5 products instead of 7, and every tensor is moved once:
-// 1032 x 62 queries over 62 keys, bf16, 8 heads of 64 take 113 us, of which
-// the bytes need 88.
+// them (unrounded, and O is not read: with few keys a rounded O would cost dQ and dK half a rounding more).  P and dS
+// then go through LDS, rows down and keys across, to be the other operand of dV and dK, of which each wave owns 32
+// keys.  5 products instead of 7, and every tensor is moved once: 1032 x 62 queries over 62 keys, bf16, 8 heads of 64
+// take 113 us, of which the bytes need 88.
 // fp16: P is held at 2^14; dS at a power of two from its own largest magnitude in the row tile, and dK's sum is
 // brought to a tile's power when that is the smaller one.
 // Waves that share a SIMD: fp16's scaling and the dropped bits together pass the registers of two.
@@ -680,7 +680,7 @@ BwdPlan plan_backward(const Shape& s, int dtype) {
   };
   BwdPlan p;
   p.nw_q = s.R <= 64 && !wide ? 2 : 4;
-  p.nw_k = s.M <= 64 && !wide ? 2 : 4;
+  p.nw_k = s.M <= 64 && dtype == PMSST_F32 && !wide ? 2 : 4;  // (16-bit types with so few keys take p.few)
   p.q_tiles = (int64_t{s.R} + 32 * p.nw_q - 1) / (32 * p.nw_q);
   p.k_tiles = (int64_t{s.M} + 32 * p.nw_k - 1) / (32 * p.nw_k);
   p.few = s.M > 0 && s.M <= 64 && dtype != PMSST_F32;
@@ -730,7 +730,7 @@ int launch_dkv(const BwdArgs& a, bool drop, hipStream_t stream) {
 
 template <typename T, int DP>
 int launch_dkv(const BwdArgs& a, int nw, bool drop, hipStream_t stream) {
-  if constexpr (DP * sizeof(T) != 512) {
+  if constexpr (sizeof(T) == 4 && DP < 128) {
     if (nw == 2) return launch_dkv<T, DP, 2>(a, drop, stream);
   }
   return launch_dkv<T, DP, 4>(a, drop, stream);
