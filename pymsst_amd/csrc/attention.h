@@ -414,6 +414,8 @@ inline Grid make_grid(int64_t pairs, int64_t per) {
   g.by_per = FastDiv(g.per);
   return g;
 }
+// A launch has less than 2^32 work-items: 2^24 blocks of up to 256.
+inline bool grid_fits(int64_t pairs, int64_t per) { return per < (int64_t{1} << 24) / (pairs + 64); }
 inline int64_t grid_blocks(const Grid& g) {
   const int64_t step = g.by_eight ? 64 : g.by_xcd ? 8 : 1;
   return (int64_t{g.pairs} + step - 1) / step * step * g.per;

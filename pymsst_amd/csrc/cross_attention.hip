@@ -400,7 +400,7 @@ int pmsst_cross_attention_forward(const void* q, const int64_t* q_strides, const
   a.row_tiles = static_cast<uint32_t>(p.row_tiles);
   a.tiles_per_split = static_cast<int32_t>(p.tiles_per_split);
   const int64_t pairs = batch * kv_heads, per = p.row_tiles * p.splits;
-  PMSST_REQUIRE(per < (int64_t{1} << 31) / (pairs + 64), "%s: too many rows for one call", what);
+  PMSST_REQUIRE(grid_fits(pairs, per), "%s: too many rows for one call", what);
   a.grid = make_grid(pairs, per);
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -42,6 +42,7 @@ struct BwdArgs {
 };
 
 constexpr int kParts = 16;
+constexpr uint32_t kBoundPairs = 1u << 18;  // pairs of a grid row of attn_bound_kernel: 2^30 work-items
 
 // Rows of a passing tile: 64, or 32 where its two LDS tiles, twice, would pass 64 KB.
 template <typename T, int DP>
@@ -73,9 +74,10 @@ __device__ __forceinline__ int pair_exponent(const BwdArgs& a, uint32_t pair) {
 template <typename T>
 __global__ __launch_bounds__(256) void attn_bound_kernel(BwdArgs a) {
   __shared__ float red[2][4];
-  const uint32_t pair = blockIdx.x / kParts;
-  const int part = static_cast<int>(blockIdx.x % kParts);
   const Shape& s = a.s;
+  const uint32_t pair = blockIdx.y * kBoundPairs + blockIdx.x / kParts;
+  const int part = static_cast<int>(blockIdx.x % kParts);
+  if (pair >= static_cast<uint32_t>(s.B) * s.Hk) return;
   const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
   // 4, 8 or 16 lanes a row, 16 bytes each
   const int units = s.D / 8, log_lanes = units <= 4 ? 2 : units <= 8 ? 3 : 4;
@@ -770,7 +772,9 @@ int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
     }
   }
   if constexpr (std::is_same<T, f16>::value) {
-    attn_bound_kernel<T><<<dim3(static_cast<uint32_t>(pairs * kParts)), 256, 0, stream>>>(a);
+    const dim3 grid(static_cast<uint32_t>(std::min<int64_t>(pairs, kBoundPairs) * kParts),
+                    static_cast<uint32_t>((pairs + kBoundPairs - 1) / kBoundPairs));
+    attn_bound_kernel<T><<<grid, 256, 0, stream>>>(a);
     const int rc = check_launch("attn_bound_kernel");
     if (rc != PMSST_OK) return rc;
   }
@@ -867,9 +871,8 @@ int pmsst_cross_attention_backward(const void* grad_out, const int64_t* grad_out
     a.part_k = reinterpret_cast<float*>(at);
     a.part_v = reinterpret_cast<float*>(at + w.part_k);
   }
-  const int64_t pairs = batch * kv_heads, per = std::max(p.q_tiles * p.q_splits, p.k_tiles * p.k_splits);
-  constexpr int64_t kGrid = int64_t{1} << 31;
-  PMSST_REQUIRE(per < kGrid / (pairs + 64) && pairs < kGrid / kParts, "%s: too many rows for one call", what);
+  const int64_t per = p.few ? p.k_splits : std::max(p.q_tiles * p.q_splits, p.k_tiles * p.k_splits);
+  PMSST_REQUIRE(grid_fits(batch * kv_heads, per), "%s: too many rows for one call", what);
   a.scale = static_cast<float>(scale);
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   hipStream_t st = static_cast<hipStream_t>(stream);

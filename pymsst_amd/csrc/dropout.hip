@@ -174,7 +174,7 @@ template <typename T, int ACT, bool SECOND, bool BACK>
 int launch(const void* x, const void* second, void* out, int64_t n, const Dropout& d, hipStream_t stream) {
   const int64_t per_block = int64_t{8} * kDropThreads * drop_unroll<ACT, SECOND>();
   const int64_t blocks = (n + per_block - 1) / per_block;
-  PMSST_REQUIRE(blocks < (int64_t{1} << 31), "dropout: %lld elements are too many for one call",
+  PMSST_REQUIRE(blocks * kDropThreads < (int64_t{1} << 32), "dropout: %lld elements are too many for one call",
                 static_cast<long long>(n));
   const bool vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(second) |
                      reinterpret_cast<uintptr_t>(out)) & 15) == 0;

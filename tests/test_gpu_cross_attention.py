@@ -124,6 +124,23 @@ def test_c_abi_refusals():
     assert fwd(b=0) == 0 and fwd(n=0) == 0  # nothing to do
 
 
+def test_calls_past_the_grid_are_refused():
+    """A launch has less than 2^32 work-items, 2^24 blocks of 256: more tiles are an argument error, not a launch's."""
+    lib = _lib.load_library()
+    one = ctypes.c_void_p(4096)  # never dereferenced
+
+    def fwd(b, n):
+        return lib.pmsst_cross_attention_forward(one, None, one, None, one, None, None, 0, None, one, None, b, n, 3, 8, 8, 8, 1.0,
+                                                 0.0, None, 2, None, 0, None)
+
+    def bwd(b, n, m, dtype):
+        return lib.pmsst_cross_attention_backward(one, None, one, None, one, None, one, None, one, one, None, 0, None, one, one,
+                                                  one, b, n, m, 8, 8, 8, 1.0, 0.0, None, dtype, one, 1 << 60, None)
+
+    assert fwd(2**21, 1) == fwd(2**14, 2**14) == -1
+    assert bwd(2**21, 1, 3, 2) == bwd(2**14, 2**14, 65, 1) == bwd(2**14, 1, 2**14, 0) == -1
+
+
 @pytest.mark.parametrize("pairs", [1, 7, 8, 16, 63, 65, 100, 512, 513, 576, 992, 2047, 2048, 2049, 8256])
 @pytest.mark.parametrize("per", [1, 3, 8])
 def test_block_numbering_visits_every_tile_once(pairs, per):
@@ -393,6 +410,21 @@ def test_streams_and_repeated_calls(hip_ext):
     torch.cuda.synchronize()
     for res in got:
         assert all(torch.equal(x, y) for x, y in zip(res, want))
+
+
+@pytest.mark.gpu
+def test_more_pairs_than_a_row_of_the_maxima(hip_ext):
+    """2^20 + 8 pairs: the fp16 maxima alone are 2^24 blocks.  The first and the last batch rows against 64 bits."""
+    b, n, m, h, d = 2**17 + 1, 1, 65, 8, 8
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, do = (torch.randn(b, n, h, d, generator=g, device="cuda", dtype=torch.float16) for _ in range(2))
+    k, v = (torch.randn(b, m, h, d, generator=g, device="cuda", dtype=torch.float16) for _ in range(2))
+    out, lse = hip_ext.cross_attention_forward(q, k, v, need_lse=True)
+    grads = hip_ext.cross_attention_backward(do, q, k, v, out, lse)
+    for rows in (slice(0, 2), slice(2**15 - 1, 2**15 + 1), slice(b - 2, b)):
+        ref = bars.reference("f16", *(to_np(t[rows]) for t in (q, k, v, do)), None, None, None, 0.0, 0, 0)
+        for name, t in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
+            bars.check(t[rows], ref[name], (name, rows))
 
 
 @pytest.mark.gpu

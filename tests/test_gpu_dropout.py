@@ -80,6 +80,14 @@ def test_c_abi_refusals():
     assert lib.pmsst_dropout_forward(None, None, None, 0, 0.1, one, 0, 0, None) == 0  # nothing to do
 
 
+def test_calls_past_the_grid_are_refused():
+    """A launch has less than 2^32 work-items: more elements are an argument error, not a launch's."""
+    lib = _lib.load_library()
+    one = ctypes.c_void_p(16)  # never dereferenced
+    assert lib.pmsst_dropout_forward(one, None, one, 2**40, 0.1, one, 0, 0, None) == -1
+    assert "too many" in _lib.last_error()
+
+
 # ---------------------------------------------------------------------- GPU
 
 
