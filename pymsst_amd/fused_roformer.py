@@ -492,7 +492,7 @@ def _patch_core_attention(ext: Any) -> bool:
     def sdpa_cuda_ext(q, k, v, dropout_p):
         d = q.shape[-1]
         if (not q.is_cuda or q.dtype not in _FLOAT_TYPES or k.dtype != q.dtype or v.dtype != q.dtype or d % 8
-                or not 8 <= d <= 128):
+                or not 8 <= d <= 128 or dropout_p >= 1):
             return original(q, k, v, dropout_p)
         out = cross_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), dropout_p=dropout_p, extension=ext)
         return out.transpose(1, 2)
@@ -515,7 +515,8 @@ def _patch_core_dropout(ext: Any) -> bool:
 
     def feed_forward_cuda_ext(self, x):
         norm, up, act, drop, down, last = self.net
-        if not self.training or not x.is_cuda or drop.p <= 0 or drop.p >= 1 or act.approximate != "none":
+        if (not drop.training or not x.is_cuda or drop.p <= 0 or drop.p >= 1
+                or getattr(act, "approximate", None) != "none"):
             return original_ff(self, x)
         h = up(norm(x))
         if h.dtype not in _FLOAT_TYPES:
@@ -524,7 +525,7 @@ def _patch_core_dropout(ext: Any) -> bool:
 
     def residual_block(block, last, x):
         p = last.p
-        if not block.training or not x.is_cuda or p <= 0 or p >= 1:
+        if not last.training or not x.is_cuda or p <= 0 or p >= 1:
             return block(x) + x
         last.p = 0.0  # the block's own call of its last dropout: passes its input on
         try:

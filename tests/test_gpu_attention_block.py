@@ -232,3 +232,31 @@ def test_patched_model_with_dropout(flags, hip_ext, amp):
     with torch.no_grad():
         got = model(mixture)
     assert float((got - want).norm()) <= 1e-5 * float(want.norm())
+
+
+@pytest.mark.gpu
+def test_dropout_modules_keep_their_own_mode(flags, hip_ext):
+    """Dropout modules set to evaluation inside a training model drop nothing, and ones left in training inside an
+    evaluated model (samples of its predictions) do: the mode is the module's, as in the stock blocks."""
+    wl = copy.deepcopy(WORKLOADS["bsr_tiny"])
+    _, mixture = (t.cuda() for t in workload_batch(wl, seed=3)[:2])
+    wl.model.update(attn_dropout=0.0, ff_dropout=0.3)
+    model = wl.build_model("cuda", seed=4).eval()
+    status = fr.apply_roformer_fused_training_backend(model, "hip", extension=hip_ext)
+    assert status.patched_dropout
+    drops = [m for m in model.modules() if isinstance(m, torch.nn.Dropout)]
+    with torch.no_grad():
+        want = model(mixture)
+        model.train()
+        for m in drops:
+            m.eval()
+        assert float((model(mixture) - want).norm()) <= 1e-5 * float(want.norm())
+        model.eval()
+        for m in drops:
+            m.train()
+        runs = []
+        for seed in (1, 1, 2):
+            torch.manual_seed(seed)
+            runs.append(model(mixture))
+    assert torch.equal(runs[0], runs[1]) and not torch.equal(runs[0], runs[2])
+    assert float((runs[0] - want).norm()) > 1e-3 * float(want.norm())
