@@ -69,6 +69,25 @@ __device__ __forceinline__ int pair_exponent(const BwdArgs& a, uint32_t pair) {
   return scale_exponent(2.f * parts_max(a.l1 + pair * kParts) * parts_max(a.vmax + pair * kParts) * a.drop.factor, 1);
 }
 
+// ---------------------------------------------------------------- one key
+// Where a query sees one key alone, P is 1 whatever the score: dS, and with it dQ and dK, is zero exactly, while
+// P from lse and D from O (rounded, and divided by 1 - p) would leave their rounding errors.  The sums are
+// stored times 0 there: one that is no finite number (dP - dP is none then) stays none.
+
+// Whether a key of this batch row outside [from, to) is seen.  Asked only where one key inside is: a scan that ends
+// at the next one.
+__device__ __forceinline__ bool seen_outside(const uint8_t* mask, int count, int from, int to) {
+  if (mask == nullptr) return from > 0 || to < count;
+  const int lane = threadIdx.x & 63;
+  for (int t = to; t < count; t += 64) {
+    if (__any(t + lane < count && mask[min(t + lane, count - 1)] != 0)) return true;
+  }
+  for (int t = from; t > 0; t -= 64) {
+    if (__any(t > lane && mask[max(t - 1 - lane, 0)] != 0)) return true;
+  }
+  return false;
+}
+
 // ---------------------------------------------------------------- fp16 bounds
 
 template <typename T>
@@ -202,6 +221,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
   }
 
   f32x16_t acc[DT]{};
+  int found = 0;  // keys seen so far
   Tile<T, DP, BK, NW> kt, vt;
   auto k_at = [&](int i) { return i * a.ks.n; };
   auto v_at = [&](int i) { return i * a.vs.n; };
@@ -235,6 +255,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
       if (t + 1 < t1) byte_next = mask_byte(t + 1);
     }
     if constexpr (BK == 32) seen &= 0xFFFFFFFFu;
+    found += __popcll(seen);
     constexpr uint64_t kAll = BK == 64 ? ~uint64_t{0} : 0xFFFFFFFFu;
     vm_wait<0>();  // this wave's moves of the tile have arrived
     if (seen != kAll || d_units != kt.UNITS) {
@@ -274,8 +295,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
       mma_cols<T, DP>(kl, u, p, acc, at_lane);
     }
   }
+  const bool lone = found == 1 && !seen_outside(mask, count, t0 * BK, t1 * BK);
   if (!row_ok) return;
-  const float out_scale = std::is_same<T, f16>::value ? ldexpf(a.scale, -e) : a.scale;
+  const float out_scale = lone ? 0.f : std::is_same<T, f16>::value ? ldexpf(a.scale, -e) : a.scale;
   if (a.part_q) {
     const int64_t at = (static_cast<int64_t>(split) * a.grid.pairs + pair) * s.R + r;
     store_cols_f32<T, DP>(a.part_q + at * s.D, acc, out_scale, s.D, h);
@@ -308,6 +330,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
   const bool seen = ki < count && (a.km.mask == nullptr || a.km.mask[b * a.km.stride + ki] != 0);
 
   const bool idle = __builtin_amdgcn_readfirstlane(key0) >= count;  // no key of this wave counts: it only moves tiles
+
+  const int wave_key0 = __builtin_amdgcn_readfirstlane(key0);
+  // (a key has two lanes)
+  const int lone = __builtin_amdgcn_readfirstlane(
+      __popcll(__ballot(seen)) == 2 &&
+      !seen_outside(a.km.mask ? a.km.mask + b * a.km.stride : nullptr, count, wave_key0, wave_key0 + 32));
 
   f32x16_t dk[DT]{}, dv[DT]{};
   float k_scale = a.scale, v_scale = DROP ? a.drop.factor : 1.f;
@@ -416,6 +444,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     }
   }
   if (ki >= s.M) return;
+  if (lone) k_scale = 0.f;
   if (!seen) {
     // nothing was learnt about a key that is not seen, whatever its columns of the tiles hold
 #pragma unroll
@@ -466,6 +495,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
   const int count = key_count(a.km, b, s.M);
   uint64_t seen = range_bits(0, count);
   if (a.km.mask) seen &= __ballot(a.km.mask[b * a.km.stride + min(lane, s.M - 1)] != 0);
+  const bool lone = __popcll(seen) == 1;
   const int tiles = (s.R + 63) / 64;
   const int t0 = static_cast<int>(split) * a.tiles_per_split;
   const int t1 = min(tiles, t0 + a.tiles_per_split);
@@ -588,8 +618,9 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
     for (int u = 0; u < 2; ++u) mma_cols<T, DP>(kv[0], u, ds[u], dq, at_lane);
     const int row = 32 * wave + (at_lane & 31);
     if (row_ok) {
+      const float dq_scale = lone ? 0.f : kHalf ? ldexpf(a.scale, -e) : a.scale;
       const int64_t to = (static_cast<int64_t>(b) * s.N + n) * s.H + head;
-      store_cols<T, DP>(static_cast<T*>(a.dq) + to * s.D, dq, kHalf ? ldexpf(a.scale, -e) : a.scale, s.D, h);
+      store_cols<T, DP>(static_cast<T*>(a.dq) + to * s.D, dq, dq_scale, s.D, h);
     }
 
     // [row][key] tiles: a lane writes its row's keys, 8 consecutive ones a unit
@@ -621,7 +652,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
   // a transposed read hands lane l the key key_row(l % 32)
   const int ki = 32 * wave + key_row(lane & 31);
   if (ki >= s.M) return;
-  const float k_scale = kHalf ? ldexpf(a.scale, -e_sum) : a.scale, v_scale = kHalf ? factor / 16384.f : factor;
+  const float k_scale = lone ? 0.f : kHalf ? ldexpf(a.scale, -e_sum) : a.scale, v_scale = kHalf ? factor / 16384.f : factor;
   if (a.part_k) {
     const int64_t to = ((static_cast<int64_t>(split) * a.grid.pairs + pair) * s.M + ki) * s.D;
     store_cols_f32<T, DP>(a.part_k + to, dk, k_scale, s.D, h);
