@@ -555,13 +555,18 @@ class HipFusedExtension:
     def _attention_operand(self, t):
         """``t`` with a dense last axis and whole 16 bytes between rows (else a dense copy), and its strides."""
         unit = 16 // t.element_size()
-        st = t.stride()
-        if st[3] != 1 or st[0] % unit or st[1] % unit or st[2] % unit or t.data_ptr() % 16:
+        st = self._attention_strides(t)
+        if t.stride(3) != 1 or st[0] % unit or st[1] % unit or st[2] % unit or t.data_ptr() % 16:
             t = t.contiguous()
             if t.data_ptr() % 16:
                 t = t.clone()
-            st = t.stride()
-        return t, (ctypes.c_int64 * 3)(*st[:3])
+            st = self._attention_strides(t)
+        return t, (ctypes.c_int64 * 3)(*st)
+
+    @staticmethod
+    def _attention_strides(t):
+        # an axis of one element is never stepped along; torch lets it carry any stride, and calls it contiguous
+        return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride())]
 
     def _attention_check(self, q, k, v, key_mask, key_lengths, scale, dropout_p, rng):
         _req(q.is_cuda and q.dim() == 4, "q must be a CUDA tensor of shape [B, N, H, D]")
