@@ -131,7 +131,8 @@ class Attention(nn.Module):
     def _attention(self, q, k, v):
         return _sdpa(q.contiguous(), k.contiguous(), v.contiguous(), self.dropout if self.training else 0.0)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def attend(self, x: torch.Tensor) -> torch.Tensor:
+        """The gated heads ``[B, N, H * D]`` that ``to_out`` takes."""
         x = self.norm(x)
         q, k, v = qkv_to_bnhd(self.to_qkv(x), self.heads)
         if self.rotary_embed is not None:
@@ -140,7 +141,10 @@ class Attention(nn.Module):
         out = self._attention(q, k, v).transpose(1, 2)  # [B, N, H, D]
         gates = self.to_gates(x).sigmoid()
         out = out * gates.unsqueeze(-1).to(out.dtype)
-        return self.to_out(out.reshape(*out.shape[:2], -1))
+        return out.reshape(*out.shape[:2], -1)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.to_out(self.attend(x))
 
 
 class FeedForward(nn.Module):

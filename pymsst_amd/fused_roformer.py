@@ -430,15 +430,17 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
     if getattr(transformer.Attention.forward, "_pymsst_fused_attention_gates", False):
         return True
     original = transformer.Attention.forward
+    original_attend = _attend_of(original)
 
-    def attention_forward_cuda_ext(self, x):
-        if (
-            not self.training
-            or x.device.type != "cuda"
-            or x.dtype not in _FLOAT_TYPES
-            or self.to_gates.bias is None
-        ):
-            return original(self, x)
+    def takes(self, x):
+        return (
+            self.training
+            and x.device.type == "cuda"
+            and x.dtype in _FLOAT_TYPES
+            and self.to_gates.bias is not None
+        )
+
+    def attend(self, x):
         x = self.norm(x)
         qkv = self.to_qkv(x)
         flash_layout = False
@@ -462,20 +464,33 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
         else:
             out = self._attention(q, k, v).transpose(1, 2)
         gate_dtype = out.dtype
-        gated = _FusedAttentionGate.apply(
+        return _FusedAttentionGate.apply(
             out,
             x.to(dtype=gate_dtype),
             self.to_gates.weight.to(dtype=gate_dtype),
             self.to_gates.bias.to(dtype=gate_dtype),
             ext,
         )
-        return self.to_out(gated)
 
+    def attention_forward_cuda_ext(self, x):
+        return self.to_out(attend(self, x)) if takes(self, x) else original(self, x)
+
+    if original_attend is not None:
+        attention_forward_cuda_ext._pymsst_attend = lambda self, x: (attend if takes(self, x) else original_attend)(self, x)
     attention_forward_cuda_ext._pymsst_fused_attention_gates = True
     attention_forward_cuda_ext._pymsst_fused_attention_gate_mode = mode
     attention_forward_cuda_ext._pymsst_original_forward = original
     transformer.Attention.forward = attention_forward_cuda_ext
     return True
+
+
+def _attend_of(forward):
+    """The part of an ``Attention.forward`` before its ``to_out``: the stock one's or that of the gates' patch;
+    ``None`` for any other."""
+    _, transformer, _ = _core()
+    if forward.__module__ == transformer.__name__ and forward.__qualname__ == "Attention.forward":
+        return lambda self, x: self.attend(x)
+    return getattr(forward, "_pymsst_attend", None)
 
 
 def _patch_core_attention(ext: Any) -> bool:
@@ -513,35 +528,36 @@ def _patch_core_dropout(ext: Any) -> bool:
         return True
     original_ff, original = transformer.FeedForward.forward, transformer.Transformer.forward
 
-    def feed_forward_cuda_ext(self, x):
-        norm, up, act, drop, down, last = self.net
-        if (not drop.training or not x.is_cuda or drop.p <= 0 or drop.p >= 1
-                or getattr(act, "approximate", None) != "none"):
-            return original_ff(self, x)
+    def before_last(ff, x):
+        norm, up, act, drop, down, _ = ff.net
         h = up(norm(x))
-        if h.dtype not in _FLOAT_TYPES:
-            return last(down(drop(act(h))))
-        return last(down(dropout(h, drop.p, activation="gelu", extension=ext)))
+        if (not drop.training or drop.p <= 0 or drop.p >= 1 or h.dtype not in _FLOAT_TYPES
+                or getattr(act, "approximate", None) != "none"):
+            return down(drop(act(h)))
+        return down(dropout(h, drop.p, activation="gelu", extension=ext))
 
-    def residual_block(block, last, x):
-        p = last.p
-        if not last.training or not x.is_cuda or p <= 0 or p >= 1:
+    def feed_forward_cuda_ext(self, x):
+        if not x.is_cuda:
+            return original_ff(self, x)
+        return self.net[5](before_last(self, x))
+
+    def residual(block, last, x, before_last):
+        # the block's modules are called one by one, without the last dropout: switching that off for the call would
+        # reach every other caller of the same modules
+        if before_last is None or not last.training or not x.is_cuda or last.p <= 0 or last.p >= 1:
             return block(x) + x
-        last.p = 0.0  # the block's own call of its last dropout: passes its input on
-        try:
-            y = block(x)
-        finally:
-            last.p = p
+        y = before_last(block, x)
         if y.dtype not in _FLOAT_TYPES:
-            return F.dropout(y, p) + x
+            return last(y) + x
         if y.dtype != x.dtype:
-            return dropout(y, p, extension=ext) + x
-        return dropout(y, p, residual=x, extension=ext)
+            return dropout(y, last.p, extension=ext) + x
+        return dropout(y, last.p, residual=x, extension=ext)
 
     def transformer_cuda_ext(self, x):
         for attn, ff in self.layers:
-            x = residual_block(attn, attn.to_out[1], x)
-            x = residual_block(ff, ff.net[5], x)
+            attend = _attend_of(type(attn).forward)
+            x = residual(attn, attn.to_out[1], x, attend and (lambda attn, x: attn.to_out[0](attend(attn, x))))
+            x = residual(ff, ff.net[5], x, before_last)
         return self.norm(x)
 
     feed_forward_cuda_ext._pymsst_original_forward = original_ff
