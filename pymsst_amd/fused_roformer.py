@@ -484,11 +484,16 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
     return True
 
 
+def _is_stock(function, name: str) -> bool:
+    _, transformer, _ = _core()
+    return (getattr(function, "__module__", None) == transformer.__name__
+            and getattr(function, "__qualname__", None) == name)
+
+
 def _attend_of(forward):
     """The part of an ``Attention.forward`` before its ``to_out``: the stock one's or that of the gates' patch;
     ``None`` for any other."""
-    _, transformer, _ = _core()
-    if forward.__module__ == transformer.__name__ and forward.__qualname__ == "Attention.forward":
+    if _is_stock(forward, "Attention.forward"):
         return lambda self, x: self.attend(x)
     return getattr(forward, "_pymsst_attend", None)
 
@@ -527,26 +532,34 @@ def _patch_core_dropout(ext: Any) -> bool:
     if getattr(transformer.Transformer.forward, "_pymsst_fused_dropout", False):
         return True
     original_ff, original = transformer.FeedForward.forward, transformer.Transformer.forward
+    if not _is_stock(original_ff, "FeedForward.forward") or not _is_stock(original, "Transformer.forward"):
+        return False  # another program's, whose parts are not known
 
-    def before_last(ff, x):
+    def drops(module):  # a dropout the kernels draw: no other module in its place, no kind of its own
+        return type(module) is torch.nn.Dropout and module.training and 0 < module.p < 1
+
+    def chain(seq, count):
+        return type(seq) is torch.nn.Sequential and len(seq) == count
+
+    def feed_forward_before_last(ff, x):
         norm, up, act, drop, down, _ = ff.net
         h = up(norm(x))
-        if (not drop.training or drop.p <= 0 or drop.p >= 1 or h.dtype not in _FLOAT_TYPES
-                or getattr(act, "approximate", None) != "none"):
+        if (not drops(drop) or type(act) is not torch.nn.GELU or act.approximate != "none"
+                or h.dtype not in _FLOAT_TYPES):
             return down(drop(act(h)))
         return down(dropout(h, drop.p, activation="gelu", extension=ext))
 
     def feed_forward_cuda_ext(self, x):
-        if not x.is_cuda:
+        if not x.is_cuda or not chain(self.net, 6):
             return original_ff(self, x)
-        return self.net[5](before_last(self, x))
+        return self.net[5](feed_forward_before_last(self, x))
 
-    def residual(block, last, x, before_last):
+    def residual(block, seq, count, before_last, x):
         # the block's modules are called one by one, without the last dropout: switching that off for the call would
         # reach every other caller of the same modules
-        if before_last is None or not last.training or not x.is_cuda or last.p <= 0 or last.p >= 1:
+        if before_last is None or not x.is_cuda or not chain(seq, count) or not drops(seq[count - 1]):
             return block(x) + x
-        y = before_last(block, x)
+        y, last = before_last(block, x), seq[count - 1]
         if y.dtype not in _FLOAT_TYPES:
             return last(y) + x
         if y.dtype != x.dtype:
@@ -556,8 +569,10 @@ def _patch_core_dropout(ext: Any) -> bool:
     def transformer_cuda_ext(self, x):
         for attn, ff in self.layers:
             attend = _attend_of(type(attn).forward)
-            x = residual(attn, attn.to_out[1], x, attend and (lambda attn, x: attn.to_out[0](attend(attn, x))))
-            x = residual(ff, ff.net[5], x, before_last)
+            x = residual(attn, getattr(attn, "to_out", None), 2,
+                         attend and (lambda attn, x: attn.to_out[0](attend(attn, x))), x)
+            x = residual(ff, getattr(ff, "net", None), 6,
+                         feed_forward_before_last if type(ff).forward is feed_forward_cuda_ext else None, x)
         return self.norm(x)
 
     feed_forward_cuda_ext._pymsst_original_forward = original_ff

@@ -12,19 +12,17 @@ from torch import nn
 from pymsst_amd import fused_roformer as fr
 from pymsst_amd.core import transformer
 
-_FLAGS = (fr.EXPERIMENTAL_FUSED_ATTENTION_ENV, fr.EXPERIMENTAL_FUSED_DROPOUT_ENV)
-
-
 @pytest.fixture
 def patched(monkeypatch, hip_ext):
-    for name in _FLAGS:
-        monkeypatch.setenv(name, "1")
-
-    def patch(block, gates=False):
+    def patch(block, gates=False, attention=True):
+        monkeypatch.setenv(fr.EXPERIMENTAL_FUSED_DROPOUT_ENV, "1")
+        if attention:
+            monkeypatch.setenv(fr.EXPERIMENTAL_FUSED_ATTENTION_ENV, "1")
         if gates:
             monkeypatch.setenv(fr.EXPERIMENTAL_ATTENTION_GATES_ENV, "1")
         status = fr.apply_roformer_fused_training_backend(block, "hip", extension=hip_ext)
-        assert status.patched_attention and status.patched_dropout and status.patched_attention_gates == gates
+        assert status.patched_dropout
+        assert status.patched_attention == attention and status.patched_attention_gates == gates
         return block
 
     yield patch
@@ -89,3 +87,108 @@ def test_two_threads_that_meet_inside_a_block_both_drop(patched, part):
     assert not errors and len(got) == 2
     for y in got:  # 76800 elements, a standard deviation of 0.002
         assert abs(float((y == x).double().mean()) - 0.5) < 0.02
+
+
+# ---------------------------------------------------------------------- other modules in a dropout's place
+
+
+class _Flipped(nn.Dropout):
+    """A dropout of another kind: it turns its input's sign, and has a p."""
+
+    def forward(self, x):
+        return -x
+
+
+class _Bare(nn.Module):
+    def forward(self, x):
+        return 2 * x
+
+
+class _OwnForward(transformer.Attention):
+    def forward(self, x):
+        return self.to_out(self.attend(x)) * 3
+
+
+class _OwnFeedForward(transformer.FeedForward):
+    def forward(self, x):
+        return self.net(x) * 3
+
+
+def _replace(block, case):
+    """Puts the case's modules into the block; what is left of nn.Dropout has p = 0, so that no mask is drawn."""
+    attn, ff = block.layers[0]
+    attn.dropout = 0.0  # of the weights
+    for m in block.modules():
+        if isinstance(m, nn.Dropout):
+            m.p = 0.0
+    if case == "identity":
+        attn.to_out[1] = ff.net[3] = ff.net[5] = nn.Identity()
+    elif case == "subclass":
+        attn.to_out[1], ff.net[3], ff.net[5] = (_Flipped(0.5) for _ in range(3))
+    elif case == "alpha":
+        attn.to_out[1], ff.net[3], ff.net[5] = (nn.AlphaDropout(0.0) for _ in range(3))
+    elif case == "shorter":
+        attn.to_out, ff.net = attn.to_out[:1], nn.Sequential(*list(ff.net)[:3], ff.net[4])
+    elif case == "longer":
+        attn.to_out.append(_Bare())
+        ff.net.append(_Bare())
+    elif case == "no sequence":
+        attn.to_out, ff.net = attn.to_out[0], nn.Sequential(ff.net[:3], ff.net[4], _Bare())
+    elif case == "own forward":
+        for m, kind in ((attn, _OwnForward), (ff, _OwnFeedForward)):
+            m.__class__ = kind
+    elif case == "tanh gelu":
+        ff.net[2] = nn.GELU(approximate="tanh")
+    elif case == "gelu subclass":
+        ff.net[2] = type("Twice", (nn.GELU,), {"forward": lambda self, x: 2 * x})()
+    return block
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("training", [True, False])
+@pytest.mark.parametrize("case", ["identity", "subclass", "alpha", "shorter", "longer", "no sequence", "own forward",
+                                  "tanh gelu", "gelu subclass"])
+def test_other_modules_in_a_dropouts_place_are_called(patched, case, training):
+    """They run as they do in the stock block, and no nn.Dropout is taken for granted: the same modules give the same
+    values and gradients, but for the order in which SDPA's backward sums."""
+    x = torch.randn(2, 30, 64, device="cuda")
+    block = _replace(_block(), case).train(training)
+
+    def run():
+        inp = x.clone().requires_grad_()
+        out = block(inp)
+        return [out.detach(), *torch.autograd.grad(out.square().sum(), [inp, *block.parameters()])]
+
+    fr.restore_stock_implementations()
+    want = run()
+    patched(block, attention=False)
+    for a, b in zip(run(), want):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.gpu
+def test_blocks_that_own_a_forward_drop_in_it(patched):
+    """Their own forward runs once, its dropout included, with nothing dropped again in the residual sum."""
+    block = patched(_block())
+    attn, ff = block.layers[0]
+    with torch.no_grad():
+        ff.net[4].weight.zero_()
+        ff.net[4].bias.zero_()
+    attn.__class__ = _OwnForward
+    x = torch.randn(4, 300, 64, device="cuda")
+    with torch.no_grad():
+        assert abs(float((block(x) == x).double().mean()) - 0.5) < 0.02
+
+
+def test_another_programs_forward_is_left_alone(monkeypatch):
+    class Ops:
+        dropout_forward = dropout_backward = None
+
+    def own(self, x):
+        return x
+
+    monkeypatch.setenv(fr.EXPERIMENTAL_FUSED_DROPOUT_ENV, "1")
+    monkeypatch.setattr(transformer.FeedForward, "forward", own)
+    block = transformer.Transformer(dim=16, depth=1, dim_head=8, heads=2, ff_dropout=0.3)
+    assert not fr.apply_roformer_fused_training_backend(block, "hip", extension=Ops()).patched_dropout
+    assert transformer.FeedForward.forward is own
