@@ -484,6 +484,15 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
     return True
 
 
+def _only_forward(module) -> bool:
+    """Whether a call of ``module`` is its class's forward alone: without hooks, a forward of its own or a compiled
+    call.  A fused op that stands for several modules' calls runs none of these."""
+    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                or module._backward_pre_hooks or "forward" in module.__dict__
+                or getattr(module, "_compiled_call_impl", None) is not None
+                or torch.nn.modules.module._has_any_global_hook())
+
+
 def _is_stock(function, name: str) -> bool:
     _, transformer, _ = _core()
     return (getattr(function, "__module__", None) == transformer.__name__
@@ -536,15 +545,15 @@ def _patch_core_dropout(ext: Any) -> bool:
         return False  # another program's, whose parts are not known
 
     def drops(module):  # a dropout the kernels draw: no other module in its place, no kind of its own
-        return type(module) is torch.nn.Dropout and module.training and 0 < module.p < 1
+        return type(module) is torch.nn.Dropout and module.training and 0 < module.p < 1 and _only_forward(module)
 
     def chain(seq, count):
-        return type(seq) is torch.nn.Sequential and len(seq) == count
+        return type(seq) is torch.nn.Sequential and len(seq) == count and _only_forward(seq)
 
     def feed_forward_before_last(ff, x):
         norm, up, act, drop, down, _ = ff.net
         h = up(norm(x))
-        if (not drops(drop) or type(act) is not torch.nn.GELU or act.approximate != "none"
+        if (not drops(drop) or type(act) is not torch.nn.GELU or act.approximate != "none" or not _only_forward(act)
                 or h.dtype not in _FLOAT_TYPES):
             return down(drop(act(h)))
         return down(dropout(h, drop.p, activation="gelu", extension=ext))
@@ -557,7 +566,8 @@ def _patch_core_dropout(ext: Any) -> bool:
     def residual(block, seq, count, before_last, x):
         # the block's modules are called one by one, without the last dropout: switching that off for the call would
         # reach every other caller of the same modules
-        if before_last is None or not x.is_cuda or not chain(seq, count) or not drops(seq[count - 1]):
+        if (before_last is None or not x.is_cuda or not chain(seq, count) or not drops(seq[count - 1])
+                or not _only_forward(block)):
             return block(x) + x
         y, last = before_last(block, x), seq[count - 1]
         if y.dtype not in _FLOAT_TYPES:

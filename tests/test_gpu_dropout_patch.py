@@ -192,3 +192,52 @@ def test_another_programs_forward_is_left_alone(monkeypatch):
     block = transformer.Transformer(dim=16, depth=1, dim_head=8, heads=2, ff_dropout=0.3)
     assert not fr.apply_roformer_fused_training_backend(block, "hip", extension=Ops()).patched_dropout
     assert transformer.FeedForward.forward is own
+
+
+# ---------------------------------------------------------------------- hooks
+
+
+def _parts(block):
+    attn, ff = block.layers[0]
+    return {"attention": attn, "attention chain": attn.to_out, "attention dropout": attn.to_out[1], "feed-forward": ff,
+            "feed-forward chain": ff.net, "gelu": ff.net[2], "hidden dropout": ff.net[3], "last dropout": ff.net[5]}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("part", ["attention", "attention chain", "attention dropout", "feed-forward",
+                                  "feed-forward chain", "gelu", "hidden dropout", "last dropout"])
+@pytest.mark.parametrize("kind", ["forward", "pre", "backward", "backward pre", "instance", "global"])
+def test_hooks_run_and_see_what_they_see_in_the_stock_block(patched, part, kind):
+    """Every module of the chain that a fused op stands for is called where something hangs on its call; a forward
+    hook on a dropout, or on what ends in one, sees the dropped output."""
+    block = patched(_block())
+    module, seen = _parts(block)[part], []
+    note = lambda *a: seen.append(a)  # noqa: E731
+    handle = None
+    if kind == "forward":
+        module.register_forward_hook(note)
+    elif kind == "pre":
+        module.register_forward_pre_hook(note)
+    elif kind == "backward":
+        module.register_full_backward_hook(note)
+    elif kind == "backward pre":
+        module.register_full_backward_pre_hook(note)
+    elif kind == "instance":
+        stock = module.forward
+        module.forward = lambda *a: (seen.append(a), stock(*a))[1]
+    else:
+        handle = nn.modules.module.register_module_forward_hook(
+            lambda m, i, o: seen.append((m, i, o)) if m is module else None)
+    try:
+        x = torch.randn(2, 100, 64, device="cuda", requires_grad=True)
+        block(x).sum().backward()
+    finally:
+        if handle is not None:
+            handle.remove()
+    assert len(seen) == 1
+    if kind in ("forward", "global") and part != "gelu":
+        assert abs(float((seen[0][2] == 0).double().mean()) - 0.5) < 0.05  # 12800 elements or more
+    seen.clear()
+    if kind == "global":  # and without it the fused ops are back
+        block(x).sum().backward()
+        assert not seen
