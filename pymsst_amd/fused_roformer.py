@@ -484,6 +484,12 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
     return True
 
 
+def _under_transform() -> bool:
+    """Inside ``torch.func`` (vmap, grad, jvp, ...) or forward-mode differentiation, which the fused ops have no rules
+    for: their derivative is one backward pass."""
+    return torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0
+
+
 def _only_forward(module) -> bool:
     """Whether a call of ``module`` is its class's forward alone: without hooks, a forward of its own or a compiled
     call.  A fused op that stands for several modules' calls runs none of these."""
@@ -509,8 +515,8 @@ def _attend_of(forward):
 
 def _patch_core_attention(ext: Any) -> bool:
     """Module-level ``_sdpa`` replacement (no reference counterpart: the stock and the gate-patched ``Attention``
-    both call PyTorch's SDPA).  What the kernels do not take (CPU, fp64, mixed dtypes, other head dimensions) goes
-    to the original."""
+    both call PyTorch's SDPA).  What the kernels do not take (CPU, fp64, mixed dtypes, other head dimensions, torch's
+    function transforms and forward mode) goes to the original."""
     if any(not hasattr(ext, n) for n in ("cross_attention_forward", "cross_attention_backward")):
         return False
     _, transformer, _ = _core()
@@ -521,7 +527,7 @@ def _patch_core_attention(ext: Any) -> bool:
     def sdpa_cuda_ext(q, k, v, dropout_p):
         d = q.shape[-1]
         if (not q.is_cuda or q.dtype not in _FLOAT_TYPES or k.dtype != q.dtype or v.dtype != q.dtype or d % 8
-                or not 8 <= d <= 128 or dropout_p >= 1):
+                or not 8 <= d <= 128 or dropout_p >= 1 or _under_transform()):
             return original(q, k, v, dropout_p)
         out = cross_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), dropout_p=dropout_p, extension=ext)
         return out.transpose(1, 2)
@@ -559,7 +565,7 @@ def _patch_core_dropout(ext: Any) -> bool:
         return down(dropout(h, drop.p, activation="gelu", extension=ext))
 
     def feed_forward_cuda_ext(self, x):
-        if not x.is_cuda or not chain(self.net, 6):
+        if not x.is_cuda or not chain(self.net, 6) or _under_transform():
             return original_ff(self, x)
         return self.net[5](feed_forward_before_last(self, x))
 
@@ -577,6 +583,8 @@ def _patch_core_dropout(ext: Any) -> bool:
         return dropout(y, last.p, residual=x, extension=ext)
 
     def transformer_cuda_ext(self, x):
+        if _under_transform():
+            return original(self, x)
         for attn, ff in self.layers:
             attend = _attend_of(type(attn).forward)
             x = residual(attn, getattr(attn, "to_out", None), 2,

@@ -241,3 +241,63 @@ def test_hooks_run_and_see_what_they_see_in_the_stock_block(patched, part, kind)
     if kind == "global":  # and without it the fused ops are back
         block(x).sum().backward()
         assert not seen
+
+
+# ---------------------------------------------------------------------- function transforms
+
+
+def _transforms():
+    def vmap(f, x):
+        return torch.func.vmap(f)(x[:, None])[:, 0]
+
+    def grad(f, x):
+        return torch.func.grad(lambda t: f(t).square().sum())(x)
+
+    def per_sample_grads(f, x):
+        return torch.func.vmap(torch.func.grad(lambda t: f(t[None]).square().sum()))(x)
+
+    def jvp(f, x):
+        return torch.func.jvp(f, (x,), (torch.ones_like(x),))[1]
+
+    def forward_mode(f, x):
+        with torch.autograd.forward_ad.dual_level():
+            out = f(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+            return torch.autograd.forward_ad.unpack_dual(out).tangent
+
+    return {f.__name__: f for f in (vmap, grad, per_sample_grads, jvp, forward_mode)}
+
+
+def _outcome(f):
+    try:
+        return f()
+    except Exception as e:  # what the stock modules cannot do either
+        return type(e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transform", list(_transforms()))
+def test_function_transforms_of_the_patched_block(patched, transform):
+    """They give what they give for the stock block (or fail as they do there); fp32, without dropped elements."""
+    f, block = _transforms()[transform], _block().eval()
+    x = torch.randn(3, 20, 64, device="cuda")
+    fr.restore_stock_implementations()
+    want = _outcome(lambda: f(block, x))
+    patched(block)
+    got = _outcome(lambda: f(block, x))
+    assert isinstance(got, torch.Tensor) == isinstance(want, torch.Tensor), (got, want)
+    if isinstance(want, torch.Tensor):
+        assert float((got - want).detach().norm()) <= 1e-5 * float(want.detach().norm())
+    else:
+        assert got is want
+    assert transform not in ("vmap", "grad") or isinstance(want, torch.Tensor)
+
+
+@pytest.mark.gpu
+def test_vmap_of_the_training_block_drops(patched):
+    block = patched(_block())
+    attn, ff = block.layers[0]
+    with torch.no_grad():
+        attn.to_out[0].weight.zero_()
+        x = torch.randn(4, 1, 300, 64, device="cuda")
+        y = torch.func.vmap(block, randomness="different")(x)
+    assert abs(float((y == x).double().mean()) - 0.5) < 0.02
