@@ -292,13 +292,16 @@ struct Tile {
       ptr[i] += step;
     }
   }
-  // The tile at row0, of which only rows below `rows` (> 0) are there.
+  // The tile at row0, of which only rows below `rows` (> 0) are there: those past the end are the last one again, or
+  // what `past` (a row) holds.
   template <typename F>
-  __device__ __forceinline__ void fetch_cut(const char* tile, const T* base, int row0, int rows, int d_units, F at) {
+  __device__ __forceinline__ void fetch_cut(const char* tile, const T* base, int row0, int rows, int d_units, F at,
+                                            const T* past = nullptr) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int row = min(row0 + row_of(i), rows - 1);
-      dma16_m0(reinterpret_cast<const char*>(base + at(row)) + byte_of(i, d_units), target(tile, i));
+      const T* from = past != nullptr && row0 + row_of(i) >= rows ? past : base + at(row);
+      dma16_m0(reinterpret_cast<const char*>(from) + byte_of(i, d_units), target(tile, i));
     }
   }
   // Zeroes this lane's units of rows whose bit is 0, and those past head_dim; the moves must have arrived.
@@ -308,6 +311,14 @@ struct Tile {
       if (unit_of(i) >= d_units || !((seen >> row_of(i)) & 1)) {
         *reinterpret_cast<u32x4_t*>(tile + (i * 64 * NW + static_cast<int>(threadIdx.x)) * 16) = u32x4_t{0, 0, 0, 0};
       }
+    }
+  }
+  // Zeroes this lane's units of the rows from `rows` on; the moves must have arrived.
+  __device__ __forceinline__ void clear_from(char* tile, int rows) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int at = (i * 64 * NW + static_cast<int>(threadIdx.x)) * 16;
+      if (at >= rows * DB) *reinterpret_cast<u32x4_t*>(tile + at) = u32x4_t{0, 0, 0, 0};
     }
   }
 };

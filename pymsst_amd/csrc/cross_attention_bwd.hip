@@ -48,6 +48,9 @@ constexpr uint32_t kBoundPairs = 1u << 18;  // pairs of a grid row of attn_bound
 template <typename T, int DP>
 constexpr int bwd_tile() { return DP * sizeof(T) == 512 ? 32 : 64; }
 
+// What stands for dO past the last row: these rows have no weight, but 0 times the last one's infinities is none.
+__device__ const u32x4_t zero_row[32] = {};
+
 // Largest power of two that keeps bound * 2^e <= 2^top (0 where the bound says nothing).
 __device__ __forceinline__ int scale_exponent(float bound, int top) {
   if (!(bound > 0.f) || bound > 3e38f) return 0;
@@ -382,7 +385,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         gt.fetch(lds[stage][1], g_step);
       } else {
         qt.fetch_cut(lds[stage][0], qb, row0, s.R, d_units, q_at);
-        gt.fetch_cut(lds[stage][1], gb, row0, s.R, d_units, g_at);
+        gt.fetch_cut(lds[stage][1], gb, row0, s.R, d_units, g_at, reinterpret_cast<const T*>(zero_row));
       }
       if (wave0 < 2 && (BQ == 64 || lane < BQ)) dma4_m0(stat_src + row0, __builtin_amdgcn_readfirstlane(lds_addr(stat[stage]) + 256 * wave0));
     };
@@ -535,6 +538,8 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
       tile.clear(rows[0], ~uint64_t{0}, d_units);
       tile.clear(rows[1], ~uint64_t{0}, d_units);
     }
+    // rows past the end hold the last one again, whose infinities would meet their weights of 0
+    if (t * 64 + 64 > s.R) tile.clear_from(rows[1], s.R - t * 64);
     __syncthreads();
 
     const int at_lane = fresh<256>(lane);  // whatever DB: this kernel has no registers for addresses
