@@ -258,7 +258,6 @@ struct Tile {
   static constexpr int UNITS = DB / 16;
   static constexpr int CH = BK * UNITS / (64 * NW);  // moves of a wave
   static constexpr int STEP = 64 * NW / UNITS;       // rows between them
-  static constexpr int BYTES = BK * DB;
   static_assert(CH >= 1 && CH * 64 * NW == BK * UNITS && 64 % UNITS == 0, "whole rows per move");
   const char* ptr[CH];
 

@@ -511,7 +511,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
   tile.fetch_cut(kv[1], static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h, 0, s.M, d_units, [&](int i) { return i * a.vs.n; });
 
   f32x16_t dk[DT]{}, dv[DT]{};
-  constexpr int kNoSum = 100;  // above every exponent: nothing but zeros so far
+  constexpr int kNoSum = 101;  // above every exponent (scale_exponent's end at 100): nothing but zeros so far
   int e_sum = kNoSum;          // dk is held at 2^e_sum
   for (int t = t0; t < t1; ++t) {
     if (t > t0) __syncthreads();  // the tiles of the rows before these have been read
