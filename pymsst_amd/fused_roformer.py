@@ -515,8 +515,8 @@ def _attend_of(forward):
 
 def _patch_core_attention(ext: Any) -> bool:
     """Module-level ``_sdpa`` replacement (no reference counterpart: the stock and the gate-patched ``Attention``
-    both call PyTorch's SDPA).  What the kernels do not take (CPU, fp64, mixed dtypes, other head dimensions, torch's
-    function transforms and forward mode) goes to the original."""
+    both call PyTorch's SDPA).  What the kernels do not take (CPU, fp64, mixed dtypes, other head dimensions, batches
+    and heads that SDPA would broadcast, torch's function transforms and forward mode) goes to the original."""
     if any(not hasattr(ext, n) for n in ("cross_attention_forward", "cross_attention_backward")):
         return False
     _, transformer, _ = _core()
@@ -527,7 +527,8 @@ def _patch_core_attention(ext: Any) -> bool:
     def sdpa_cuda_ext(q, k, v, dropout_p):
         d = q.shape[-1]
         if (not q.is_cuda or q.dtype not in _FLOAT_TYPES or k.dtype != q.dtype or v.dtype != q.dtype or d % 8
-                or not 8 <= d <= 128 or dropout_p >= 1 or _under_transform()):
+                or not 8 <= d <= 128 or q.dim() != 4 or k.shape != v.shape or k.shape[:2] != q.shape[:2]
+                or k.shape[-1] != d or q.shape[1] == 0 or dropout_p >= 1 or _under_transform()):
             return original(q, k, v, dropout_p)
         out = cross_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), dropout_p=dropout_p, extension=ext)
         return out.transpose(1, 2)

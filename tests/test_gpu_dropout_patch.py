@@ -301,3 +301,35 @@ def test_vmap_of_the_training_block_drops(patched):
         x = torch.randn(4, 1, 300, 64, device="cuda")
         y = torch.func.vmap(block, randomness="different")(x)
     assert abs(float((y == x).double().mean()) - 0.5) < 0.02
+
+
+# ---------------------------------------------------------------------- shapes
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [
+    ((2, 4, 30, 32), (2, 4, 50, 32), (2, 4, 50, 64)),  # values of another head dimension
+    ((2, 4, 30, 32), (1, 4, 50, 32), (1, 4, 50, 32)),  # a batch that is broadcast
+    ((2, 4, 30, 32), (2, 1, 50, 32), (2, 1, 50, 32)),  # heads that are
+    ((4, 30, 32), (4, 50, 32), (4, 50, 32)),           # no heads
+    ((2, 4, 30, 36), (2, 4, 50, 36), (2, 4, 50, 36)),  # no multiple of 8
+    ((2, 4, 30, 32), (2, 4, 50, 32), (2, 4, 50, 32)),  # the kernels'
+])
+def test_what_the_kernels_do_not_take_goes_to_sdpa(patched, shapes):
+    q, k, v = (torch.randn(s, device="cuda") for s in shapes)
+    fr.restore_stock_implementations()
+    want = _outcome(lambda: transformer._sdpa(q, k, v, 0.0))
+    patched(_block())
+    got = _outcome(lambda: transformer._sdpa(q, k, v, 0.0))
+    assert isinstance(want, torch.Tensor) and got.shape == want.shape
+    assert float((got - want).norm()) <= 1e-6 * float(want.norm())  # fp32, sums of 50 terms
+
+
+@pytest.mark.gpu
+def test_the_models_attention_of_no_heads_goes_to_sdpa(patched):
+    q = torch.randn(2, 0, 30, 32, device="cuda")
+    fr.restore_stock_implementations()
+    want = _outcome(lambda: transformer._sdpa(q, q, q, 0.0))
+    patched(_block())
+    got = _outcome(lambda: transformer._sdpa(q, q, q, 0.0))
+    assert type(got) is type(want) and getattr(got, "shape", got) == getattr(want, "shape", want)
