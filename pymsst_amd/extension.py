@@ -647,7 +647,7 @@ class HipFusedExtension:
             return [grad_q, grad_k.zero_(), grad_v.zero_()]
         (q, qs), (k, ks), (v, vs) = self._attention_operand(q), self._attention_operand(k), self._attention_operand(v)
         grad_out, gs = self._attention_operand(grad_out)
-        out, lse = out.contiguous(), lse.contiguous()
+        (out, _), lse = self._attention_operand(out.contiguous()), lse.contiguous()
         with _DeviceGuard(q.device):
             size = self._lib.pmsst_cross_attention_backward_workspace_size(b, n, m, h, hk, d, code)
             ws = _workspace(size, q.device)

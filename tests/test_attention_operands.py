@@ -91,3 +91,21 @@ def test_views_with_single_axes_on_the_gpu(hip_ext, dtype):
         go = torch.matmul(torch.ones(b, 5, 24, device="cuda", dtype=dtype), w.t().contiguous())[:, :, None].contiguous()
         (want,) = torch.autograd.grad(out2, q, go)
         assert torch.equal(g, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", _F)
+def test_a_saved_output_between_16_bytes_is_copied(hip_ext, dtype):
+    """A forward's output and log-sums kept in a buffer of the caller's own, at any offset and stride."""
+    q, do = (torch.randn(2, 37, 4, 64, device="cuda").to(dtype) for _ in range(2))
+    k = torch.randn(2, 90, 2, 64, device="cuda").to(dtype)
+    out, lse = hip_ext.cross_attention_forward(q, k, k, need_lse=True)
+    want = hip_ext.cross_attention_backward(do, q, k, k, out, lse)
+    flat = torch.empty(out.numel() + 1, dtype=dtype, device="cuda")
+    kept = flat[1:].view(out.shape).copy_(out)
+    wide = torch.empty(2, 37, 4, 65, dtype=dtype, device="cuda")
+    strided = wide[..., 1:].copy_(out)
+    sums = torch.empty(2, 37, 4, device="cuda").transpose(1, 2).copy_(lse)
+    for o in (kept, strided):
+        for x, y in zip(hip_ext.cross_attention_backward(do, q, k, k, o, sums), want):
+            assert torch.equal(x, y)
