@@ -555,13 +555,15 @@ class HipFusedExtension:
     def _attention_operand(self, t):
         """``t`` with a dense last axis and whole 16 bytes between rows (else a dense copy), and its strides."""
         unit = 16 // t.element_size()
-        st = self._attention_strides(t)
-        if t.stride(3) != 1 or st[0] % unit or st[1] % unit or st[2] % unit or t.data_ptr() % 16:
-            t = t.contiguous()
-            if t.data_ptr() % 16:
-                t = t.clone()
+        st = t.stride()
+        if st[3] != 1 or st[0] % unit or st[1] % unit or st[2] % unit or t.data_ptr() % 16:
             st = self._attention_strides(t)
-        return t, (ctypes.c_int64 * 3)(*st)
+            if t.stride(3) != 1 or any(s % unit for s in st) or t.data_ptr() % 16:
+                t = t.contiguous()
+                if t.data_ptr() % 16:
+                    t = t.clone()
+                st = self._attention_strides(t)
+        return t, (ctypes.c_int64 * 3)(*st[:3])
 
     @staticmethod
     def _attention_strides(t):
