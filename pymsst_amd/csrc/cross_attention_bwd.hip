@@ -82,11 +82,19 @@ __device__ __forceinline__ int pair_exponent(const BwdArgs& a, uint32_t pair) {
 __device__ __forceinline__ bool seen_outside(const uint8_t* mask, int count, int from, int to) {
   if (mask == nullptr) return from > 0 || to < count;
   const int lane = threadIdx.x & 63;
-  for (int t = to; t < count; t += 64) {
-    if (__any(t + lane < count && mask[min(t + lane, count - 1)] != 0)) return true;
+  // 256 keys a step, so that four loads are on their way; an index past either end stands for the last (first) key,
+  // which lies outside as well
+  for (int t = to; t < count; t += 256) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 256; i += 64) any |= mask[min(t + i + lane, count - 1)];
+    if (__any(any != 0)) return true;
   }
-  for (int t = from; t > 0; t -= 64) {
-    if (__any(t > lane && mask[max(t - 1 - lane, 0)] != 0)) return true;
+  for (int t = from - 1; t >= 0; t -= 256) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 256; i += 64) any |= mask[max(t - i - lane, 0)];
+    if (__any(any != 0)) return true;
   }
   return false;
 }
