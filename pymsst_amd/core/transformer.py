@@ -131,8 +131,8 @@ class Attention(nn.Module):
     def _attention(self, q, k, v):
         return _sdpa(q.contiguous(), k.contiguous(), v.contiguous(), self.dropout if self.training else 0.0)
 
-    def attend(self, x: torch.Tensor) -> torch.Tensor:
-        """The gated heads ``[B, N, H * D]`` that ``to_out`` takes."""
+    def gated_heads(self, x: torch.Tensor) -> torch.Tensor:
+        """The heads after their gates, ``[B, N, H * D]``: what ``to_out`` takes."""
         x = self.norm(x)
         q, k, v = qkv_to_bnhd(self.to_qkv(x), self.heads)
         if self.rotary_embed is not None:
@@ -144,7 +144,7 @@ class Attention(nn.Module):
         return out.reshape(*out.shape[:2], -1)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return self.to_out(self.attend(x))
+        return self.to_out(self.gated_heads(x))
 
 
 class FeedForward(nn.Module):

@@ -430,7 +430,7 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
     if getattr(transformer.Attention.forward, "_pymsst_fused_attention_gates", False):
         return True
     original = transformer.Attention.forward
-    original_attend = _attend_of(original)
+    original_heads = _gated_heads_of(original)
 
     def takes(self, x):
         return (
@@ -440,7 +440,7 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
             and self.to_gates.bias is not None
         )
 
-    def attend(self, x):
+    def gated_heads(self, x):
         x = self.norm(x)
         qkv = self.to_qkv(x)
         flash_layout = False
@@ -473,10 +473,10 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
         )
 
     def attention_forward_cuda_ext(self, x):
-        return self.to_out(attend(self, x)) if takes(self, x) else original(self, x)
+        return self.to_out(gated_heads(self, x)) if takes(self, x) else original(self, x)
 
-    if original_attend is not None:
-        attention_forward_cuda_ext._pymsst_attend = lambda self, x: (attend if takes(self, x) else original_attend)(self, x)
+    if original_heads is not None:
+        attention_forward_cuda_ext._pymsst_gated_heads = lambda self, x: (gated_heads if takes(self, x) else original_heads)(self, x)
     attention_forward_cuda_ext._pymsst_fused_attention_gates = True
     attention_forward_cuda_ext._pymsst_fused_attention_gate_mode = mode
     attention_forward_cuda_ext._pymsst_original_forward = original
@@ -505,12 +505,12 @@ def _is_stock(function, name: str) -> bool:
             and getattr(function, "__qualname__", None) == name)
 
 
-def _attend_of(forward):
+def _gated_heads_of(forward):
     """The part of an ``Attention.forward`` before its ``to_out``: the stock one's or that of the gates' patch;
     ``None`` for any other."""
     if _is_stock(forward, "Attention.forward"):
-        return lambda self, x: self.attend(x)
-    return getattr(forward, "_pymsst_attend", None)
+        return lambda self, x: self.gated_heads(x)
+    return getattr(forward, "_pymsst_gated_heads", None)
 
 
 def _patch_core_attention(ext: Any) -> bool:
@@ -528,7 +528,7 @@ def _patch_core_attention(ext: Any) -> bool:
         d = q.shape[-1]
         if (not q.is_cuda or q.dtype not in _FLOAT_TYPES or k.dtype != q.dtype or v.dtype != q.dtype or d % 8
                 or not 8 <= d <= 128 or q.dim() != 4 or k.shape != v.shape or k.shape[:2] != q.shape[:2]
-                or k.shape[-1] != d or q.shape[1] == 0 or dropout_p >= 1 or _under_transform()):
+                or k.shape[-1] != d or dropout_p >= 1 or _under_transform()):
             return original(q, k, v, dropout_p)
         out = cross_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), dropout_p=dropout_p, extension=ext)
         return out.transpose(1, 2)
@@ -587,9 +587,9 @@ def _patch_core_dropout(ext: Any) -> bool:
         if _under_transform():
             return original(self, x)
         for attn, ff in self.layers:
-            attend = _attend_of(type(attn).forward)
+            heads = _gated_heads_of(type(attn).forward)
             x = residual(attn, getattr(attn, "to_out", None), 2,
-                         attend and (lambda attn, x: attn.to_out[0](attend(attn, x))), x)
+                         heads and (lambda attn, x: attn.to_out[0](heads(attn, x))), x)
             x = residual(ff, getattr(ff, "net", None), 6,
                          feed_forward_before_last if type(ff).forward is feed_forward_cuda_ext else None, x)
         return self.norm(x)
