@@ -433,7 +433,8 @@ size_t pmsst_cross_attention_backward_workspace_size(int64_t batch, int64_t quer
                                                      int64_t kv_heads, int64_t head_dim, int dtype);
 /* Gradients of the forward (same masks, scale, dropout_p and rng values) from its dense out and its lse:
  * grad_q[batch, queries, heads, head_dim], grad_k and grad_v[batch, keys, kv_heads, head_dim], dense, fully
- * written (zeros for keys that are not seen; heads that share a key head are summed). */
+ * written (zeros for keys that are not seen; heads that share a key head are summed; exact zeros in grad_q and grad_k
+ * where a query sees one key). */
 int pmsst_cross_attention_backward(const void* grad_out, const int64_t* grad_out_strides, const void* q,
                                    const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                                    const int64_t* v_strides, const void* out, const float* lse, const uint8_t* key_mask,

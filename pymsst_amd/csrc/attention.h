@@ -323,7 +323,7 @@ struct Tile {
 };
 
 // Tiles lie in two stages: while one is multiplied, the next one's move fills the other.  (Three stages hold more
-// LDS than the wait they save is worth: 124 x 948 queries, forward 365 us, with two 330.)
+// LDS than the wait they save is worth: 124 x 948 queries, forward 365 us against 330 when the third was given up.)
 constexpr int kStages = 2;
 
 // Uses a loaded register here, so that the compiler waits for the load here and not (for every load in flight)
@@ -406,8 +406,9 @@ __device__ __forceinline__ void store_cols_f32(float* row, const f32x16_t (&acc)
 // Blocks of one (batch, key head) share its keys: they run on one XCD (the hardware deals block i to XCD
 // i % 8) where the pairs fill the XCDs evenly; few pairs are spread block by block instead.  Many pairs are dealt
 // eight at a time: the heads of a batch row, whose rows are neighbours in memory, follow each other on one XCD
-// (1032 x 62 queries over 62 keys, 8 heads, backward 128 -> 117 us); fewer go one by one, so that the heads of a
-// long batch row are spread (2 rows of 8 heads over 8192 and 4096 keys: 222 us, by eights 290).
+// (1032 x 62 queries over 62 keys, 8 heads, forward and backward in turn: one by one 196 us, by eights 177); fewer go
+// one by one, so that the heads of a long batch row are spread (2 rows of 8 heads over 8192 and 4096 keys: 240 us, by
+// eights, all on two XCDs, 827).
 struct Grid {
   uint32_t pairs;  // batch * key heads
   uint32_t per;    // blocks of a pair

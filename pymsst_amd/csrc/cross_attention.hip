@@ -8,9 +8,11 @@
 //
 // Bound: with many rows the matrix cores and the vector unit together (exponentials, sums and conversions of a tile take
 // about as long as its products), at the clock that this mix leaves, 1.7 to 1.9 GHz of 2.4: 124 x 948 queries over 948
-// keys, 8 heads of 64, fp16, 340 us = 670 TFLOP/s (a library product of 8192^3 reaches 1100).  With short rows HBM:
-// 1032 x 62 over 62, 50 us = 5.2 TB/s, a copy's rate.  With single queries HBM as well: 16 x 8 heads over up to 16500
-// keys, 90 us = 4.5 TB/s.
+// keys, 8 heads of 64, fp16, 334 us = 680 TFLOP/s (a library product of 8192^3 reaches 1100).  With short rows HBM:
+// 1032 x 62 over 62, bf16, 62 us = 4.2 TB/s in a training step (50 us where the call before has left its tensors in the
+// last-level cache).  With single queries of 16 bits HBM as well: 16 x 8 heads over up to 16500 keys, 84 us = 4.8 TB/s.
+// In fp32 their empty rows bound them: a wave multiplies 32 rows for the one that is there (8 x 8 heads over up to
+// 16500 keys, as many bytes, 192 us).
 //
 // Few rows over many keys (single queries) are split over the keys: every split leaves its normalised O and
 // its lse in the workspace, and a second kernel adds them with weights exp(lse_i - lse).
@@ -253,9 +255,11 @@ struct FwdPlan {
 // Waves of a block: 2 where that covers the rows (half a block of 4 would idle; fp32 rows of 512 bytes keep 4,
 // whose lanes hold half as much of a tile on its way), else 4.  Splits: of at least 128 keys, up to 4 blocks of 4
 // waves a CU, whose products bound them and whose ragged ends so even out (2760 queries over up to 8192 keys,
-// heads of 128: 235 us; with 2 blocks a CU 266, with 8 253), or of at least 512 keys, up to 2 blocks of 2 waves, which the
-// keys' bytes bound (16 single queries over up to 16500 keys: 89 us; with 4 blocks 102; a tile of 64 keys takes about
-// 1 us and the second kernel 5).
+// heads of 128: 240 us; with 2 blocks a CU 272, with 8 258), or of at least 512 keys, up to 2 blocks of 2 waves, which the
+// keys' bytes bound in 16 bits (16 single queries over up to 16500 keys: 89 us; with 4 blocks 100, with 1 134; a tile of 64
+// keys takes about 1 us and the second kernel 5).  fp32's single queries, bound by the products of empty rows, gain
+// nothing by more blocks either (8 over up to 16500 keys: 192 us; with 4 blocks 203); rows of 512 bytes come under the first
+// rule (16 over up to 4097 keys, heads of 128: 101 us; with 2 blocks 108, with 8 102).
 FwdPlan plan_forward(const Shape& s, int dtype) {
   FwdPlan p;
   const bool wide = padded_dim(s.D) * static_cast<int>(dtype_size(dtype)) == 512;

@@ -9,8 +9,8 @@
 //  * attn_dkv_kernel: a wave owns 32 keys (its K and V in registers) and passes over the row tiles of every
 //    query head that shares the key head.
 // Both recompute S and dO V^T (7 products in all; one kernel would need 5 and atomics, or dQ partials, to sum dQ).
-// Bound as the forward: 124 x 948 over 948, 8 heads of 64, fp16: dQ 430 us (796 TFLOP/s of its 3 products), dK and dV
-// 600 us (760 of their 4), together 1050 (543 of the 5 that are needed).
+// Bound as the forward: 124 x 948 over 948, 8 heads of 64, fp16: dQ 451 us (758 TFLOP/s of its 3 products), dK and dV
+// 615 us (742 of their 4), together 1066 (535 of the 5 that are needed); the least of six passes 426 and 573.
 // Few owners over a long axis are split over it: fp32 partial sums in the workspace, added in a fixed order.
 //
 // fp16 only: P and dS are rounded to 16 bits as operands, and fp16 loses digits below 2^-14.  Both are scaled by
@@ -482,7 +482,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
 // them (unrounded, and O is not read: with few keys a rounded O would cost dQ and dK half a rounding more).  P and dS
 // then go through LDS, rows down and keys across, to be the other operand of dV and dK, of which each wave owns 32
 // keys.  5 products instead of 7, and every tensor is moved once: 1032 x 62 queries over 62 keys, bf16, 8 heads of 64
-// take 113 us, of which the bytes need 88.
+// take 105 us, of which the bytes need 88.
 // fp16: P is held at 2^14; dS at a power of two from its own largest magnitude in the row tile, and dK's sum is
 // brought to a tile's power when that is the smaller one.
 // Waves that share a SIMD: fp16's scaling and the dropped bits together pass the registers of two.

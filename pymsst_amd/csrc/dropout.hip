@@ -9,8 +9,9 @@
 // tail keeps its digits.  The derivative Phi(x) + x phi(x) shares the exponential.
 //
 // A thread takes whole blocks of 8 elements (one Philox block, 16 bytes of a 16-bit type).  Bound: HBM
-// (x and y, or dy, x and dx, once each): 63984 x 768 bf16 with a GELU 37 us forward (5.3 TB/s; without the random
-// numbers 38, so they are hidden) and 48 us backward (6.1 TB/s); 63984 x 192 with a residual 12.5 us (5.9 TB/s).
+// (x and y, or dy, x and dx, once each): 63984 x 768 bf16 with a GELU 40 us forward (4.9 TB/s; with p = 0, without the
+// random numbers, 38 to 40, so they are hidden) and 44 us backward (6.7 TB/s, x still in the last-level cache); 63984 x 192
+// with a residual 12.5 us (5.9 TB/s, likewise).
 #include "common.h"
 #include "philox.h"
 
@@ -20,8 +21,8 @@ namespace {
 constexpr int kDropThreads = 256;
 
 // Blocks of 8 elements a thread loads before it computes: 2, but 1 for the GELU forward, whose arithmetic needs the
-// waves that the second block's registers cost (63984 x 768 bf16: 42 us, with 2 46; a residual sum 63984 x 192:
-// 13.4 us, with 1 14.1).
+// waves that the second block's registers cost (63984 x 768 bf16, one call after the other: 39 us, with 2 42; a residual
+// sum 63984 x 192: 12.6 us, with 1 13.4).
 template <int ACT, bool SECOND>
 constexpr int drop_unroll() { return ACT == PMSST_ACT_GELU && !SECOND ? 1 : 2; }
 
