@@ -475,8 +475,10 @@ def _patch_core_attention_gates(ext: Any, mode: str) -> bool:
     def attention_forward_cuda_ext(self, x):
         return self.to_out(gated_heads(self, x)) if takes(self, x) else original(self, x)
 
-    if original_heads is not None:
-        attention_forward_cuda_ext._pymsst_gated_heads = lambda self, x: (gated_heads if takes(self, x) else original_heads)(self, x)
+    def either_heads(self, x):
+        return gated_heads(self, x) if takes(self, x) else original_heads(self, x)
+
+    attention_forward_cuda_ext._pymsst_gated_heads = either_heads if original_heads is not None else None
     attention_forward_cuda_ext._pymsst_fused_attention_gates = True
     attention_forward_cuda_ext._pymsst_fused_attention_gate_mode = mode
     attention_forward_cuda_ext._pymsst_original_forward = original
@@ -576,12 +578,13 @@ def _patch_core_dropout(ext: Any) -> bool:
         if (before_last is None or not x.is_cuda or not chain(seq, count) or not drops(seq[count - 1])
                 or not _only_forward(block)):
             return block(x) + x
-        y, last = before_last(block, x), seq[count - 1]
+        last = seq[count - 1]
+        p, y = last.p, before_last(block, x)
         if y.dtype not in _FLOAT_TYPES:
             return last(y) + x
         if y.dtype != x.dtype:
-            return dropout(y, last.p, extension=ext) + x
-        return dropout(y, last.p, residual=x, extension=ext)
+            return dropout(y, p, extension=ext) + x
+        return dropout(y, p, residual=x, extension=ext)
 
     def transformer_cuda_ext(self, x):
         if _under_transform():
