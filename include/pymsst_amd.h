@@ -443,6 +443,74 @@ int pmsst_cross_attention_backward(const void* grad_out, const int64_t* grad_out
                                    int64_t kv_heads, int64_t head_dim, double scale, double dropout_p, const int64_t* rng,
                                    int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ local attention
+ * No reference counterpart.  Cross attention (its layouts, strides, masks, shared heads and rounding) where a query
+ * sees the frames of a window and a few first ones, with a learned bias by distance added to the scores.  Query n of
+ * batch row b stands at frame p = query_starts[b] + n (device int32, cut to [-2^29, 2^29]; NULL: n) of the keys' axis
+ * and sees frame j where key_mask and key_lengths let it,
+ *   j <= p + right  and  (j >= p - left  or  j < sinks);        left, right: -1 for no limit, at most 2^29
+ *   S = scale q k^T + bias[bucket_of[clamp(j - p, -max_distance, max_distance) + max_distance], head]
+ * bias: [buckets, heads], fp32 or q's dtype (bias_dtype), or NULL; bucket_of: device int32[2 max_distance + 1], read
+ * cut to [0, buckets); max_distance and buckets at most 1024.  Finite entries of the bias are cut to +-2^20; one of
+ * -1e30 or less (-inf, the lowest number of fp32 and bf16) hides its bucket's frames.  With a bias, scale lies in
+ * [2^-20, 2^20].
+ * What frames hide by key_mask or key_lengths is not read into any result.  A frame that the window alone hides from a
+ * query has weight 0, and 0 times what it holds is added: such frames must be finite.  A query that sees no frame gets
+ * out = 0 and lse = -inf, and no gradient.  Results are the same bit for bit on every run.
+ */
+
+/* Bytes of workspace of the forward on the current device (0 unless few queries meet many frames). */
+size_t pmsst_local_attention_forward_workspace_size(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                                    int64_t kv_heads, int64_t head_dim, int64_t left, int64_t right,
+                                                    int64_t sinks, int has_starts, int dtype);
+/* out[batch, queries, heads, head_dim] dense; lse[batch, heads, queries] = log sum exp(S), fp32, may be NULL. */
+int pmsst_local_attention_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                  const void* v, const int64_t* v_strides, const uint8_t* key_mask,
+                                  int64_t key_mask_stride, const int32_t* key_lengths, const int32_t* query_starts,
+                                  int64_t left, int64_t right, int64_t sinks, const void* bias, int bias_dtype,
+                                  const int32_t* bucket_of, int64_t buckets, int64_t max_distance, void* out, float* lse,
+                                  int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                  double scale, int dtype, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of the backward on the current device (buckets: 0 without a bias). */
+size_t pmsst_local_attention_backward_workspace_size(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                                     int64_t kv_heads, int64_t head_dim, int64_t left, int64_t right,
+                                                     int64_t sinks, int has_starts, int64_t buckets, int dtype);
+/* Gradients of the forward (same masks, limits, bias and scale) from its dense out and its lse: grad_q[batch, queries,
+ * heads, head_dim], grad_k and grad_v[batch, keys, kv_heads, head_dim], and with a bias grad_bias[buckets, heads] in
+ * the bias's dtype, all dense and fully written (exact zeros in grad_q and grad_k where a query sees one frame).
+ * An fp32 grad_bias of 16-bit tensors is summed from unrounded fp32 values.
+ * bucket_order, bucket_first: device int32[2 max_distance + 1] and [buckets + 1], the indexes of bucket_of in the order
+ * of their buckets, and where each bucket's begin. */
+int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out_strides, const void* q,
+                                   const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                   const int64_t* v_strides, const void* out, const float* lse,
+                                   const uint8_t* key_mask, int64_t key_mask_stride, const int32_t* key_lengths,
+                                   const int32_t* query_starts, int64_t left, int64_t right, int64_t sinks, const void* bias,
+                                   int bias_dtype, const int32_t* bucket_of, const int32_t* bucket_order,
+                                   const int32_t* bucket_first, int64_t buckets, int64_t max_distance, void* grad_q,
+                                   void* grad_k, void* grad_v, void* grad_bias, int64_t batch, int64_t queries, int64_t keys,
+                                   int64_t heads, int64_t kv_heads, int64_t head_dim, double scale, int dtype,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of the step on the current device (0 unless few streams have long windows). */
+size_t pmsst_local_attention_step_workspace_size(int64_t batch, int64_t frames, int64_t heads, int64_t kv_heads,
+                                                 int64_t head_dim, int64_t left, int64_t sinks, int dtype);
+/* Frame by frame: `frames` new frames of each stream are written into its caches and attended to with what the caches
+ * hold.  Stream b stands at frame positions[b] (device int32), which q, k, v[b, 0] are; frame f lies in slot f of the
+ * caches if f < sinks, else in slot sinks + (f - sinks) % (slots - sinks).  A query at frame p sees the frames from
+ * p - left to p and the first `sinks`; slots - sinks must be at least left + frames.  positions[b] < 0: the stream is
+ * idle, its caches stay as they are and its out is 0.  k_cache, v_cache: [batch, slots, kv_heads, head_dim] with
+ * strides as elsewhere (no two elements in one place), apart from q, k and v; bias as in the forward. */
+int pmsst_local_attention_step(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                               const void* v, const int64_t* v_strides, void* k_cache, const int64_t* k_cache_strides,
+                               void* v_cache, const int64_t* v_cache_strides, const int32_t* positions, int64_t left,
+                               int64_t sinks, const void* bias, int bias_dtype, const int32_t* bucket_of, int64_t buckets,
+                               int64_t max_distance, void* out, int64_t batch, int64_t frames, int64_t slots, int64_t heads,
+                               int64_t kv_heads, int64_t head_dim, double scale, int dtype, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

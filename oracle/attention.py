@@ -1,4 +1,4 @@
-"""64-bit statements of the dropout and the cross attention (test infrastructure only; no reference kernels:
+"""64-bit statements of the dropout, the cross attention and the local attention (test infrastructure only; no reference kernels:
 the stock blocks run ``nn.Dropout``, ``nn.GELU`` and SDPA).
 
 Nothing is rounded to a storage dtype here: the tests' bars count the rounding.
@@ -11,7 +11,8 @@ import math
 import numpy as np
 
 __all__ = ["philox4x32", "dropout_bits", "dropout_factors", "gelu", "gelu_grad", "dropout_forward", "dropout_backward",
-           "cross_attention_forward", "cross_attention_backward"]
+           "cross_attention_forward", "cross_attention_backward", "local_attention_forward", "local_attention_backward",
+           "local_attention_step"]
 
 _M32 = 0xFFFFFFFF
 
@@ -134,3 +135,119 @@ def cross_attention_backward(grad, q, k, v, key_mask=None, key_lengths=None, sca
             dq[i, :, j] = ds @ kk
             dk[i, :, c] += ds.T @ q[i, :, j]
     return dq, dk, dv
+
+
+# ---------------------------------------------------------------------- local attention
+
+
+def local_seen(b, n, m, left=None, right=None, sinks=0, starts=None, key_mask=None, key_lengths=None):
+    """``[B, N, M]``: whether query ``n`` of batch row ``b`` sees frame ``m``."""
+    p = np.arange(n)[None, :, None] + (0 if starts is None else np.asarray(starts, dtype=np.int64)[:, None, None])
+    j = np.arange(m)[None, None, :]
+    seen = np.repeat(_seen(b, m, key_mask, key_lengths)[:, None, :], n, axis=1)
+    if right is not None:
+        seen &= j <= p + right
+    if left is not None:
+        seen &= (j >= p - left) | (j < sinks)
+    return seen
+
+
+def bias_numbers(bias):
+    """The bias's entries as they count: those of -1e30 or less hide, others are cut to +-2^20."""
+    return np.where(bias <= -1e30, -np.inf, np.clip(bias, -(2.0**20), 2.0**20))
+
+
+def _local_bias(bias, bucket_of, distance):
+    """``(bias[..., H], bucket)`` of an array of distances."""
+    most = (len(bucket_of) - 1) // 2
+    bucket = np.asarray(bucket_of)[np.clip(distance, -most, most) + most]
+    return bias_numbers(bias)[bucket], bucket
+
+
+def _local_weights(q, k, scale, seen, added):
+    """One head: ``(P[N, M], lse[N])`` of the scores ``scale q k^T + added`` where ``seen``."""
+    s = np.where(seen, (q @ k.T) * scale + added, -np.inf)
+    top = s.max(axis=1, initial=-np.inf)
+    e = np.exp(s - np.where(np.isfinite(top), top, 0.0)[:, None])
+    total = e.sum(axis=1)
+    with np.errstate(divide="ignore"):
+        lse = np.where(total > 0, np.log(total) + np.where(np.isfinite(top), top, 0.0), -np.inf)
+    return e / np.where(total > 0, total, 1.0)[:, None], lse
+
+
+def _local_parts(q, k, v, left, right, sinks, bias, bucket_of, key_mask, key_lengths, starts, scale):
+    """For every batch row and head: its index, K and V without what no query may read, the seen pairs, the added
+    bias and the pairs' buckets."""
+    b, n, h, d = q.shape
+    m, hk = k.shape[1:3]
+    kept = _seen(b, m, key_mask, key_lengths)
+    seen = local_seen(b, n, m, left, right, sinks, starts, key_mask, key_lengths)
+    for i in range(b):
+        p = np.arange(n)[:, None] + (0 if starts is None else int(starts[i]))
+        added, bucket = (np.zeros((n, m, h)), None) if bias is None else _local_bias(bias, bucket_of, np.arange(m)[None] - p)
+        for j in range(h):
+            c = j // (h // hk)
+            kk, vv = (np.where(kept[i][:, None], t[i, :, c], 0.0) for t in (k, v))
+            yield i, j, c, kk, vv, seen[i], added[..., j], bucket
+
+
+def local_attention_forward(q, k, v, left=None, right=None, sinks=0, bias=None, bucket_of=None, key_mask=None,
+                            key_lengths=None, starts=None, scale=None):
+    """``q[B, N, H, D]`` over ``k`` / ``v[B, M, Hk, D]`` -> ``(out[B, N, H, D], lse[B, H, N])``."""
+    b, n, h, d = q.shape
+    scale = d**-0.5 if scale is None else scale
+    out, lse = np.zeros((b, n, h, d)), np.zeros((b, h, n))
+    for i, j, c, kk, vv, seen, added, _ in _local_parts(q, k, v, left, right, sinks, bias, bucket_of, key_mask, key_lengths,
+                                                        starts, scale):
+        w, lse[i, j] = _local_weights(q[i, :, j], kk, scale, seen, added)
+        out[i, :, j] = w @ vv
+    return out, lse
+
+
+def local_attention_backward(grad, q, k, v, left=None, right=None, sinks=0, bias=None, bucket_of=None, key_mask=None,
+                             key_lengths=None, starts=None, scale=None):
+    """``(grad_q, grad_k, grad_v, grad_bias or None)``."""
+    d = q.shape[3]
+    scale = d**-0.5 if scale is None else scale
+    dq, dk, dv = np.zeros(q.shape), np.zeros(k.shape), np.zeros(v.shape)
+    db = None if bias is None else np.zeros(bias.shape)
+    for i, j, c, kk, vv, seen, added, bucket in _local_parts(q, k, v, left, right, sinks, bias, bucket_of, key_mask,
+                                                             key_lengths, starts, scale):
+        w, _ = _local_weights(q[i, :, j], kk, scale, seen, added)
+        g = grad[i, :, j]
+        dv[i, :, c] += w.T @ g
+        dw = g @ vv.T
+        ds = w * (dw - (w * dw).sum(axis=1, keepdims=True))
+        dq[i, :, j] = ds @ kk * scale
+        dk[i, :, c] += ds.T @ q[i, :, j] * scale
+        if bias is not None:
+            np.add.at(db[:, j], bucket, ds)
+    return dq, dk, dv, db
+
+
+def ring_slot(frame: int, sinks: int, ring: int) -> int:
+    return frame if frame < sinks else sinks + (frame - sinks) % ring
+
+
+def local_attention_step(q, k, v, k_cache, v_cache, positions, left, sinks=0, bias=None, bucket_of=None, scale=None):
+    """``(out[B, N, H, D], k_cache, v_cache)``; the caches given are left as they are."""
+    b, n, h, d = q.shape
+    hk, ring = k.shape[2], k_cache.shape[1] - sinks
+    scale = d**-0.5 if scale is None else scale
+    out, kc, vc = np.zeros((b, n, h, d)), k_cache.copy(), v_cache.copy()
+    for i in range(b):
+        p = int(positions[i])
+        if p < 0:
+            continue
+        for x in range(n):
+            at = ring_slot(p + x, sinks, ring)
+            kc[i, at], vc[i, at] = k[i, x], v[i, x]
+        frames = np.array([f for f in range(p + n) if f < sinks or f >= p - left])
+        slots = np.array([ring_slot(int(f), sinks, ring) for f in frames])
+        distance = frames[None, :] - (p + np.arange(n))[:, None]
+        seen = (distance <= 0) & ((distance >= -left) | (frames < sinks)[None, :])
+        added = np.zeros((n, len(frames), h)) if bias is None else _local_bias(bias, bucket_of, distance)[0]
+        for j in range(h):
+            w, _ = _local_weights(q[i, :, j], kc[i, slots, j // (h // hk)], scale, seen, added[..., j])
+            out[i, :, j] = w @ vc[i, slots, j // (h // hk)]
+    return out, kc, vc

@@ -16,7 +16,7 @@
 // fp16 only: P and dS are rounded to 16 bits as operands, and fp16 loses digits below 2^-14.  Both are scaled by
 // powers of two that cannot overflow, from the bound |dO V^T o f - D| <= 2 max|V| |dO row|_1 / (1 - p); a small
 // kernel before the others takes the maxima.
-#include "attention.h"
+#include "attention_bwd.h"
 
 namespace pmsst {
 namespace {
@@ -41,31 +41,9 @@ struct BwdArgs {
   Dropout drop;
 };
 
-constexpr int kParts = 16;
-constexpr uint32_t kBoundPairs = 1u << 18;  // pairs of a grid row of attn_bound_kernel: 2^30 work-items
-
 // Rows of a passing tile: 64, or 32 where its two LDS tiles, twice, would pass 64 KB.
 template <typename T, int DP>
 constexpr int bwd_tile() { return DP * sizeof(T) == 512 ? 32 : 64; }
-
-// What stands for dO past the last row: these rows have no weight, but 0 times the last one's infinities is none.
-__device__ const u32x4_t zero_row[32] = {};
-
-// Largest power of two that keeps bound * 2^e <= 2^top (0 where the bound says nothing).
-__device__ __forceinline__ int scale_exponent(float bound, int top) {
-  if (!(bound > 0.f) || bound > 3e38f) return 0;
-  int x;
-  frexpf(bound, &x);
-  const int e = top - x;
-  return e < -100 ? -100 : e > 100 ? 100 : e;
-}
-
-__device__ __forceinline__ float parts_max(const float* parts) {
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) m = fmaxf(m, parts[i]);
-  return m;
-}
 
 // fp16: dK's power of two, of a pair (P is held at 2^14 there, so dS at 2^(14 + this)).
 __device__ __forceinline__ int pair_exponent(const BwdArgs& a, uint32_t pair) {
@@ -97,60 +75,6 @@ __device__ __forceinline__ bool seen_outside(const uint8_t* mask, int count, int
     if (__any(any != 0)) return true;
   }
   return false;
-}
-
-// ---------------------------------------------------------------- fp16 bounds
-
-template <typename T>
-__global__ __launch_bounds__(256) void attn_bound_kernel(BwdArgs a) {
-  __shared__ float red[2][4];
-  const Shape& s = a.s;
-  const uint32_t pair = blockIdx.y * kBoundPairs + blockIdx.x / kParts;
-  const int part = static_cast<int>(blockIdx.x % kParts);
-  if (pair >= static_cast<uint32_t>(s.B) * s.Hk) return;
-  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
-  // 4, 8 or 16 lanes a row, 16 bytes each
-  const int units = s.D / 8, log_lanes = units <= 4 ? 2 : units <= 8 ? 3 : 4;
-  const int lane_u = threadIdx.x & ((1 << log_lanes) - 1), row_u = threadIdx.x >> log_lanes, step = 256 >> log_lanes;
-  const int count = key_count(a.km, b, s.M);
-  const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
-  const T* gb = static_cast<const T*>(a.dout) + b * a.gs.b;
-  float vm = 0.f, lm = 0.f;
-#pragma unroll 4
-  for (int64_t m = part * step + row_u; m < count; m += step * kParts) {
-    if (a.km.mask && a.km.mask[b * a.km.stride + m] == 0) continue;
-    if (lane_u < units) {
-      float x[8];
-      load_pack<T, 8>(vb + m * a.vs.n + 8 * lane_u, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vm = fmaxf(vm, fabsf(x[i]));
-    }
-  }
-#pragma unroll 4
-  for (int64_t r = part * step + row_u; r < s.R; r += step * kParts) {
-    const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(r))), head = hk * s.G + static_cast<int>(r) - n * s.G;
-    float sum = 0.f;
-    if (lane_u < units) {
-      float x[8];
-      load_pack<T, 8>(gb + n * a.gs.n + head * a.gs.h + 8 * lane_u, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum += fabsf(x[i]);
-    }
-    lm = fmaxf(lm, group_sum(sum, 1 << log_lanes));
-  }
-  for (int off = 32; off > 0; off >>= 1) {
-    vm = fmaxf(vm, __shfl_xor(vm, off, kWave));
-    lm = fmaxf(lm, __shfl_xor(lm, off, kWave));
-  }
-  if ((threadIdx.x & 63) == 0) {
-    red[0][threadIdx.x >> 6] = vm;
-    red[1][threadIdx.x >> 6] = lm;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    a.vmax[pair * kParts + part] = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    a.l1[pair * kParts + part] = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
-  }
 }
 
 // ---------------------------------------------------------------- dQ
@@ -816,10 +740,7 @@ int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
     }
   }
   if constexpr (std::is_same<T, f16>::value) {
-    const dim3 grid(static_cast<uint32_t>(std::min<int64_t>(pairs, kBoundPairs) * kParts),
-                    static_cast<uint32_t>((pairs + kBoundPairs - 1) / kBoundPairs));
-    attn_bound_kernel<T><<<grid, 256, 0, stream>>>(a);
-    const int rc = check_launch("attn_bound_kernel");
+    const int rc = launch_bound<T>(a, pairs, stream);
     if (rc != PMSST_OK) return rc;
   }
   a.tiles = static_cast<uint32_t>(p.q_tiles);

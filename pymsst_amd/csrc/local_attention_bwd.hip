@@ -1,0 +1,834 @@
+// Local attention backward.  With P the weights, recomputed from the saved lse, and dO the output's gradient:
+//   D  = rowsum(dO o O)          dV = P^T dO          dS = P o (dO V^T - D)
+//   dQ = scale dS K              dK = scale dS^T Q    dbias[c] = sum of dS over the pairs whose distance has bucket c
+//
+// Two kernels as in the cross attention, so that every sum has one owner: local_dq_kernel (a wave owns 32 queries and
+// passes over the frames they see; it also writes D) and local_dkv_kernel (a wave owns 32 frames
+// and passes over the queries that see them).
+//
+// The first frames (sinks) are seen by every later query: the block of their keys would pass over all rows while others
+// pass over a window's.  Their rows past the window go to blocks of their own, as many tiles each as an ordinary block
+// has; the sums meet in fp32 in the workspace and a third kernel adds them.
+//
+// The bias's gradient sums dS along diagonals, in local_dkv_kernel.  A wave's 32 x 32 tile holds 63 of them.  With one
+// frame a lane and 8 queries in a row in its registers, adding the registers one after the other while the sum moves on by
+// a lane in between brings every diagonal into one lane: 16 additions with a lane shift in the same instruction, for
+// either half of the wave.  39 sums of 8 queries then go to the wave's own bins in LDS, one a distance.  Tiles beyond the
+// table's distances add up in registers.  The bins of a block are summed by bucket, in a fixed order, and a last kernel
+// adds the blocks.
+#include "attention_bwd.h"
+#include "local_attention.h"
+
+namespace pmsst {
+namespace {
+
+using namespace attn;
+
+struct BwdArgs {
+  const void *q, *k, *v, *out, *dout;
+  Strides qs, ks, vs, os, gs;
+  KeyMask km;
+  Window w;
+  BiasArgs bias;
+  const float* lse;  // [B, H, N]
+  void *dq, *dk, *dv, *dbias;
+  // [B * H, rows_pad]: -lse in log2 units (- inf: no weight), D, and 0 where a query sees one frame alone (else 1)
+  float *base, *delta, *alive;
+  int32_t rows_pad;     // N rounded up to 64
+  float *vmax, *l1;     // fp16: [pairs, kParts] maxima of |V| over the seen frames and of |dO row|_1
+  float *part_k, *part_v;  // [1 + chunks, pairs, sink_keys, D], NULL: no sinks
+  float* part_bias;     // [H, B * blocks of a pair in local_dkv_kernel, buckets]
+  Shape s;
+  Grid grid;
+  uint32_t row_tiles, key_tiles, sink_tiles, chunks;
+  int32_t chunk_tiles, sink_keys;
+  bool late_first;
+  float scale, scale_log2, bias_unit;
+  struct { float factor; } drop;  // what attn_bound_kernel's bound is multiplied by: no dropout here
+};
+
+// Rows of a passing tile: 64, or 32 where its two LDS tiles, twice, would pass 64 KB.
+template <typename T, int DP>
+constexpr int local_tile() { return DP * sizeof(T) == 512 ? 32 : 64; }
+
+// fp16: dK's power of two, of a pair (P is held at 2^14 there, so dS at 2^(14 + this)).
+__device__ __forceinline__ int pair_exponent(const BwdArgs& a, uint32_t pair) {
+  return scale_exponent(2.f * parts_max(a.l1 + pair * kParts) * parts_max(a.vmax + pair * kParts), 1);
+}
+
+// ---------------------------------------------------------------- diagonals
+
+// The value of the lane before (after) this one; 0 enters at the wave's end.
+__device__ __forceinline__ float from_before(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x138, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float from_after(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x130, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float keep_bits(float x, uint32_t m) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & m);
+}
+// Adds to a bin of this wave alone: one instruction's lanes have bins of their own, and a wave's come in order.
+__device__ __forceinline__ void add_bin(float* bin, float x) {
+  __hip_atomic_fetch_add(bin, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+
+// Adds the diagonals of x (lane l: frame l % 32, queries reg_key(i) + 8 (l / 32)) to bins[query - frame].  A lower lane's
+// query c at frame r ends in lane r + 7 - c: it moves up with each query after it; the 7 places past lane 31 are
+// free, as the upper half's values are left out.  The upper half moves down likewise.
+__device__ __forceinline__ void add_diagonals(float* bins, const f32x16_t& x, int lane) {
+  const uint32_t low = lane < 32 ? ~0u : 0u;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    float up = keep_bits(x[8 * s], low), down = keep_bits(x[8 * s + 7], ~low);
+#pragma unroll
+    for (int c = 1; c < 8; ++c) {
+      up = from_before(up) + keep_bits(x[8 * s + c], low);
+      down = from_after(down) + keep_bits(x[8 * s + 7 - c], ~low);
+    }
+    if (lane < 39) add_bin(bins + (16 * s + 7 - lane), up);
+    if (lane >= 25) add_bin(bins + (16 * s + 40 - lane), down);
+  }
+}
+
+// ---------------------------------------------------------------- dQ
+
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 ? 1 : 2))) void local_dq_kernel(BwdArgs a) {
+  constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
+  constexpr int BK = local_tile<T, DP>(), SUBS = BK / 32;
+  constexpr bool kHalf = std::is_same<T, f16>::value;
+  __shared__ __attribute__((aligned(16))) char lds[kStages][2][BK * DB];
+  extern __shared__ float table[];  // the bias by distance
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t pair, sub_block;
+  if (!locate(a.grid, pair, sub_block)) return;
+  const Shape& s = a.s;
+  const uint32_t tile_up = s.by_g.div(sub_block), g = sub_block - tile_up * static_cast<uint32_t>(s.G);
+  const uint32_t row_tile = a.late_first ? a.row_tiles - 1 - tile_up : tile_up;
+  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk, head = hk * s.G + static_cast<int>(g);
+  const int d_units = s.D * static_cast<int>(sizeof(T)) / 16;
+  const int64_t bh = static_cast<int64_t>(b) * s.H + head;
+
+  const int n0 = static_cast<int>(row_tile) * 32 * NW, n = n0 + wave * 32 + (lane & 31);
+  const bool row_ok = n < s.N;
+  const bool idle = n0 + wave * 32 >= s.N;  // no query of this wave is there: it only moves tiles
+  const int n_at = row_ok ? n : 0;
+  u32x4_t qf[NS], gf[NS];
+  float delta = 0.f, l1 = 0.f;
+  load_frags<T, DP>(static_cast<const T*>(a.dout) + b * a.gs.b + head * a.gs.h + n_at * a.gs.n, row_ok, d_units, h, gf);
+  {
+    u32x4_t of[NS];
+    load_frags<T, DP>(static_cast<const T*>(a.out) + b * a.os.b + head * a.os.h + n_at * a.os.n, row_ok, d_units, h, of);
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      float x[E], y[E];
+      unpack<T>(of[i], x);
+      unpack<T>(gf[i], y);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        delta = fmaf(x[j], y[j], delta);
+        if constexpr (kHalf) l1 += fabsf(y[j]);
+      }
+    }
+    delta = half_sum(delta);
+  }
+  hold(true);
+  load_frags<T, DP>(static_cast<const T*>(a.q) + b * a.qs.b + head * a.qs.h + n_at * a.qs.n, row_ok, d_units, h, qf);
+  // -lse in log2 units: a row that sees no frame (and one past the end) has no weight
+  float base = -kInf;
+  if (row_ok) {
+    const float lse = a.lse[bh * s.N + n];
+    base = lse == -kInf ? -kInf : -lse * kLog2e;
+  }
+
+  const int count = key_count(a.km, b, s.M);
+  const int start = start_of(a.w, b);
+  const int p0 = start + n0 + wave * 32, pos = start + n;
+  const TileList list = tiles_of<BK>(a.w, start + n0, start + min(n0 + 32 * NW, s.N) - 1, count);
+  const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
+  const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
+  const uint8_t* mask = a.km.mask ? a.km.mask + b * a.km.stride : nullptr;
+  const int low = low_of(a.w, pos), high = high_of(a.w, pos, count);
+  const int sinks = min(a.w.sinks, high);
+  auto mask_byte = [&](int t) { return mask[min(t * BK + lane, count - 1)]; };
+  constexpr uint64_t kAll = BK == 64 ? ~uint64_t{0} : 0xFFFFFFFFu;
+
+  // Where a query sees one frame alone, P is 1 whatever the score: dS, and with it dQ and dK, is zero exactly, while P
+  // from lse and D from O would leave their rounding errors.
+  int found = 0;
+  if (mask == nullptr) {
+    found = max(0, high - low) + max(0, min(sinks, low));
+  } else {
+    for (int i = 0; i < list.total; ++i) {  // ends where every query has two
+      const int key0 = list.at(i) * BK;
+      uint64_t seen = range_bits(key0, count) & __ballot(mask_byte(list.at(i)) != 0) & kAll;
+#pragma unroll
+      for (int u = 0; u < SUBS; ++u) {
+        const int at = key0 + 32 * u;
+        found += __popc(static_cast<uint32_t>(seen >> (32 * u)) & frames_seen(low, high, a.w.sinks, at));
+      }
+      if (!__any(row_ok && found < 2)) break;
+    }
+  }
+  const float alive = found == 1 ? 0.f : 1.f;
+  const bool any_lone = __any(found == 1);
+
+  const float row_base = base;
+  int e = 0;
+  if constexpr (kHalf) {
+    e = scale_exponent(2.f * half_sum(l1) * parts_max(a.vmax + pair * kParts), 15);
+    base += static_cast<float>(e);
+  }
+
+  f32x16_t acc[DT]{};
+  Tile<T, DP, BK, NW> kt, vt;
+  auto k_at = [&](int i) { return i * a.ks.n; };
+  auto v_at = [&](int i) { return i * a.vs.n; };
+  const int64_t k_step = BK * static_cast<int64_t>(sizeof(T)) * a.ks.n, v_step = BK * static_cast<int64_t>(sizeof(T)) * a.vs.n;
+  kt.start(kb, list.at(0) * BK, d_units, k_at);
+  vt.start(vb, list.at(0) * BK, d_units, v_at);
+  uint8_t byte_now = 1, byte_next = 1;  // this lane's key of the mask
+  auto fetch = [&](int i, int stage) {
+    const int key0 = list.at(i) * BK;
+    if (DB < 512 && key0 + BK <= count) {
+      if (i == list.sink && i != 0) {
+        skip(kt, (list.first - i) * k_step);
+        skip(vt, (list.first - i) * v_step);
+      }
+      kt.fetch(lds[stage][0], k_step);
+      vt.fetch(lds[stage][1], v_step);
+    } else {
+      kt.fetch_cut(lds[stage][0], kb, key0, count, d_units, k_at);
+      vt.fetch_cut(lds[stage][1], vb, key0, count, d_units, v_at);
+    }
+  };
+  arrive(qf);
+  arrive(gf);
+  asm volatile("" : "+v"(base), "+v"(delta));
+  if (mask && list.total > 0) byte_next = mask_byte(list.at(0));
+  if (list.total > 0) fetch(0, 0);
+  const float* lane_table = nullptr;  // this lane's entry for frame 0
+  float far_low = 0.f, far_high = 0.f, rest[2] = {0.f, 0.f};
+  if constexpr (BIAS) {
+    fill_bias<T, false>(table, a.bias, s.H, head, a.bias_unit, 64 * NW);
+    __syncthreads();
+    far_low = table[0];
+    far_high = table[2 * a.bias.distance + 2 * kPad];
+    lane_table = table + (a.bias.distance + kPad + 8 * h - pos);
+  }
+  int stage = 0;
+  for (int i = 0; i < list.total; ++i) {
+    const int t = list.at(i);
+    char* kl = lds[stage][0];
+    char* vl = lds[stage][1];
+    uint64_t seen = range_bits(t * BK, count);
+    if (mask) {
+      byte_now = byte_next;
+      seen &= __ballot(byte_now != 0);
+      if (i + 1 < list.total) byte_next = mask_byte(list.at(i + 1));
+    }
+    seen &= kAll;
+    vm_wait<0>();  // this wave's moves of the tile have arrived
+    if (seen != kAll || d_units != kt.UNITS) {
+      kt.clear(kl, seen, d_units);
+      vt.clear(vl, seen, d_units);
+    }
+    __syncthreads();
+    if (i + 1 < list.total) fetch(i + 1, stage ^ 1);
+    stage ^= 1;
+    if (idle) continue;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      const int key0 = t * BK + 32 * u;
+      const uint32_t sub_seen = static_cast<uint32_t>(seen >> (32 * u));
+      const Sees what = sees(a.w, p0, key0, count);
+      if (sub_seen == 0 || what == Sees::kNone) continue;
+      const int at_lane = fresh<DB>(lane);
+      f32x16_t p;
+      if constexpr (BIAS) {
+        bool upper;
+        if (bias_far(key0 - p0 - 31, a.bias.distance, upper)) {
+          const float far = upper ? far_high : far_low;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p[r] = far;
+        } else {
+          p = bias_tile(lane_table + key0);
+        }
+        p = mma_rows_from<T, DP>(p, kl, u, qf, at_lane);
+      } else {
+        p = mma_rows<T, DP>(kl, u, qf, at_lane);
+      }
+      const f32x16_t dp = mma_rows<T, DP>(vl, u, gf, at_lane);
+      if (what == Sees::kSome || sub_seen != 0xFFFFFFFFu) {
+        uint32_t bits = sub_seen;
+        if (what == Sees::kSome) bits &= frames_seen(low, high, a.w.sinks, key0);
+        bits >>= 8 * h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = where_bit(bits, reg_key(r), p[r], -kInf);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base)) * (dp[r] - delta);
+      }
+      if (any_lone) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] *= alive;
+      }
+      if constexpr (BIAS) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) rest[r & 1] += p[r];
+      }
+      mma_cols<T, DP>(kl, u, p, acc, at_lane);
+    }
+  }
+  if (row_ok) {
+    const float out_scale = kHalf ? ldexpf(a.scale, -e) : a.scale;
+    const int64_t at = (static_cast<int64_t>(b) * s.N + n) * s.H + head;
+    store_cols<T, DP>(static_cast<T*>(a.dq) + at * s.D, acc, out_scale, s.D, h);
+  }
+  // for the other kernel, in the form it takes them; rows past the end have no weight
+  if constexpr (BIAS) {
+    // What a row's dS adds up to, 0 but for D's error (out is rounded, and so were the weights it is a sum of): with it, D
+    // is rowsum(P o dP) to fp32's precision, which the bias's gradient needs (with D from out it is 3e-4 off).
+    const float total = half_sum(rest[0] + rest[1]);
+    delta += kHalf ? ldexpf(total, -e) : total;
+  }
+  if (h == 0 && n < a.rows_pad) {
+    if constexpr (kHalf) delta = ldexpf(delta, pair_exponent(a, pair));
+    const int64_t at = bh * a.rows_pad + n;
+    a.base[at] = row_base + (kHalf ? 14.f : 0.f);
+    a.delta[at] = delta;
+    a.alive[at] = alive;
+  }
+}
+
+// dbias[bucket, head] = the sum of the blocks' parts, in a fixed order; 32 buckets a block.
+template <typename B>
+__global__ __launch_bounds__(1024) void local_bias_sum_kernel(const float* parts, B* out, int64_t blocks, int buckets, int heads) {
+  __shared__ float red[32][33];
+  const int c = static_cast<int>(blockIdx.y) * 32 + static_cast<int>(threadIdx.x & 31), y = threadIdx.x >> 5;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < buckets) {
+    const float* part = parts + static_cast<int64_t>(blockIdx.x) * blocks * buckets + c;
+    int64_t i = y;
+    for (; i + 96 < blocks; i += 128) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += part[(i + 32 * j) * buckets];
+    }
+    for (; i < blocks; i += 32) sum[0] += part[i * buckets];
+  }
+  red[y][threadIdx.x & 31] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  __syncthreads();
+  if (threadIdx.x < 32 && c < buckets) {
+    float t = 0.f;
+    for (int j = 0; j < 32; ++j) t += red[j][threadIdx.x];
+    out[static_cast<int64_t>(c) * heads + blockIdx.x] = from_f32<B>(t);
+  }
+}
+
+// ---------------------------------------------------------------- dK, dV
+
+// Waves that share a SIMD: fp32 rows of 64 with a bias pass the registers of two by a few.
+template <typename T, int DP, bool BIAS>
+constexpr int dkv_waves() { return DP == 128 || (DP == 64 && BIAS && sizeof(T) == 4) ? 1 : 2; }
+
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_waves<T, DP, BIAS>()))) void local_dkv_kernel(BwdArgs a) {
+  constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
+  constexpr int BQ = local_tile<T, DP>(), SUBS = BQ / 32;
+  constexpr bool kHalf = std::is_same<T, f16>::value;
+  __shared__ __attribute__((aligned(16))) char lds[kStages][2][BQ * DB];
+  __shared__ __attribute__((aligned(16))) float stat[kStages][3][64];  // -lse (log2 units), D, alive
+  extern __shared__ float table[];  // the bias by falling distance, then each wave's bins
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t pair, sub_block;
+  if (!locate(a.grid, pair, sub_block)) return;
+  const Shape& s = a.s;
+  // the ordinary blocks, then those of the sinks' later rows
+  uint32_t key_tile = sub_block, slot = 0;
+  if (sub_block >= a.key_tiles) {
+    const uint32_t i = sub_block - a.key_tiles;
+    slot = i / a.sink_tiles;
+    key_tile = i - slot * a.sink_tiles;
+    ++slot;
+  }
+  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
+  const int d_units = s.D * static_cast<int>(sizeof(T)) / 16;
+  const int count = key_count(a.km, b, s.M);
+  const int start = start_of(a.w, b);
+  const int block_key0 = static_cast<int>(key_tile) * 32 * NW, block_end = min(block_key0 + 32 * NW, count);
+  const int key0 = block_key0 + wave * 32, ki = key0 + (lane & 31);
+  const bool seen = ki < count && (a.km.mask == nullptr || a.km.mask[b * a.km.stride + ki] != 0);
+  const bool idle = key0 >= count;  // no frame of this wave counts: it only moves tiles
+  const bool any_unseen = __any(!seen);
+
+  const RowTiles rows = rows_of<BQ>(a.w, start, s.N, s.G, block_key0, block_end, static_cast<int>(slot),
+                                    static_cast<int>(a.chunks), a.chunk_tiles);
+  const int first = rows.first, tiles = rows.tiles, from = rows.from, to = block_key0 < count ? rows.to : rows.from;
+  float* part_bias = nullptr;  // of the pair's first head; further heads lie part_step apart
+  int64_t part_step = 0;
+  if constexpr (BIAS) {
+    part_step = static_cast<int64_t>(s.B) * a.grid.per * a.bias.buckets;
+    part_bias = a.part_bias + hk * s.G * part_step + (static_cast<int64_t>(b) * a.grid.per + sub_block) * a.bias.buckets;
+    // the heads that have no tile here
+    const int g_from = from < to ? from / tiles : 0, g_to = from < to ? (to - 1) / tiles + 1 : 0;
+    for (int g = 0; g < s.G; ++g) {
+      if (g >= g_from && g < g_to) continue;
+      for (int c = threadIdx.x; c < a.bias.buckets; c += 64 * NW) part_bias[g * part_step + c] = 0.f;
+    }
+  }
+
+  f32x16_t dk[DT]{}, dv[DT]{};
+  float k_scale = a.scale, v_scale = 1.f;
+  if (from < to) {
+    u32x4_t kf[NS], vf[NS];
+    load_frags<T, DP>(static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h + (seen ? ki * a.ks.n : 0), seen, d_units, h, kf);
+    load_frags<T, DP>(static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h + (seen ? ki * a.vs.n : 0), seen, d_units, h, vf);
+    // P' = 2^14 P (in base), dS' = P' 2^e (...): as in the cross attention
+    float dp_scale = 1.f, dp_unscale = 1.f;
+    if constexpr (kHalf) {
+      const int e = pair_exponent(a, pair);
+      dp_scale = ldexpf(1.f, e);
+      dp_unscale = ldexpf(1.f, -e);
+      k_scale = ldexpf(a.scale, -e - 14);
+      v_scale = ldexpf(1.f, -14);
+    }
+    const T* qb = static_cast<const T*>(a.q) + b * a.qs.b;
+    const T* gb = static_cast<const T*>(a.dout) + b * a.gs.b;
+    const int64_t q_step = BQ * static_cast<int64_t>(sizeof(T)) * a.qs.n, g_step = BQ * static_cast<int64_t>(sizeof(T)) * a.gs.n;
+    Tile<T, DP, BQ, NW> qt, gt;
+    auto q_at = [&](int i) { return i * a.qs.n; };
+    auto g_at = [&](int i) { return i * a.gs.n; };
+    int next_g = from / tiles, next_t = first + from - next_g * tiles;  // the tile that is fetched next
+    const T *q_head = nullptr, *g_head = nullptr;
+    const float* stat_head = nullptr;
+    auto begin_head = [&] {
+      const int head = hk * s.G + next_g;
+      q_head = qb + head * a.qs.h;
+      g_head = gb + head * a.gs.h;
+      qt.start(q_head, next_t * BQ, d_units, q_at);
+      gt.start(g_head, next_t * BQ, d_units, g_at);
+      stat_head = a.base + (static_cast<int64_t>(b) * s.H + head) * a.rows_pad + lane;
+    };
+    const int64_t stat_step = static_cast<int64_t>(s.B) * s.H * a.rows_pad;  // base, delta and alive follow each other
+    auto fetch = [&](int stage) {
+      const int row0 = next_t * BQ;
+      if (DB < 512 && row0 + BQ <= s.N) {
+        qt.fetch(lds[stage][0], q_step);
+        gt.fetch(lds[stage][1], g_step);
+      } else {
+        qt.fetch_cut(lds[stage][0], q_head, row0, s.N, d_units, q_at);
+        gt.fetch_cut(lds[stage][1], g_head, row0, s.N, d_units, g_at, reinterpret_cast<const T*>(zero_row));
+      }
+#pragma unroll
+      for (int j = 0; j < 3; j += NW < 3 ? NW : 3) {
+        const int which = j + wave;
+        if (which < 3 && (BQ == 64 || lane < BQ)) {
+          dma4_m0(stat_head + which * stat_step + row0, __builtin_amdgcn_readfirstlane(lds_addr(stat[stage][0]) + 256 * which));
+        }
+      }
+      if (++next_t == first + tiles) {
+        next_t = first;
+        ++next_g;
+      }
+    };
+    arrive(kf);
+    arrive(vf);
+    int g_now = next_g, t_now = next_t;
+    begin_head();
+    fetch(0);
+    const float* lane_table = nullptr;  // this lane's entry for a query at frame 0
+    float far_low = 0.f, far_high = 0.f, sum_low = 0.f, sum_high = 0.f;
+    const int entries = 2 * a.bias.distance + 1 + 2 * kPad;
+    float* bins = nullptr;
+    auto begin_table = [&](int g) {
+      fill_bias<T, true>(table, a.bias, s.H, hk * s.G + g, a.bias_unit, 64 * NW);
+      for (int i = lane; i < entries; i += 64) bins[i] = 0.f;
+      sum_low = sum_high = 0.f;
+      __syncthreads();
+      far_high = table[0];
+      far_low = table[entries - 1];
+    };
+    // a head's bins, summed by bucket
+    auto end_table = [&](int g) {
+      // past the table's ends, and the far tiles' sums: into the end bins
+      const float above = group_sum(sum_high + bins[lane], kWave);
+      const float under = group_sum(sum_low + bins[entries - kPad + lane], kWave);
+      if (lane == 0) {
+        bins[kPad] += above;
+        bins[entries - 1 - kPad] += under;
+      }
+      __syncthreads();
+      const int span = 2 * a.bias.distance + 1;
+      const float unscale = kHalf ? v_scale * dp_unscale : 1.f;
+      for (int c = threadIdx.x; c < a.bias.buckets; c += 64 * NW) {
+        const int begin = max(0, a.bias.first[c]), end = min(span, a.bias.first[c + 1]);
+        float sum = 0.f;
+        for (int i = begin; i < end; ++i) {
+          const float* bin = table + 2 * entries - 1 - kPad - min(max(a.bias.order[i], 0), span - 1);
+#pragma unroll
+          for (int w = 0; w < NW; ++w) sum += bin[w * entries];
+        }
+        part_bias[g * part_step + c] = sum * unscale;
+      }
+      __syncthreads();  // before the bins are cleared
+    };
+    if constexpr (BIAS) {
+      bins = table + entries * (1 + wave);
+      begin_table(g_now);
+      lane_table = table + (a.bias.distance + kPad + 8 * h - ki);
+    }
+    int stage = 0;
+    for (int i = from; i < to; ++i) {
+      char* ql = lds[stage][0];
+      char* gl = lds[stage][1];
+      const float* base = stat[stage][0];
+      const float* delta = stat[stage][1];
+      vm_wait<0>();  // this wave's moves of the tile have arrived
+      if (d_units != qt.UNITS) {
+        qt.clear(ql, ~uint64_t{0}, d_units);
+        gt.clear(gl, ~uint64_t{0}, d_units);
+      }
+      __syncthreads();
+      if constexpr (BIAS) {
+        if (i > from && t_now == first) {  // every wave is past the head before
+          end_table(g_now - 1);
+          begin_table(g_now);
+        }
+      }
+      const float* alive = stat[stage][2];
+      const uint64_t lone = __ballot((BQ == 64 || lane < BQ) && alive[BQ == 64 ? lane : lane & (BQ - 1)] == 0.f);
+      if (i + 1 < to) {
+        if (next_t == first) begin_head();
+        fetch(stage ^ 1);
+      }
+      stage ^= 1;
+      const int row_tile0 = t_now * BQ;
+      if (++t_now == first + tiles) {
+        t_now = first;
+        ++g_now;
+      }
+      if (idle) continue;
+#pragma unroll
+      for (int u = 0; u < SUBS; ++u) {
+        const int row0 = row_tile0 + 32 * u, p0 = start + row0;
+        if (row0 >= s.N) continue;
+        const Sees what = sees(a.w, p0, key0, count);
+        if (what == Sees::kNone) continue;
+        hold(sizeof(T) == 4);
+        const int at_lane = fresh<DB>(lane);
+        f32x16_t p;
+        bool near = false, upper = false;
+        if constexpr (BIAS) {
+          near = !bias_far(key0 - p0 - 31, a.bias.distance, upper);
+          if (near) {
+            p = bias_tile(lane_table + p0);
+          } else {
+            const float far = upper ? far_high : far_low;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] = far;
+          }
+          p = mma_rows_from<T, DP>(p, ql, u, kf, at_lane);
+        } else {
+          p = mma_rows<T, DP>(ql, u, kf, at_lane);
+        }
+        f32x16_t ds = mma_rows<T, DP>(gl, u, vf, at_lane);
+        // (what lanes of unseen frames hold is dropped at the end, but for the bias's sums)
+        if (what == Sees::kSome || (BIAS && any_unseen)) {
+          uint32_t bits = queries_seeing(a.w, start, ki, row0) >> (8 * h);
+          if constexpr (BIAS) bits = seen ? bits : 0u;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p[r] = where_bit(bits, reg_key(r), p[r], -kInf);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = 32 * u + reg_key(r) + 8 * h;
+          p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base[row]));
+          ds[r] = p[r] * fmaf(ds[r], dp_scale, -delta[row]);
+        }
+        const uint32_t sub_lone = static_cast<uint32_t>(lone >> (32 * u));
+        if (sub_lone != 0) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) ds[r] *= alive[32 * u + reg_key(r) + 8 * h];
+        }
+        if constexpr (BIAS) {
+          if (near) {
+            add_diagonals(bins + (a.bias.distance + kPad + p0 - key0), ds, lane);
+          } else {
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[r & 1] += ds[r];
+            const float both = sum[0] + sum[1];
+            sum_high += upper ? both : 0.f;
+            sum_low += upper ? 0.f : both;
+          }
+        }
+        hold(sizeof(T) == 4);
+        mma_cols<T, DP>(gl, u, p, dv, at_lane);
+        mma_cols<T, DP>(ql, u, ds, dk, at_lane);
+      }
+    }
+    if constexpr (BIAS) end_table(g_now - (t_now == first ? 1 : 0));
+  }
+  if (ki >= s.M) return;
+  if (!seen) {
+    // nothing was learnt about a frame that is not seen, whatever its columns of the tiles hold
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      dk[dt] = f32x16_t{};
+      dv[dt] = f32x16_t{};
+    }
+  }
+  if (key_tile < a.sink_tiles) {
+    const int64_t at = ((static_cast<int64_t>(slot) * a.grid.pairs + pair) * a.sink_keys + ki) * s.D;
+    store_cols_f32<T, DP>(a.part_k + at, dk, k_scale, s.D, h);
+    store_cols_f32<T, DP>(a.part_v + at, dv, v_scale, s.D, h);
+  } else {
+    const int64_t at = ((static_cast<int64_t>(b) * s.M + ki) * s.Hk + hk) * s.D;
+    store_cols<T, DP>(static_cast<T*>(a.dk) + at, dk, k_scale, s.D, h);
+    store_cols<T, DP>(static_cast<T*>(a.dv) + at, dv, v_scale, s.D, h);
+  }
+}
+
+// The sinks' keys: dk, dv = the sum of their blocks' parts.  A thread takes 4 columns; the grid's y is the gradient.
+template <typename T>
+__global__ __launch_bounds__(256) void local_sink_sum_kernel(BwdArgs a, int keys) {
+  const Shape& s = a.s;
+  const float* part = blockIdx.y != 0 ? a.part_v : a.part_k;
+  T* out = static_cast<T*>(blockIdx.y != 0 ? a.dv : a.dk);
+  const int64_t quads = s.D / 4, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= a.grid.pairs * keys * quads) return;
+  const int64_t row = i / quads, quad = i - row * quads, pair = row / keys, key = row - pair * keys;
+  const int64_t b = pair / s.Hk, hk = pair - b * s.Hk;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (uint32_t c = 0; c <= a.chunks; ++c) {
+    float x[4];
+    load_pack<float, 4>(part + (((static_cast<int64_t>(c) * a.grid.pairs + pair) * a.sink_keys + key) * quads + quad) * 4, x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] += x[j];
+  }
+  store_pack<T, 4>(out + ((b * s.M + key) * s.Hk + hk) * s.D + 4 * quad, o);
+}
+
+// ---------------------------------------------------------------- host
+
+struct BwdPlan {
+  int nw_q, nw_k;
+  int64_t row_tiles, key_tiles, sink_tiles, chunks, chunk_tiles;
+};
+
+BwdPlan plan_backward(const Shape& s, const Window& w, int dtype) {
+  const bool wide = padded_dim(s.D) * static_cast<int>(dtype_size(dtype)) == 512;
+  const int64_t bq = wide ? 32 : 64;
+  BwdPlan p{};
+  p.nw_q = s.N <= 64 && !wide ? 2 : 4;
+  p.nw_k = s.M <= 64 && !wide ? 2 : 4;
+  const int64_t block_keys = 32 * p.nw_k;
+  p.row_tiles = (int64_t{s.N} + 32 * p.nw_q - 1) / (32 * p.nw_q);
+  p.key_tiles = (int64_t{s.M} + block_keys - 1) / block_keys;
+  if (w.sinks > 0 && w.left >= 0) {
+    p.sink_tiles = std::min<int64_t>(p.key_tiles, (w.sinks + block_keys - 1) / block_keys);
+    // as many tiles a block as an ordinary one has, at least 8 (about 10 us)
+    const int64_t all = (int64_t{s.N} + bq - 1) / bq * s.G;
+    const int64_t usual = w.right < 0 ? all : (int64_t{w.left} + w.right + block_keys + bq - 1) / bq * s.G;
+    p.chunk_tiles = std::max<int64_t>(8, std::min(usual, all));
+    p.chunks = (all + p.chunk_tiles - 1) / p.chunk_tiles;
+  }
+  return p;
+}
+
+struct BwdSpace {
+  size_t stat, bound, part_k, part_bias, total;
+};
+
+BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int64_t buckets, int dtype) {
+  const size_t pairs = static_cast<size_t>(s.B) * s.Hk;
+  BwdSpace w;
+  w.stat = static_cast<size_t>(s.B) * s.H * align_up(s.N, 64) * 4;
+  w.bound = dtype == PMSST_F16 ? align_up(pairs * kParts * 4, 256) : 0;
+  const size_t sink_keys = p.sink_tiles * 32 * p.nw_k;
+  w.part_k = align_up((1 + p.chunks) * pairs * sink_keys * s.D * 4, 256);
+  w.part_bias = align_up(static_cast<size_t>(s.B) * s.H * (p.key_tiles + p.sink_tiles * p.chunks) * buckets * 4, 256);
+  w.total = align_up(3 * w.stat, 256) + 2 * w.bound + 2 * w.part_k + w.part_bias;
+  return w;
+}
+
+template <typename T, int DP, int NW>
+int launch_dq(const BwdArgs& a, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
+  if (a.bias.table) {
+    local_dq_kernel<T, DP, NW, true><<<grid, 64 * NW, bias_entries(a.bias.distance) * 4, stream>>>(a);
+  } else {
+    local_dq_kernel<T, DP, NW, false><<<grid, 64 * NW, 0, stream>>>(a);
+  }
+  return check_launch("local_dq_kernel");
+}
+
+template <typename T, int DP, int NW>
+int launch_dkv(const BwdArgs& a, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
+  if (a.bias.table) {
+    local_dkv_kernel<T, DP, NW, true><<<grid, 64 * NW, bias_entries(a.bias.distance) * 4 * (1 + NW), stream>>>(a);
+  } else {
+    local_dkv_kernel<T, DP, NW, false><<<grid, 64 * NW, 0, stream>>>(a);
+  }
+  return check_launch("local_dkv_kernel");
+}
+
+template <typename T, int DP>
+int launch_dkv(const BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+  if constexpr (DP * sizeof(T) != 512) {
+    if (p.nw_k == 2) return launch_dkv<T, DP, 2>(a, stream);
+  }
+  return launch_dkv<T, DP, 4>(a, stream);
+}
+
+template <typename T, int DP>
+int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+  const int64_t pairs = int64_t{a.s.B} * a.s.Hk;
+  int rc = PMSST_OK;
+  if constexpr (std::is_same<T, f16>::value) rc = launch_bound<T>(a, pairs, stream);
+  if (rc != PMSST_OK) return rc;
+  a.grid = make_grid(pairs, p.row_tiles * a.s.G);
+  if constexpr (DP * sizeof(T) != 512) {
+    rc = p.nw_q == 2 ? launch_dq<T, DP, 2>(a, stream) : launch_dq<T, DP, 4>(a, stream);
+  } else {
+    rc = launch_dq<T, DP, 4>(a, stream);
+  }
+  if (rc != PMSST_OK) return rc;
+  const int64_t per = p.key_tiles + p.sink_tiles * p.chunks;
+  if (per > 0) {
+    a.grid = make_grid(pairs, per);
+    rc = launch_dkv<T, DP>(a, p, stream);
+    if (rc != PMSST_OK) return rc;
+  }
+  if (a.bias.table) {
+    const dim3 grid(static_cast<uint32_t>(a.s.H), static_cast<uint32_t>((a.bias.buckets + 31) / 32));
+    const int64_t blocks = int64_t{a.s.B} * per;  // 0 without frames: zeros
+    if (a.bias.f32) {
+      local_bias_sum_kernel<float><<<grid, 1024, 0, stream>>>(a.part_bias, static_cast<float*>(a.dbias), blocks, a.bias.buckets, a.s.H);
+    } else {
+      local_bias_sum_kernel<T><<<grid, 1024, 0, stream>>>(a.part_bias, static_cast<T*>(a.dbias), blocks, a.bias.buckets, a.s.H);
+    }
+    if ((rc = check_launch("local_bias_sum_kernel")) != PMSST_OK) return rc;
+  }
+  if (p.sink_tiles == 0) return rc;
+  const int keys = std::min(a.sink_keys, a.s.M);
+  const int64_t blocks = (pairs * keys * (a.s.D / 4) + 255) / 256;
+  local_sink_sum_kernel<T><<<dim3(static_cast<uint32_t>(blocks), 2), 256, 0, stream>>>(a, keys);
+  return check_launch("local_sink_sum_kernel");
+}
+
+template <typename T>
+int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+  return a.s.D <= 32 ? run_bwd<T, 32>(a, p, stream) : a.s.D <= 64 ? run_bwd<T, 64>(a, p, stream) : run_bwd<T, 128>(a, p, stream);
+}
+
+}  // namespace
+}  // namespace pmsst
+
+extern "C" {
+
+size_t pmsst_local_attention_backward_workspace_size(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
+                                                     int64_t head_dim, int64_t left, int64_t right, int64_t sinks,
+                                                     int has_starts, int64_t buckets, int dtype) {
+  using namespace pmsst::attn;
+  LocalArgs l;
+  static const int32_t some = 0;
+  if (make_local("pmsst_local_attention_backward", batch, queries, keys, heads, kv_heads, head_dim, left, right, sinks,
+                 has_starts ? &some : nullptr, nullptr, 0, nullptr, 0, 0, 1.0, dtype, l) != PMSST_OK ||
+      buckets < 0 || buckets > kMaxBuckets || l.s.B == 0 || l.s.N == 0)
+    return 0;
+  return pmsst::bwd_space(l.s, pmsst::plan_backward(l.s, l.w, dtype), buckets, dtype).total;
+}
+
+int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out_strides, const void* q, const int64_t* q_strides,
+                                   const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                   const void* out, const float* lse, const uint8_t* key_mask, int64_t key_mask_stride,
+                                   const int32_t* key_lengths, const int32_t* query_starts, int64_t left,
+                                   int64_t right, int64_t sinks, const void* bias, int bias_dtype, const int32_t* bucket_of,
+                                   const int32_t* bucket_order, const int32_t* bucket_first, int64_t buckets,
+                                   int64_t max_distance, void* grad_q, void* grad_k, void* grad_v, void* grad_bias, int64_t batch,
+                                   int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t head_dim, double scale,
+                                   int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace pmsst;
+  using namespace pmsst::attn;
+  const char* what = "pmsst_local_attention_backward";
+  LocalArgs l;
+  int rc = make_local(what, batch, queries, keys, heads, kv_heads, head_dim, left, right, sinks, query_starts, bias, bias_dtype,
+                      bucket_of, buckets, max_distance, scale, dtype, l);
+  if (rc != PMSST_OK) return rc;
+  if (batch == 0) return PMSST_OK;
+  PMSST_REQUIRE(queries > 0, "%s: queries must be positive (the other gradients are zero without any)", what);
+  PMSST_REQUIRE(grad_out && q && out && lse && grad_q && (keys == 0 || (k && v && grad_k && grad_v)), "%s: null pointer", what);
+  PMSST_REQUIRE(bias == nullptr || (grad_bias && bucket_order && bucket_first), "%s: null pointer (bias)", what);
+  BwdArgs a{};
+  a.s = l.s;
+  a.w = l.w;
+  a.bias = l.bias;
+  a.bias.order = bucket_order;
+  a.bias.first = bucket_first;
+  if ((rc = make_strides(what, grad_out, grad_out_strides, queries, heads, head_dim, dtype, a.gs)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, out, nullptr, queries, heads, head_dim, dtype, a.os)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, q, q_strides, queries, heads, head_dim, dtype, a.qs)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, k, k_strides, keys, kv_heads, head_dim, dtype, a.ks)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, v, v_strides, keys, kv_heads, head_dim, dtype, a.vs)) != PMSST_OK) return rc;
+  PMSST_REQUIRE(((reinterpret_cast<uintptr_t>(grad_q) | reinterpret_cast<uintptr_t>(grad_k) | reinterpret_cast<uintptr_t>(grad_v)) &
+                 15) == 0,
+                "%s: gradients must be 16-byte aligned", what);
+  const BwdPlan p = plan_backward(a.s, a.w, dtype);
+  const BwdSpace w = bwd_space(a.s, p, bias ? buckets : 0, dtype);
+  if (workspace == nullptr || workspace_bytes < w.total)
+    return fail(PMSST_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, w.total, workspace_bytes);
+  PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: workspace must be 16-byte aligned", what);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.dout = grad_out;
+  a.km = {key_mask, key_mask_stride, key_lengths};
+  a.lse = lse;
+  a.dq = grad_q;
+  a.dk = grad_k;
+  a.dv = grad_v;
+  a.dbias = grad_bias;
+  char* at = static_cast<char*>(workspace);
+  a.rows_pad = static_cast<int32_t>(align_up(a.s.N, 64));
+  a.base = reinterpret_cast<float*>(at);
+  a.delta = reinterpret_cast<float*>(at + w.stat);
+  a.alive = reinterpret_cast<float*>(at + 2 * w.stat);
+  at += align_up(3 * w.stat, 256);
+  a.vmax = reinterpret_cast<float*>(at);
+  at += w.bound;
+  a.l1 = reinterpret_cast<float*>(at);
+  at += w.bound;
+  a.part_k = reinterpret_cast<float*>(at);
+  at += w.part_k;
+  a.part_v = reinterpret_cast<float*>(at);
+  at += w.part_k;
+  a.part_bias = reinterpret_cast<float*>(at);
+  a.row_tiles = static_cast<uint32_t>(p.row_tiles);
+  a.key_tiles = static_cast<uint32_t>(p.key_tiles);
+  a.sink_tiles = static_cast<uint32_t>(p.sink_tiles);
+  a.chunks = static_cast<uint32_t>(p.chunks);
+  a.chunk_tiles = static_cast<int32_t>(p.chunk_tiles);
+  a.sink_keys = static_cast<int32_t>(p.sink_tiles * 32 * p.nw_k);
+  a.late_first = a.w.right >= 0 && a.w.left < 0;
+  const int64_t per = std::max(p.row_tiles * a.s.G, p.key_tiles + p.sink_tiles * p.chunks);
+  PMSST_REQUIRE(grid_fits(batch * kv_heads, per), "%s: too many rows for one call", what);
+  PMSST_REQUIRE(batch * kv_heads * a.sink_keys * (head_dim / 4) < int64_t{1} << 31, "%s: too many sinks for one call", what);
+  a.scale = static_cast<float>(scale);
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  a.bias_unit = static_cast<float>(1.0 / scale);
+  a.drop.factor = 1.f;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case PMSST_F32: return run_bwd<float>(a, p, st);
+    case PMSST_F16: return run_bwd<f16>(a, p, st);
+    default: return run_bwd<bf16>(a, p, st);
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,446 @@
+// Local attention frame by frame: a few new frames of each stream are written into its ring caches and attended to with
+// the first frames (sinks) and the last ones that the caches hold, in one launch.
+//
+// The bytes of the keys and values bound it, so there are no matrix instructions and no LDS tiles: a row of K is
+// spread over the lanes of a group, 16 bytes each, and a wave's load takes 64 / group rows.  Every lane keeps the
+// products' columns it loads: its part of q, of the sums O, and its group's own maximum and sum of the weights.  Groups
+// meet once, at the end: within the wave by lane exchanges, between waves through LDS, between blocks (where few
+// streams have long windows) through the workspace and a second kernel.
+//
+// A block takes up to 8 rows (query heads that share the key head, times new frames) so that each K and V is read once
+// for all of them.
+//
+// The slots that are written hold frames that no query of the call sees (slots - sinks >= left + frames), and the new
+// frames are read from k and v, not from the caches: no block waits for another.
+#include "local_attention.h"
+
+namespace pmsst {
+namespace {
+
+using namespace attn;
+
+struct StepArgs {
+  const void *q, *k, *v;
+  void *k_cache, *v_cache;
+  Strides qs, ks, vs, kcs, vcs;
+  const int32_t* positions;
+  int32_t left, sinks, ring;
+  BiasArgs bias;
+  void* out;
+  float *part_o, *part_m, *part_l;  // [splits, B * Hk, R, D] and [splits, B * Hk, R]: sums, maxima, sums of weights
+  Shape s;                          // N: new frames; R = G * N rows of a (stream, key head), r = n * G + g
+  Grid grid;                        // per = row chunks * splits
+  FastDiv by_ring;
+  uint32_t splits;
+  int32_t per_split;                // frames
+  float scale_log2;
+};
+
+// 16 bytes as floats.
+template <typename T>
+struct Unit {
+  static constexpr int E = 16 / sizeof(T);
+};
+
+// What the lanes past a row's end multiply (with 0: nothing there may be infinite).
+static __device__ const u32x4_t zero_unit = {0, 0, 0, 0};
+
+constexpr int kUnroll = 4;  // loads of K (and of V) on their way in a wave
+
+// LPR: lanes of a row (a power of two), RT: rows of the block.
+template <typename T, int LPR, int RT, bool BIAS>
+__global__ __launch_bounds__(256) void local_step_kernel(StepArgs a) {
+  constexpr int E = Unit<T>::E, KPW = 64 / LPR;
+  extern __shared__ float shared[];  // the bias of the rows' heads by distance back, then the waves' results
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  uint32_t pair, sub;
+  if (!locate(a.grid, pair, sub)) return;
+  const Shape& s = a.s;
+  const uint32_t chunk = sub / a.splits, split = sub - chunk * a.splits;
+  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
+  const int r0 = static_cast<int>(chunk) * RT, rows = min(RT, s.R - r0);
+  const int unit = lane & (LPR - 1), slot_in_wave = lane / LPR;
+  const bool unit_ok = unit < s.D / E;
+  const int at = unit_ok ? unit * E : 0;
+  const int32_t now = a.positions[b];
+
+  // the stream's frames in the order they are visited: the sinks' (their slots are their frames), the window's, the new
+  const int sink_frames = now < 0 ? 0 : min(a.sinks, now);
+  const int window_first = max(sink_frames, now - a.left);
+  const int window_frames = now < 0 ? 0 : now - window_first;
+  const int old_frames = sink_frames + window_frames;
+  const int total = now < 0 ? 0 : old_frames + s.N;
+  // (a window that holds frames begins behind the sinks)
+  const uint32_t window_slot = window_frames > 0 ? a.by_ring.mod(static_cast<uint32_t>(window_first - a.sinks)) : 0u;
+
+  const T* kc = static_cast<const T*>(a.k_cache) + b * a.kcs.b + hk * a.kcs.h;
+  const T* vc = static_cast<const T*>(a.v_cache) + b * a.vcs.b + hk * a.vcs.h;
+  const T* kn = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
+  const T* vn = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
+
+  const int x0 = static_cast<int>(split) * a.per_split;
+  const int x1 = split + 1 == a.splits ? total : min(total, x0 + a.per_split);
+
+  // where frame number x of the order lies
+  auto locate_frame = [&](int x, const T*& kp, const T*& vp) {
+    if (x < old_frames) {
+      uint32_t slot = static_cast<uint32_t>(x);
+      if (x >= sink_frames) {
+        slot = window_slot + static_cast<uint32_t>(x - sink_frames);
+        if (slot >= static_cast<uint32_t>(a.ring)) slot -= a.ring;
+        slot += a.sinks;
+      }
+      kp = kc + slot * a.kcs.n;
+      vp = vc + slot * a.vcs.n;
+    } else {
+      kp = kn + (x - old_frames) * a.ks.n;
+      vp = vn + (x - old_frames) * a.vs.n;
+    }
+  };
+  auto frame_of = [&](int x) { return x < sink_frames ? x : x < old_frames ? window_first + (x - sink_frames) : now + (x - old_frames); };
+
+  u32x4_t kf[kUnroll], vf[kUnroll];
+  const int step = KPW * kUnroll * waves;
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int x = min(base + u * KPW + slot_in_wave, x1 - 1);
+      const T *kp, *vp;
+      locate_frame(x, kp, vp);
+      kf[u] = *(unit_ok ? reinterpret_cast<const u32x4_t*>(kp + at) : &zero_unit);
+      vf[u] = *(unit_ok ? reinterpret_cast<const u32x4_t*>(vp + at) : &zero_unit);
+    }
+  };
+  const int first = x0 + wave * KPW * kUnroll;
+  if (first < x1) fetch(first);
+
+  // q in log2 units
+  float q[RT][E], o[RT][E], m[RT], l[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    m[r] = -kInf;
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) q[r][i] = o[r][i] = 0.f;
+    if (r < rows && unit_ok) {
+      const int row = r0 + r, n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(row))), head = hk * s.G + (row - n * s.G);
+      load_pack<T, E>(static_cast<const T*>(a.q) + b * a.qs.b + n * a.qs.n + head * a.qs.h + at, q[r]);
+#pragma unroll
+      for (int i = 0; i < E; ++i) q[r][i] *= a.scale_log2;
+    }
+  }
+
+  // the new frames go into the caches: once, by the block of the first rows and frames
+  if (sub == 0 && now >= 0) {
+    const int units = s.D / E;
+    for (int i = threadIdx.x; i < s.N * units; i += blockDim.x) {
+      const int n = i / units, u = i - n * units;
+      const uint32_t frame = static_cast<uint32_t>(now) + static_cast<uint32_t>(n);
+      const uint32_t slot = frame < static_cast<uint32_t>(a.sinks)
+                                ? frame
+                                : a.sinks + a.by_ring.mod(frame - static_cast<uint32_t>(a.sinks));
+      *reinterpret_cast<u32x4_t*>(static_cast<T*>(a.k_cache) + b * a.kcs.b + hk * a.kcs.h + slot * a.kcs.n + u * E) =
+          *reinterpret_cast<const u32x4_t*>(kn + n * a.ks.n + u * E);
+      *reinterpret_cast<u32x4_t*>(static_cast<T*>(a.v_cache) + b * a.vcs.b + hk * a.vcs.h + slot * a.vcs.n + u * E) =
+          *reinterpret_cast<const u32x4_t*>(vn + n * a.vs.n + u * E);
+    }
+  }
+
+  const int entries = a.bias.distance + 1;  // distances 0 .. back
+  if constexpr (BIAS) {
+    const int heads = min(rows, s.G);
+    for (int i = threadIdx.x; i < heads * entries; i += blockDim.x) {
+      const int g = i / entries, back = i - g * entries;
+      const int head = hk * s.G + (r0 + g) % s.G;
+      shared[i] = bias_value(a.bias, dtype_code<T>(), s.H, head, -back, kLog2e);
+    }
+    __syncthreads();
+  }
+
+  for (int base = first; base < x1; base += step) {
+    u32x4_t kg[kUnroll], vg[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      kg[u] = kf[u];
+      vg[u] = vf[u];
+    }
+    if (base + step < x1) fetch(base + step);
+    float w[RT][kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float x[E];
+      unpack<T>(kg[u], x);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) sum = fmaf(q[r][i], x[i], sum);
+        w[r][u] = group_sum(sum, LPR);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int x = base + u * KPW + slot_in_wave;
+      const int frame = frame_of(x);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(r0 + r)));
+        const int back = now + n - frame;
+        const bool seen = x < x1 && back >= 0 && (back <= a.left || frame < a.sinks);
+        if constexpr (BIAS) {
+          const int g = s.G >= RT ? r : r % s.G;
+          w[r][u] += shared[min(g, min(rows, s.G) - 1) * entries + min(max(back, 0), a.bias.distance)];
+        }
+        w[r][u] = seen ? w[r][u] : -kInf;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float top = w[r][0];
+#pragma unroll
+      for (int u = 1; u < kUnroll; ++u) top = fmaxf(top, w[r][u]);
+      if (top > m[r]) {
+        const float alpha = __builtin_amdgcn_exp2f(m[r] - top);
+        m[r] = top;
+        l[r] *= alpha;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[r][i] *= alpha;
+      }
+      const float ref = m[r] == -kInf ? 0.f : m[r];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        w[r][u] = __builtin_amdgcn_exp2f(w[r][u] - ref);
+        l[r] += w[r][u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float x[E];
+      unpack<T>(vg[u], x);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[r][i] = fmaf(w[r][u], x[i], o[r][i]);
+      }
+    }
+  }
+
+  // the wave's groups, then the waves
+  if constexpr (BIAS) __syncthreads();  // the bias has been read
+  const int pitch = s.D + 2;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    float top = m[r];
+#pragma unroll
+    for (int off = LPR; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+    const float f = m[r] == -kInf ? 0.f : __builtin_amdgcn_exp2f(m[r] - top);
+    l[r] = cross_group_sum(l[r] * f, LPR);
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[r][i] = cross_group_sum(o[r][i] * f, LPR);
+    float* to = shared + (wave * RT + r) * pitch;
+    if (slot_in_wave == 0 && unit_ok) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) to[at + i] = o[r][i];
+    }
+    if (lane == 0) {
+      to[s.D] = top;
+      to[s.D + 1] = l[r];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * s.D; i += blockDim.x) {
+    const int r = i / s.D, d = i - r * s.D;
+    float top = -kInf;
+    for (int w = 0; w < waves; ++w) top = fmaxf(top, shared[(w * RT + r) * pitch + s.D]);
+    float sum = 0.f, x = 0.f;
+    for (int w = 0; w < waves; ++w) {
+      const float* from = shared + (w * RT + r) * pitch;
+      const float f = from[s.D] == -kInf ? 0.f : __builtin_amdgcn_exp2f(from[s.D] - top);
+      sum = fmaf(f, from[s.D + 1], sum);
+      x = fmaf(f, from[d], x);
+    }
+    const int row = r0 + r;
+    if (a.part_o) {
+      const int64_t p = (static_cast<int64_t>(split) * a.grid.pairs + pair) * s.R + row;
+      a.part_o[p * s.D + d] = x;
+      if (d == 0) {
+        a.part_m[p] = top;
+        a.part_l[p] = sum;
+      }
+    } else {
+      const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(row))), head = hk * s.G + (row - n * s.G);
+      static_cast<T*>(a.out)[((static_cast<int64_t>(b) * s.N + n) * s.H + head) * s.D + d] = from_f32<T>(sum == 0.f ? 0.f : x / sum);
+    }
+  }
+}
+
+// Joins the splits: a thread takes a column of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void local_step_join_kernel(StepArgs a, uint32_t total) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= total) return;
+  const Shape& s = a.s;
+  const uint32_t prow = i / static_cast<uint32_t>(s.D), d = i - prow * static_cast<uint32_t>(s.D);
+  const int64_t rows = static_cast<int64_t>(a.grid.pairs) * s.R;
+  float top = -kInf, sum = 0.f, x = 0.f;
+  for (uint32_t k = 0; k < a.splits; ++k) top = fmaxf(top, a.part_m[k * rows + prow]);
+  for (uint32_t k = 0; k < a.splits; ++k) {
+    const float m = a.part_m[k * rows + prow], f = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    sum = fmaf(f, a.part_l[k * rows + prow], sum);
+    x = fmaf(f, a.part_o[(k * rows + prow) * s.D + d], x);
+  }
+  const uint32_t pair = prow / static_cast<uint32_t>(s.R);
+  const int row = static_cast<int>(prow - pair * static_cast<uint32_t>(s.R));
+  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
+  const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(row))), head = hk * s.G + (row - n * s.G);
+  static_cast<T*>(a.out)[((static_cast<int64_t>(b) * s.N + n) * s.H + head) * s.D + d] = from_f32<T>(sum == 0.f ? 0.f : x / sum);
+}
+
+// ---------------------------------------------------------------- host
+
+struct StepPlan {
+  int lanes, rows, waves;  // of a K row, of a block, of a block
+  int64_t chunks, splits, per_split;
+};
+
+StepPlan plan_step(const Shape& s, int64_t left, int64_t sinks, int dtype) {
+  StepPlan p;
+  const int units = s.D * static_cast<int>(dtype_size(dtype)) / 16;
+  p.lanes = units <= 4 ? 4 : units <= 8 ? 8 : units <= 16 ? 16 : 32;
+  p.rows = s.R == 1 ? 1 : s.R == 2 ? 2 : s.R <= 4 ? 4 : 8;
+  p.chunks = (int64_t{s.R} + p.rows - 1) / p.rows;
+  const int64_t frames = left + s.N + sinks, per_wave = 64 / p.lanes * kUnroll;
+  p.waves = 4;
+  const int64_t blocks = int64_t{s.B} * s.Hk * p.chunks, want = 2 * num_cus();
+  p.splits = 1;
+  if (blocks < want) p.splits = std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, frames / (per_wave * p.waves * 4)));
+  p.per_split = (frames + p.splits - 1) / p.splits;
+  p.splits = (frames + p.per_split - 1) / p.per_split;
+  return p;
+}
+
+size_t step_workspace(const Shape& s, const StepPlan& p) {
+  if (p.splits == 1) return 0;
+  const size_t rows = static_cast<size_t>(p.splits) * s.B * s.Hk * s.R;
+  return align_up(rows * s.D * 4, 256) + 2 * align_up(rows * 4, 256);
+}
+
+template <typename T, int LPR, int RT>
+int launch_step(const StepArgs& a, const StepPlan& p, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
+  const size_t results = static_cast<size_t>(p.waves) * RT * (a.s.D + 2) * 4;
+  if (a.bias.table) {
+    const size_t table = static_cast<size_t>(std::min<int>(RT, a.s.G)) * (a.bias.distance + 1) * 4;
+    local_step_kernel<T, LPR, RT, true><<<grid, 64 * p.waves, std::max(results, table), stream>>>(a);
+  } else {
+    local_step_kernel<T, LPR, RT, false><<<grid, 64 * p.waves, results, stream>>>(a);
+  }
+  return check_launch("local_step_kernel");
+}
+
+template <typename T, int LPR>
+int launch_step(const StepArgs& a, const StepPlan& p, hipStream_t stream) {
+  switch (p.rows) {
+    case 1: return launch_step<T, LPR, 1>(a, p, stream);
+    case 2: return launch_step<T, LPR, 2>(a, p, stream);
+    case 4: return launch_step<T, LPR, 4>(a, p, stream);
+    default: return launch_step<T, LPR, 8>(a, p, stream);
+  }
+}
+
+template <typename T>
+int run_step(const StepArgs& a, const StepPlan& p, hipStream_t stream) {
+  int rc = PMSST_OK;
+  if constexpr (sizeof(T) == 4) {
+    if (p.lanes == 32) rc = launch_step<T, 32>(a, p, stream);
+  }
+  if (p.lanes == 4) rc = launch_step<T, 4>(a, p, stream);
+  if (p.lanes == 8) rc = launch_step<T, 8>(a, p, stream);
+  if (p.lanes == 16) rc = launch_step<T, 16>(a, p, stream);
+  if (rc != PMSST_OK || p.splits == 1) return rc;
+  const uint32_t total = a.grid.pairs * static_cast<uint32_t>(a.s.R) * a.s.D;
+  local_step_join_kernel<T><<<dim3((total + 255) / 256), 256, 0, stream>>>(a, total);
+  return check_launch("local_step_join_kernel");
+}
+
+}  // namespace
+}  // namespace pmsst
+
+extern "C" {
+
+size_t pmsst_local_attention_step_workspace_size(int64_t batch, int64_t frames, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                                 int64_t left, int64_t sinks, int dtype) {
+  using namespace pmsst::attn;
+  LocalArgs l;
+  static const int32_t some = 0;
+  if (left < 0 || make_local("pmsst_local_attention_step", batch, frames, 0, heads, kv_heads, head_dim, left, 0, sinks, &some,
+                             nullptr, 0, nullptr, 0, 0, 1.0, dtype, l) != PMSST_OK ||
+      l.s.B == 0 || l.s.N == 0)
+    return 0;
+  return pmsst::step_workspace(l.s, pmsst::plan_step(l.s, left, sinks, dtype));
+}
+
+int pmsst_local_attention_step(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                               const int64_t* v_strides, void* k_cache, const int64_t* k_cache_strides, void* v_cache,
+                               const int64_t* v_cache_strides, const int32_t* positions, int64_t left, int64_t sinks,
+                               const void* bias, int bias_dtype, const int32_t* bucket_of, int64_t buckets, int64_t max_distance,
+                               void* out, int64_t batch, int64_t frames, int64_t slots, int64_t heads, int64_t kv_heads,
+                               int64_t head_dim, double scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace pmsst;
+  using namespace pmsst::attn;
+  const char* what = "pmsst_local_attention_step";
+  PMSST_REQUIRE(left >= 0, "%s: left must not be negative", what);
+  LocalArgs l;
+  int rc = make_local(what, batch, frames, slots, heads, kv_heads, head_dim, left, 0, sinks, positions, bias, bias_dtype, bucket_of,
+                      buckets, max_distance, scale, dtype, l);
+  if (rc != PMSST_OK) return rc;
+  if (batch == 0 || frames == 0) return PMSST_OK;
+  PMSST_REQUIRE(slots - sinks >= left + frames, "%s: the caches must have sinks + left + frames slots", what);
+  PMSST_REQUIRE(q && k && v && k_cache && v_cache && positions && out, "%s: null pointer", what);
+  StepArgs a{};
+  a.s = l.s;
+  a.bias = l.bias;
+  if ((rc = make_strides(what, q, q_strides, frames, heads, head_dim, dtype, a.qs)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, k, k_strides, frames, kv_heads, head_dim, dtype, a.ks)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, v, v_strides, frames, kv_heads, head_dim, dtype, a.vs)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, k_cache, k_cache_strides, slots, kv_heads, head_dim, dtype, a.kcs)) != PMSST_OK) return rc;
+  if ((rc = make_strides(what, v_cache, v_cache_strides, slots, kv_heads, head_dim, dtype, a.vcs)) != PMSST_OK) return rc;
+  const StepPlan p = plan_step(a.s, left, sinks, dtype);
+  const size_t need = step_workspace(a.s, p);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(PMSST_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
+  PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0 || need == 0, "%s: workspace must be 16-byte aligned", what);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.positions = positions;
+  a.left = static_cast<int32_t>(left);
+  a.sinks = static_cast<int32_t>(sinks);
+  a.ring = static_cast<int32_t>(slots - sinks);
+  a.by_ring = FastDiv(static_cast<uint32_t>(a.ring));
+  a.out = out;
+  if (need > 0) {
+    const size_t rows = static_cast<size_t>(p.splits) * a.s.B * a.s.Hk * a.s.R;
+    char* at = static_cast<char*>(workspace);
+    a.part_o = reinterpret_cast<float*>(at);
+    at += align_up(rows * a.s.D * 4, 256);
+    a.part_m = reinterpret_cast<float*>(at);
+    a.part_l = reinterpret_cast<float*>(at + align_up(rows * 4, 256));
+  }
+  a.splits = static_cast<uint32_t>(p.splits);
+  a.per_split = static_cast<int32_t>(p.per_split);
+  const int64_t pairs = batch * kv_heads, per = p.chunks * p.splits;
+  PMSST_REQUIRE(grid_fits(pairs, per), "%s: too many rows for one call", what);
+  a.grid = make_grid(pairs, per);
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case PMSST_F32: return run_step<float>(a, p, st);
+    case PMSST_F16: return run_step<f16>(a, p, st);
+    default: return run_step<bf16>(a, p, st);
+  }
+}
+
+}  // extern "C"

@@ -36,6 +36,35 @@ class BandRowsPlan(NamedTuple):
     num_sel: int
 
 
+class RelativeBiasPlan(NamedTuple):
+    """Device tables of a relative bias's buckets (see ``HipFusedExtension.relative_bias_plan``)."""
+
+    bucket_of: torch.Tensor
+    order: torch.Tensor
+    first: torch.Tensor
+    num_buckets: int
+    max_distance: int
+
+
+def relative_buckets(num_buckets: int, max_distance: int, bidirectional: bool = True) -> list[int]:
+    """The bucket of each distance ``-max_distance .. max_distance`` (frame minus query).
+
+    A side's distances have a bucket each up to half of its buckets, ``near``; further ones share
+    ``near + floor(log(f / near) / log(max_distance / near) * rest)``, cut to the last.  With ``bidirectional``
+    the frames ahead have the upper half of the buckets, else all that lies ahead has bucket 0.  Borders are
+    compared in whole numbers, so a distance on one lies in the bucket that begins there."""
+    side = num_buckets // 2 if bidirectional else num_buckets
+    near, j, behind = side // 2, 0, []
+    rest = side - near
+    for f in range(max_distance + 1):
+        # the last j with (f / near)^rest >= (max_distance / near)^j
+        while f >= near and j + 1 < rest and f**rest * near ** (j + 1) >= max_distance ** (j + 1) * near**rest:
+            j += 1
+        behind.append(f if f < near else near + j)
+    ahead = [side + b for b in behind[1:]] if bidirectional else [0] * max_distance
+    return behind[::-1] + ahead
+
+
 def _req(cond: bool, msg: str) -> None:
     if not cond:
         raise RuntimeError(msg)
@@ -660,6 +689,194 @@ class HipFusedExtension:
             )
         check(rc, "pmsst_cross_attention_backward")
         return [grad_q, grad_k, grad_v]
+
+    # ------------------------------------------------------------------ local attention
+
+    @staticmethod
+    def relative_bias_plan(num_buckets: int, max_distance: int, device, bidirectional: bool = True, bucket_of=None):
+        """Build-addition helper: device tables of a learned bias by distance for :meth:`local_attention_forward`,
+        its backward and :meth:`local_attention_step`, built once for a model.
+
+        The buckets are those of :func:`relative_buckets` (near distances one each, further ones by their
+        logarithm, from ``max_distance`` on the last), or ``bucket_of``, the bucket of each distance
+        ``-max_distance .. max_distance``.  Validated here."""
+        num_buckets, max_distance = int(num_buckets), int(max_distance)
+        _req(0 <= max_distance <= 1024 and 1 <= num_buckets <= 1024,
+             "max_distance must lie in [0, 1024] and num_buckets in [1, 1024]")
+        if bucket_of is None:
+            side = num_buckets // 2 if bidirectional else num_buckets
+            _req(side >= 2 and (not bidirectional or num_buckets % 2 == 0),
+                 "num_buckets must be at least 2 a side, and even where there are two")
+            _req(max_distance > side // 2, "max_distance must be larger than the distances with buckets of their own")
+            bucket_of = relative_buckets(num_buckets, max_distance, bidirectional)
+        of = torch.as_tensor(bucket_of, dtype=torch.int64).detach().cpu()
+        _req(of.shape == (2 * max_distance + 1,), "bucket_of must have 2 * max_distance + 1 entries")
+        _req(int(of.min()) >= 0 and int(of.max()) < num_buckets, "buckets must lie in [0, num_buckets)")
+        first = torch.zeros(num_buckets + 1, dtype=torch.int64)
+        first[1:] = torch.cumsum(torch.bincount(of, minlength=num_buckets), 0)
+        with torch.inference_mode(False):  # kept across modes
+            tables = [t.to(torch.int32).to(device) for t in (of, torch.argsort(of, stable=True), first)]
+        return RelativeBiasPlan(*tables, num_buckets, max_distance)
+
+    def _local_check(self, q, k, v, left, right, sinks, bias, plan, key_mask, key_lengths, query_starts, scale):
+        key_mask, stride, key_lengths, scale = self._attention_check(q, k, v, key_mask, key_lengths, scale, 0.0, None)
+        left, right = (-1 if t is None else int(t) for t in (left, right))
+        _req(-1 <= left <= 2**29 and -1 <= right <= 2**29, "left and right must be None or lie in [0, 2**29]")
+        _req(0 <= sinks <= 2**28, "sinks must lie in [0, 2**28]")
+        if query_starts is not None:
+            _req(query_starts.device == q.device and query_starts.dtype == torch.int32
+                 and query_starts.shape == (q.shape[0],), "query_starts must be an int32 tensor of shape [B] on q's device")
+            query_starts = query_starts.contiguous()
+        bias = self._bias_check(q, bias, plan, scale)
+        return left, right, int(sinks), bias, key_mask, stride, key_lengths, query_starts, scale
+
+    @staticmethod
+    def _bias_check(q, bias, plan, scale):
+        if bias is None:
+            return None
+        _req(plan is not None, "a bias needs its bias_plan")
+        _req(bias.device == q.device and bias.dtype in (q.dtype, torch.float32)
+             and bias.shape == (plan.num_buckets, q.shape[2]),
+             "bias must be a tensor of shape [num_buckets, H] on q's device, float32 or of q's dtype")
+        _req(plan.bucket_of.device == q.device, "bias_plan must be on q's device")
+        _req(2.0**-20 <= scale <= 2.0**20, "with a bias, scale must lie in [2**-20, 2**20]")
+        return bias.contiguous()
+
+    @staticmethod
+    def _bias_args(bias, plan, backward=False):
+        if bias is None:
+            return (None, 0, None, None, None, 0, 0) if backward else (None, 0, None, 0, 0)
+        tables = (plan.bucket_of, plan.order, plan.first) if backward else (plan.bucket_of,)
+        return (_ptr(bias), dtype_code(bias.dtype), *map(_ptr, tables), plan.num_buckets, plan.max_distance)
+
+    def local_attention_forward(self, q, k, v, left=None, right=None, sinks: int = 0, bias=None, bias_plan=None,
+                                key_mask=None, key_lengths=None, query_starts=None, scale=None, need_lse: bool = False):
+        """Build addition: :meth:`cross_attention_forward` where a query sees the frames of a window and a few first
+        ones, with a learned bias by distance.  Query ``n`` of ``q[B, N, H, D]`` stands at frame
+        ``p = query_starts[b] + n`` (int32 ``[B]``; 0 unless given) of the ``M`` frames of ``k`` / ``v[B, M, Hk, D]``
+        and sees frame ``j`` where the masks let it, ``j <= p + right``, and ``j >= p - left`` or ``j < sinks``
+        (``None``: no limit).
+
+        ``bias[num_buckets, H]`` (fp32 or q's dtype) with its ``bias_plan``: ``bias[bucket(j - p), h]`` is added to the
+        scaled scores; an entry of -1e30 or less hides its bucket's frames, others are cut to +-2**20.
+        Strides, shared heads, masks and scale as there.  A frame that only the window hides must be finite.
+
+        Returns ``[out]``, or ``[out, lse]`` with ``need_lse`` (``lse[B, H, N]`` fp32, what the backward takes)."""
+        left, right, sinks, bias, key_mask, mask_stride, key_lengths, query_starts, scale = self._local_check(
+            q, k, v, left, right, sinks, bias, bias_plan, key_mask, key_lengths, query_starts, scale)
+        code = dtype_code(q.dtype)
+        (q, qs), (k, ks), (v, vs) = self._attention_operand(q), self._attention_operand(k), self._attention_operand(v)
+        b, n, h, d = q.shape
+        m, hk = k.shape[1], k.shape[2]
+        out = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
+        lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device) if need_lse else None
+        with _DeviceGuard(q.device):
+            size = self._lib.pmsst_local_attention_forward_workspace_size(b, n, m, h, hk, d, left, right, sinks,
+                                                                          query_starts is not None, code)
+            ws = _workspace(size, q.device) if size else None
+            rc = self._lib.pmsst_local_attention_forward(
+                _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(key_mask), mask_stride, _ptr(key_lengths),
+                _ptr(query_starts), left, right, sinks, *self._bias_args(bias, bias_plan), _ptr(out), _ptr(lse),
+                b, n, m, h, hk, d, scale, code, _ptr(ws), size, _stream(q.device),
+            )
+        check(rc, "pmsst_local_attention_forward")
+        return [out, lse] if need_lse else [out]
+
+    def local_attention_backward(self, grad_out, q, k, v, out, lse, left=None, right=None, sinks: int = 0, bias=None,
+                                 bias_plan=None, key_mask=None, key_lengths=None, query_starts=None, scale=None):
+        """Gradients ``[grad_q, grad_k, grad_v]`` of :meth:`local_attention_forward` (dense, in the inputs' shapes), and
+        with a bias ``[grad_q, grad_k, grad_v, grad_bias]``, from its ``out`` and ``lse`` and the same other arguments.
+        The weights are computed again; every sum is taken in a fixed order."""
+        left, right, sinks, bias, key_mask, mask_stride, key_lengths, query_starts, scale = self._local_check(
+            q, k, v, left, right, sinks, bias, bias_plan, key_mask, key_lengths, query_starts, scale)
+        b, n, h, d = q.shape
+        m, hk = k.shape[1], k.shape[2]
+        for t, name in ((grad_out, "grad_out"), (out, "out")):
+            _req(t.device == q.device and t.shape == q.shape and t.dtype == q.dtype,
+                 f"{name} must have q's shape, dtype and device")
+        _req(lse.device == q.device and lse.dtype == torch.float32 and lse.shape == (b, h, n),
+             "lse must be the forward's, float32 [B, H, N]")
+        code = dtype_code(q.dtype)
+        grad_q = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
+        grad_k = torch.empty((b, m, hk, d), dtype=q.dtype, device=q.device)
+        grad_v = torch.empty((b, m, hk, d), dtype=q.dtype, device=q.device)
+        grads = [grad_q, grad_k, grad_v]
+        if bias is not None:
+            grads.append(torch.empty_like(bias))
+        if n == 0 or b == 0:
+            return [t.zero_() for t in grads]
+        (q, qs), (k, ks), (v, vs) = self._attention_operand(q), self._attention_operand(k), self._attention_operand(v)
+        grad_out, gs = self._attention_operand(grad_out)
+        (out, _), lse = self._attention_operand(out.contiguous()), lse.contiguous()
+        with _DeviceGuard(q.device):
+            size = self._lib.pmsst_local_attention_backward_workspace_size(
+                b, n, m, h, hk, d, left, right, sinks, query_starts is not None,
+                0 if bias is None else bias_plan.num_buckets, code)
+            ws = _workspace(size, q.device)
+            rc = self._lib.pmsst_local_attention_backward(
+                _ptr(grad_out), gs, _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(out), _ptr(lse),
+                _ptr(key_mask), mask_stride, _ptr(key_lengths), _ptr(query_starts), left, right, sinks,
+                *self._bias_args(bias, bias_plan, backward=True), _ptr(grad_q), _ptr(grad_k), _ptr(grad_v),
+                _ptr(grads[3]) if bias is not None else None, b, n, m, h, hk, d, scale, code, _ptr(ws), size,
+                _stream(q.device),
+            )
+        check(rc, "pmsst_local_attention_backward")
+        return grads
+
+    def local_attention_step(self, q, k, v, k_cache, v_cache, positions, left: int, sinks: int = 0, bias=None,
+                             bias_plan=None, scale=None):
+        """Build addition: frame-by-frame local attention.  The new frames ``k`` / ``v[B, N, Hk, D]`` of each stream are
+        written into its caches ``[B, slots, Hk, D]`` (in place) and ``q[B, N, H, D]`` attends to what they hold; returns
+        ``out[B, N, H, D]``.
+
+        ``positions`` (int32 ``[B]``, read when the kernel runs): the frame of each stream's first new one; below 0 the
+        stream is idle, its caches stay and its ``out`` is 0.  Frame ``f`` lies in slot ``f`` if ``f < sinks``, else
+        in ``sinks + (f - sinks) % (slots - sinks)``.  A query at frame ``p`` sees the frames ``p - left .. p`` and the
+        first ``sinks``; the caches must have at least ``sinks + left + N`` slots, and hold what was written for the
+        frames that are seen.  Caches: rows dense and whole 16 bytes apart, no two in one place, none of them ``k`` or
+        ``v``.  Bias and scale as in :meth:`local_attention_forward`."""
+        _req(k.dim() == 4 and q.dim() == 4 and k.shape[1] == q.shape[1], "q, k and v must have as many new frames")
+        _, _, _, scale = self._attention_check(q, k, v, None, None, scale, 0.0, None)
+        b, n, h, d = q.shape
+        hk = k.shape[2]
+        _req(0 <= left <= 2**28 and 0 <= sinks <= 2**28, "left and sinks must lie in [0, 2**28]")
+        strides = []
+        for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+            _req(t.device == q.device and t.dtype == q.dtype and t.dim() == 4 and t.shape[0] == b and t.shape[2:] == k.shape[2:],
+                 f"{name} must have shape [B, slots, Hk, D] and q's dtype and device")
+            strides.append(self._cache_strides(t, name))
+        slots = k_cache.shape[1]
+        _req(v_cache.shape == k_cache.shape, "k_cache and v_cache must have one shape")
+        _req(slots - sinks >= left + n, "the caches must have at least sinks + left + N slots")
+        _req(positions.device == q.device and positions.dtype == torch.int32 and positions.shape == (b,),
+             "positions must be an int32 tensor of shape [B] on q's device")
+        bias = self._bias_check(q, bias, bias_plan, scale)
+        code = dtype_code(q.dtype)
+        (q, qs), (k, ks), (v, vs) = self._attention_operand(q), self._attention_operand(k), self._attention_operand(v)
+        positions = positions.contiguous()
+        out = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
+        with _DeviceGuard(q.device):
+            size = self._lib.pmsst_local_attention_step_workspace_size(b, n, h, hk, d, left, sinks, code)
+            ws = _workspace(size, q.device) if size else None
+            rc = self._lib.pmsst_local_attention_step(
+                _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(k_cache), strides[0], _ptr(v_cache), strides[1],
+                _ptr(positions), left, sinks, *self._bias_args(bias, bias_plan), _ptr(out), b, n, slots, h, hk, d, scale,
+                code, _ptr(ws), size, _stream(q.device),
+            )
+        check(rc, "pmsst_local_attention_step")
+        return out
+
+    def _cache_strides(self, t, name):
+        """A cache's strides: it is written in place, so its rows must lie apart and cannot be copied."""
+        unit = 16 // t.element_size()
+        st = self._attention_strides(t)
+        apart, extent = True, t.shape[3]
+        for size, stride in sorted(((s, p) for s, p in zip(t.shape[:3], st) if s > 1), key=lambda x: x[1]):
+            apart &= stride >= extent
+            extent = stride * (size - 1) + extent
+        _req(t.stride(3) == 1 and apart and not any(s % unit for s in st) and t.data_ptr() % 16 == 0,
+             f"{name} must have dense rows, whole 16 bytes apart, and no two in one place")
+        return (ctypes.c_int64 * 3)(*st)
 
     # ------------------------------------------------------------------ dropout
 

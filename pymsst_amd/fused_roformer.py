@@ -1553,6 +1553,31 @@ class _FusedCrossAttention(torch.autograd.Function):
         return (*grads, None, None, None, None, None, None)
 
 
+class _FusedLocalAttention(torch.autograd.Function):
+    """Attention within a window, with sinks and a learned bias (this build's addition); saves the output
+    and the rows' log-sums, no weights and no matrix of biases."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bias, bias_plan, left, right, sinks, key_mask, key_lengths, query_starts, scale, extension):
+        kw = dict(left=left, right=right, sinks=sinks, key_mask=key_mask, key_lengths=key_lengths, query_starts=query_starts,
+                  scale=scale, bias=bias, bias_plan=bias_plan)
+        if not any(ctx.needs_input_grad[:4]):
+            return extension.local_attention_forward(q, k, v, **kw)[0]
+        out, lse = extension.local_attention_forward(q, k, v, need_lse=True, **kw)
+        ctx.save_for_backward(q, k, v, bias, out, lse, key_mask, key_lengths, query_starts)
+        ctx.kw = dict(left=left, right=right, sinks=sinks, scale=scale, bias_plan=bias_plan)
+        ctx.extension = extension
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, bias, out, lse, key_mask, key_lengths, query_starts = ctx.saved_tensors
+        grads = ctx.extension.local_attention_backward(grad_out, q, k, v, out, lse, bias=bias, key_mask=key_mask,
+                                                       key_lengths=key_lengths, query_starts=query_starts, **ctx.kw)
+        return (*grads[:3], grads[3] if bias is not None else None, *[None] * 9)
+
+
 class _FusedDropout(torch.autograd.Function):
     """``dropout(act(x)) + residual`` (this build's addition); saves the seed and offset, and ``x`` for a GELU."""
 
@@ -1587,6 +1612,17 @@ def cross_attention(q, k, v, *, key_mask=None, key_lengths=None, scale=None, dro
     if dropout_p > 0.0 and rng is None:
         rng = draw_rng(q.device)
     return _FusedCrossAttention.apply(q, k, v, key_mask, key_lengths, scale, float(dropout_p), rng, ext)
+
+
+def local_attention(q, k, v, *, left=None, right=None, sinks: int = 0, bias=None, bias_plan=None, key_mask=None,
+                    key_lengths=None, query_starts=None, scale=None, extension=None) -> torch.Tensor:
+    """Differentiable attention of ``q[B, N, H, D]`` over the frames ``k`` / ``v[B, M, Hk, D]`` within a window of ``left``
+    frames back and ``right`` ahead and the first ``sinks`` frames, with a learned ``bias[num_buckets, H]`` by distance
+    (its gradient among the others'; ``bias_plan`` of ``HipFusedExtension.relative_bias_plan``).  See
+    ``HipFusedExtension.local_attention_forward`` for the rule, masks, shared heads and layouts."""
+    ext = extension if extension is not None else load_fused_band_split_extension()
+    return _FusedLocalAttention.apply(q, k, v, bias, bias_plan, left, right, sinks, key_mask, key_lengths, query_starts,
+                                      scale, ext)
 
 
 def dropout(x, p: float, *, activation=None, residual=None, rng=None, extension=None) -> torch.Tensor:
@@ -1761,6 +1797,7 @@ __all__ = [
     "apply_roformer_fused_training_backend",
     "apply_runtime_preset",
     "cross_attention",
+    "local_attention",
     "draw_rng",
     "dropout",
     "load_fused_band_split_extension",
