@@ -473,10 +473,10 @@ int pmsst_local_attention_forward(const void* q, const int64_t* q_strides, const
                                   double scale, int dtype, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
-/* Bytes of workspace of the backward on the current device (buckets: 0 without a bias). */
+/* Bytes of workspace of the backward on the current device (max_distance: -1 without a bias). */
 size_t pmsst_local_attention_backward_workspace_size(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
                                                      int64_t kv_heads, int64_t head_dim, int64_t left, int64_t right,
-                                                     int64_t sinks, int has_starts, int64_t buckets, int dtype);
+                                                     int64_t sinks, int has_starts, int64_t max_distance, int dtype);
 /* Gradients of the forward (same masks, limits, bias and scale) from its dense out and its lse: grad_q[batch, queries,
  * heads, head_dim], grad_k and grad_v[batch, keys, kv_heads, head_dim], and with a bias grad_bias[buckets, heads] in
  * the bias's dtype, all dense and fully written (exact zeros in grad_q and grad_k where a query sees one frame).

@@ -35,9 +35,7 @@ struct Window {
 struct BiasArgs {
   const void* table;         // [buckets, H], NULL: no bias
   const int32_t* bucket_of;  // [2 distance + 1]: the bucket of distance i - distance
-  const int32_t* order;      // backward: [2 distance + 1], the indexes of bucket_of by bucket,
-  const int32_t* first;      // and [buckets + 1], where each bucket's begin
-  int32_t buckets, distance;
+  int32_t buckets, distance;  // `distance` is cut to what a call reaches, and bucket_of moved along
   int32_t f32;               // the table's type: fp32, or that of q
 };
 
@@ -99,25 +97,39 @@ __device__ __forceinline__ Sees sees(const Window& w, int p0, int key0, int coun
   return Sees::kSome;
 }
 
-// An entry of the bias table as the kernels take it, in units of 1 / unit.
-__device__ __forceinline__ float bias_value(const BiasArgs& t, int dtype, int heads, int head, int distance, float unit) {
-  int bucket = t.bucket_of[distance + t.distance];
+// A bucket's entry of the bias.
+__device__ __forceinline__ float bias_entry(const BiasArgs& t, int dtype, int heads, int head, int bucket) {
   bucket = bucket < 0 ? 0 : bucket >= t.buckets ? t.buckets - 1 : bucket;
   const int64_t at = static_cast<int64_t>(bucket) * heads + head;
-  const float v = t.f32              ? static_cast<const float*>(t.table)[at]
-                  : dtype == PMSST_F16 ? static_cast<float>(static_cast<const f16*>(t.table)[at])
-                                       : static_cast<float>(static_cast<const bf16*>(t.table)[at]);
+  return t.f32                ? static_cast<const float*>(t.table)[at]
+         : dtype == PMSST_F16 ? static_cast<float>(static_cast<const f16*>(t.table)[at])
+                              : static_cast<float>(static_cast<const bf16*>(t.table)[at]);
+}
+// As the kernels take it, in units of 1 / unit.
+__device__ __forceinline__ float bias_value(float v, float unit) {
   if (v <= kBiasHides) return -kInf;
   return (v > kBiasMost ? kBiasMost : v < -kBiasMost ? -kBiasMost : v) * unit;  // NaN stays
 }
 
-// Fills `table` by distance, kPad + distance entries on either side of 0 (falling distances if DOWN).
+// Fills `table` by distance, kPad + distance entries on either side of 0 (falling distances if DOWN).  Two loads, one
+// waiting for the other, make an entry: four are on their way at once.
 template <typename T, bool DOWN>
 __device__ __forceinline__ void fill_bias(float* table, const BiasArgs& t, int heads, int head, float unit, int threads) {
-  for (int i = threadIdx.x; i < 2 * t.distance + 1 + 2 * kPad; i += threads) {
-    int d = i - kPad - t.distance;
-    d = d < -t.distance ? -t.distance : d > t.distance ? t.distance : d;
-    table[i] = bias_value(t, dtype_code<T>(), heads, head, DOWN ? -d : d, unit);
+  const int entries = 2 * t.distance + 1 + 2 * kPad;
+  for (int base = threadIdx.x; base < entries; base += 4 * threads) {
+    int bucket[4];
+    float value[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = min(max(min(base + j * threads, entries - 1) - kPad - t.distance, -t.distance), t.distance);
+      bucket[j] = t.bucket_of[t.distance + (DOWN ? -d : d)];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) value[j] = bias_entry(t, dtype_code<T>(), heads, head, bucket[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (base + j * threads < entries) table[base + j * threads] = bias_value(value[j], unit);
+    }
   }
 }
 
@@ -156,28 +168,31 @@ __device__ __forceinline__ void skip(TileT& t, int64_t bytes) {
   for (int i = 0; i < TileT::CH; ++i) t.ptr[i] += bytes;
 }
 
-// The tiles of BQ queries that see any of the frames [key0, key_end) of a block, by the window (slot 0), or what a block
-// of the sinks' later queries takes: those past the window, of every head in turn, `chunk_tiles` of them a slot.
+// The tiles of BQ queries that a block with the frames [key0, key_end) passes over: of those that see any by the window,
+// of every head in turn, the slot's share (slots below `splits`), or of those past the window, that see sinks alone,
+// `chunk_tiles` a slot (the others, `chunks` in number).
 struct RowTiles {
   int first, tiles;  // of a head
   int from, to;      // of the tiles of all heads in turn
 };
 template <int BQ>
 __device__ __forceinline__ RowTiles rows_of(const Window& w, int start, int queries, int group, int key0, int key_end, int slot,
-                                            int slots, int chunk_tiles) {
+                                            int splits, int chunks, int chunk_tiles) {
   const int all = (queries + BQ - 1) / BQ;
   const int low = w.right < 0 ? 0 : max(0, key0 - w.right - start);
   const int high = w.left < 0 ? queries : min(queries, key_end + w.left - start);
   RowTiles r;
   r.first = min(low / BQ, all);
   r.tiles = high <= low ? 0 : max(0, (high + BQ - 1) / BQ - r.first);
-  r.from = 0;
-  r.to = r.tiles * group;
-  if (slot > 0) {
+  if (slot < splits) {
+    const int64_t total = static_cast<int64_t>(r.tiles) * group;
+    r.from = static_cast<int>(total * slot / splits);
+    r.to = static_cast<int>(total * (slot + 1) / splits);
+  } else {
     r.first += r.tiles;
     r.tiles = all - r.first;
-    r.from = min((slot - 1) * chunk_tiles, r.tiles * group);
-    r.to = slot == slots ? r.tiles * group : min(r.from + chunk_tiles, r.tiles * group);
+    r.from = min((slot - splits) * chunk_tiles, r.tiles * group);
+    r.to = slot + 1 == splits + chunks ? r.tiles * group : min(r.from + chunk_tiles, r.tiles * group);
   }
   return r;
 }
@@ -188,7 +203,14 @@ struct LocalArgs {
   Shape s;
   Window w;
   BiasArgs bias;
+  int32_t cut;  // the distances cut off on either side of bucket_of
 };
+// The largest distance that a pair can have, up to `distance`.
+inline int64_t reach_of(const Shape& s, const Window& w, int64_t distance) {
+  if (w.starts == nullptr) distance = std::min<int64_t>(distance, std::max<int64_t>(std::max(s.N, s.M) - 1, 0));
+  if (w.left >= 0 && w.right >= 0 && w.sinks == 0) distance = std::min<int64_t>(distance, std::max(w.left, w.right));
+  return distance;
+}
 int make_local(const char* what, int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t head_dim,
                int64_t left, int64_t right, int64_t sinks, const int32_t* starts, const void* bias, int bias_dtype,
                const int32_t* bucket_of, int64_t buckets, int64_t distance, double scale, int dtype, LocalArgs& out);

@@ -328,13 +328,16 @@ int make_local(const char* what, int64_t batch, int64_t queries, int64_t keys, i
   if (starts == nullptr && right >= keys - 1) right = -1;
   out.w = {static_cast<int32_t>(left), static_cast<int32_t>(right), left < 0 ? 0 : static_cast<int32_t>(sinks), starts};
   out.bias = {};
+  out.cut = 0;
   if (bias == nullptr) return PMSST_OK;
   PMSST_REQUIRE(bucket_of != nullptr, "%s: null pointer (bucket_of)", what);
   PMSST_REQUIRE(buckets >= 1 && buckets <= kMaxBuckets, "%s: the bias has 1 to %d buckets", what, kMaxBuckets);
   PMSST_REQUIRE(distance >= 0 && distance <= kMaxDistance, "%s: the bias's largest distance must lie in [0, %d]", what, kMaxDistance);
   PMSST_REQUIRE(scale >= 0x1p-20 && scale <= 0x1p20, "%s: with a bias, scale must lie in [2^-20, 2^20]", what);
   if (bias_dtype != PMSST_F32 && bias_dtype != dtype) return fail(PMSST_EDTYPE, "%s: the bias must be fp32 or of q's dtype", what);
-  out.bias = {bias, bucket_of, nullptr, nullptr, static_cast<int32_t>(buckets), static_cast<int32_t>(distance), bias_dtype == PMSST_F32};
+  const int64_t reach = reach_of(out.s, out.w, distance);
+  out.cut = static_cast<int32_t>(distance - reach);
+  out.bias = {bias, bucket_of + out.cut, static_cast<int32_t>(buckets), static_cast<int32_t>(reach), bias_dtype == PMSST_F32};
   return PMSST_OK;
 }
 

@@ -8,14 +8,16 @@
 //
 // The first frames (sinks) are seen by every later query: the block of their keys would pass over all rows while others
 // pass over a window's.  Their rows past the window go to blocks of their own, as many tiles each as an ordinary block
-// has; the sums meet in fp32 in the workspace and a third kernel adds them.
+// has; the sums meet in fp32 in the workspace and a third kernel adds them.  So do the sums of blocks that are split over
+// their queries, where there are few of them.
 //
 // The bias's gradient sums dS along diagonals, in local_dkv_kernel.  A wave's 32 x 32 tile holds 63 of them.  With one
-// frame a lane and 8 queries in a row in its registers, adding the registers one after the other while the sum moves on by
-// a lane in between brings every diagonal into one lane: 16 additions with a lane shift in the same instruction, for
-// either half of the wave.  39 sums of 8 queries then go to the wave's own bins in LDS, one a distance.  Tiles beyond the
-// table's distances add up in registers.  The bins of a block are summed by bucket, in a fixed order, and a last kernel
-// adds the blocks.
+// frame a lane and queries in a row in its registers, adding the registers one after the other while the sum moves on by a
+// lane in between brings every diagonal into one lane: 16 additions with a lane shift in the same instruction, for either
+// half of the wave.  The sums then go to the wave's own bins in LDS, one a distance.  Tiles beyond the table's distances
+// add up in registers.  Every block leaves its bins in the workspace, and a last kernel adds the blocks and the distances
+// of a bucket, in a fixed order.  (With the bins summed by bucket in every block, that sum took half of the kernel's time:
+// 16 x 2760 queries, window of 1024, 320 buckets, 1074 us against 552.)
 #include "attention_bwd.h"
 #include "local_attention.h"
 
@@ -30,18 +32,21 @@ struct BwdArgs {
   KeyMask km;
   Window w;
   BiasArgs bias;
+  const int32_t *order, *first;  // bucket_of's indexes by bucket, and where each bucket's begin
+  int32_t cut;                   // indexes cut off on either side of the bias's table
   const float* lse;  // [B, H, N]
   void *dq, *dk, *dv, *dbias;
-  // [B * H, rows_pad]: -lse in log2 units (- inf: no weight), D, and 0 where a query sees one frame alone (else 1)
-  float *base, *delta, *alive;
+  float *base, *delta;  // [B * H, rows_pad]: -lse in log2 units (- inf: no weight), D
+  uint32_t* lone;       // [B * H, rows_pad / 32]: a bit for each query that sees one frame alone
   int32_t rows_pad;     // N rounded up to 64
   float *vmax, *l1;     // fp16: [pairs, kParts] maxima of |V| over the seen frames and of |dO row|_1
-  float *part_k, *part_v;  // [1 + chunks, pairs, sink_keys, D], NULL: no sinks
-  float* part_bias;     // [H, B * blocks of a pair in local_dkv_kernel, buckets]
+  float *part_k, *part_v;  // [splits + chunks, pairs, part_keys, D]: of the keys that several blocks share
+  float* part_bias;     // [H, B * blocks of a pair in local_dkv_kernel, span]: sums by falling distance
+  float* sum_bias;      // [H, groups of kSumRows of those, span]
   Shape s;
   Grid grid;
-  uint32_t row_tiles, key_tiles, sink_tiles, chunks;
-  int32_t chunk_tiles, sink_keys;
+  uint32_t row_tiles, key_tiles, splits, sink_tiles, chunks;
+  int32_t chunk_tiles, sink_keys, part_keys;
   bool late_first;
   float scale, scale_log2, bias_unit;
   struct { float factor; } drop;  // what attn_bound_kernel's bound is multiplied by: no dropout here
@@ -57,6 +62,7 @@ __device__ __forceinline__ int pair_exponent(const BwdArgs& a, uint32_t pair) {
 }
 
 // ---------------------------------------------------------------- diagonals
+constexpr int kBinPad = 16;  // places on either side of a wave's bins that add_diagonals adds zeros to
 
 // The value of the lane before (after) this one; 0 enters at the wave's end.
 __device__ __forceinline__ float from_before(float x) {
@@ -68,27 +74,36 @@ __device__ __forceinline__ float from_after(float x) {
 __device__ __forceinline__ float keep_bits(float x, uint32_t m) {
   return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & m);
 }
-// Adds to a bin of this wave alone: one instruction's lanes have bins of their own, and a wave's come in order.
-__device__ __forceinline__ void add_bin(float* bin, float x) {
-  __hip_atomic_fetch_add(bin, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-}
 
-// Adds the diagonals of x (lane l: frame l % 32, queries reg_key(i) + 8 (l / 32)) to bins[query - frame].  A lower lane's
-// query c at frame r ends in lane r + 7 - c: it moves up with each query after it; the 7 places past lane 31 are
-// free, as the upper half's values are left out.  The upper half moves down likewise.
+// Adds the diagonals of x (lane l: frame l % 32, queries reg_key(i) + 8 (l / 32)) to bins[query - frame], this wave's alone.
+// The halves first exchange 8 registers, so that each holds 16 queries in a row.  A lower lane's query c at frame r
+// then ends in lane r + 15 - c: it moves up with each query after it, and the 15 places past lane 31 are free, as the
+// upper half's values are left out.  The upper half moves down likewise.
 __device__ __forceinline__ void add_diagonals(float* bins, const f32x16_t& x, int lane) {
-  const uint32_t low = lane < 32 ? ~0u : 0u;
+  uint32_t low = lane < 32 ? ~0u : 0u;
+  asm volatile("" : "+v"(low));  // a register's mask, not one of the few scalar pairs
+  float y[16];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    float up = keep_bits(x[8 * s], low), down = keep_bits(x[8 * s + 7], ~low);
-#pragma unroll
-    for (int c = 1; c < 8; ++c) {
-      up = from_before(up) + keep_bits(x[8 * s + c], low);
-      down = from_after(down) + keep_bits(x[8 * s + 7 - c], ~low);
-    }
-    if (lane < 39) add_bin(bins + (16 * s + 7 - lane), up);
-    if (lane >= 25) add_bin(bins + (16 * s + 40 - lane), down);
+  for (int c = 0; c < 8; ++c) {
+    const float near = x[c], far = x[8 + c];
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, near), __builtin_bit_cast(uint32_t, far), false, false);
+    const uint32_t first = r[0], second = r[1];  // queries c and 16 + c of the halves, 8 + c and 24 + c
+    y[c] = __builtin_bit_cast(float, first);
+    y[8 + c] = __builtin_bit_cast(float, second);
   }
+  float up = keep_bits(y[0], low), down = keep_bits(y[15], ~low);
+#pragma unroll
+  for (int c = 1; c < 16; ++c) {
+    up = from_before(up) + keep_bits(y[c], low);
+    down = from_after(down) + keep_bits(y[15 - c], ~low);
+  }
+  // Every lane adds; those beyond the diagonals (from 47 on, below 17) add 0, up to 17 places past them.  A lane's places in
+  // the two additions differ, and the compiler may not read the second before it writes the first: they are other lanes'.
+  asm volatile("" ::: "memory");
+  bins[15 - lane] += up;
+  asm volatile("" ::: "memory");
+  bins[48 - lane] += down;
+  asm volatile("" ::: "memory");
 }
 
 // ---------------------------------------------------------------- dQ
@@ -172,8 +187,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
       if (!__any(row_ok && found < 2)) break;
     }
   }
+  const uint32_t lone = static_cast<uint32_t>(__ballot(found == 1));
   const float alive = found == 1 ? 0.f : 1.f;
-  const bool any_lone = __any(found == 1);
 
   const float row_base = base;
   int e = 0;
@@ -272,7 +287,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
       for (int r = 0; r < 16; ++r) {
         p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base)) * (dp[r] - delta);
       }
-      if (any_lone) {
+      if (lone != 0) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] *= alive;
       }
@@ -300,32 +315,53 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
     const int64_t at = bh * a.rows_pad + n;
     a.base[at] = row_base + (kHalf ? 14.f : 0.f);
     a.delta[at] = delta;
-    a.alive[at] = alive;
+    if (lane == 0) a.lone[at / 32] = lone;
   }
 }
 
-// dbias[bucket, head] = the sum of the blocks' parts, in a fixed order; 32 buckets a block.
-template <typename B>
-__global__ __launch_bounds__(1024) void local_bias_sum_kernel(const float* parts, B* out, int64_t blocks, int buckets, int heads) {
-  __shared__ float red[32][33];
-  const int c = static_cast<int>(blockIdx.y) * 32 + static_cast<int>(threadIdx.x & 31), y = threadIdx.x >> 5;
+// The blocks' bins become the buckets' sums in two steps, each in a fixed order: `rows` blocks' at a time by distance,
+// then those sums by bucket.
+constexpr int kSumRows = 256;
+__global__ __launch_bounds__(1024) void local_bins_sum_kernel(const float* parts, float* sums, int64_t blocks, int span) {
+  __shared__ float red[16][64];
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6, at = static_cast<int>(blockIdx.y) * 64 + x;
+  const int64_t head = blockIdx.x, from = int64_t{blockIdx.z} * kSumRows, to = from + kSumRows < blocks ? from + kSumRows : blocks;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < buckets) {
-    const float* part = parts + static_cast<int64_t>(blockIdx.x) * blocks * buckets + c;
-    int64_t i = y;
-    for (; i + 96 < blocks; i += 128) {
+  if (at < span) {
+    const float* part = parts + head * blocks * span + at;
+    int64_t k = from + y;
+    for (; k + 48 < to; k += 64) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] += part[(i + 32 * j) * buckets];
+      for (int j = 0; j < 4; ++j) sum[j] += part[(k + 16 * j) * span];
     }
-    for (; i < blocks; i += 32) sum[0] += part[i * buckets];
+    for (; k < to; k += 16) sum[0] += part[k * span];
   }
-  red[y][threadIdx.x & 31] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  red[y][x] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
   __syncthreads();
-  if (threadIdx.x < 32 && c < buckets) {
-    float t = 0.f;
-    for (int j = 0; j < 32; ++j) t += red[j][threadIdx.x];
-    out[static_cast<int64_t>(c) * heads + blockIdx.x] = from_f32<B>(t);
+  if (y != 0 || at >= span) return;
+  float t = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) t += red[j][x];
+  sums[(head * gridDim.z + blockIdx.z) * span + at] = t;
+}
+
+// dbias[bucket, head]; a wave a bucket.  `order` and `first` are by the whole table's indexes, of which `cut` lie off
+// either end; the sums are by falling distance.
+template <typename B>
+__global__ __launch_bounds__(256) void local_bias_sum_kernel(const float* sums, B* out, const int32_t* order, const int32_t* first,
+                                                             int parts, int span, int cut, int buckets, int heads) {
+  const int x = threadIdx.x & 63, c = static_cast<int>(blockIdx.y) * 4 + static_cast<int>(threadIdx.x >> 6), all = span + 2 * cut;
+  if (c >= buckets) return;
+  const float* from = sums + static_cast<int64_t>(blockIdx.x) * parts * span;
+  const int begin = max(0, first[c]), end = min(all, first[c + 1]);
+  float sum = 0.f;
+  for (int i = begin + x; i < end; i += 64) {
+    const int at = span - 1 - (order[i] - cut);
+    if (at < 0 || at >= span) continue;
+    for (int z = 0; z < parts; ++z) sum += from[static_cast<int64_t>(z) * span + at];
   }
+  sum = group_sum(sum, kWave);
+  if (x == 0) out[static_cast<int64_t>(c) * heads + blockIdx.x] = from_f32<B>(sum);
 }
 
 // ---------------------------------------------------------------- dK, dV
@@ -340,20 +376,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
   constexpr int BQ = local_tile<T, DP>(), SUBS = BQ / 32;
   constexpr bool kHalf = std::is_same<T, f16>::value;
   __shared__ __attribute__((aligned(16))) char lds[kStages][2][BQ * DB];
-  __shared__ __attribute__((aligned(16))) float stat[kStages][3][64];  // -lse (log2 units), D, alive
+  __shared__ __attribute__((aligned(16))) float stat[kStages][2][64];  // -lse (log2 units), D
   extern __shared__ float table[];  // the bias by falling distance, then each wave's bins
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t pair, sub_block;
   if (!locate(a.grid, pair, sub_block)) return;
   const Shape& s = a.s;
   // the ordinary blocks, then those of the sinks' later rows
-  uint32_t key_tile = sub_block, slot = 0;
-  if (sub_block >= a.key_tiles) {
-    const uint32_t i = sub_block - a.key_tiles;
-    slot = i / a.sink_tiles;
-    key_tile = i - slot * a.sink_tiles;
-    ++slot;
-  }
+  const uint32_t ordinary = a.key_tiles * a.splits;
+  const uint32_t of = sub_block < ordinary ? a.key_tiles : a.sink_tiles, i = sub_block < ordinary ? sub_block : sub_block - ordinary;
+  const uint32_t key_tile = i % of, slot = i / of + (sub_block < ordinary ? 0u : a.splits);
   const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
   const int d_units = s.D * static_cast<int>(sizeof(T)) / 16;
   const int count = key_count(a.km, b, s.M);
@@ -365,18 +397,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
   const bool any_unseen = __any(!seen);
 
   const RowTiles rows = rows_of<BQ>(a.w, start, s.N, s.G, block_key0, block_end, static_cast<int>(slot),
-                                    static_cast<int>(a.chunks), a.chunk_tiles);
+                                    static_cast<int>(a.splits), static_cast<int>(a.chunks), a.chunk_tiles);
   const int first = rows.first, tiles = rows.tiles, from = rows.from, to = block_key0 < count ? rows.to : rows.from;
   float* part_bias = nullptr;  // of the pair's first head; further heads lie part_step apart
   int64_t part_step = 0;
   if constexpr (BIAS) {
-    part_step = static_cast<int64_t>(s.B) * a.grid.per * a.bias.buckets;
-    part_bias = a.part_bias + hk * s.G * part_step + (static_cast<int64_t>(b) * a.grid.per + sub_block) * a.bias.buckets;
+    const int span = 2 * a.bias.distance + 1;
+    part_step = static_cast<int64_t>(s.B) * a.grid.per * span;
+    part_bias = a.part_bias + hk * s.G * part_step + (static_cast<int64_t>(b) * a.grid.per + sub_block) * span;
     // the heads that have no tile here
     const int g_from = from < to ? from / tiles : 0, g_to = from < to ? (to - 1) / tiles + 1 : 0;
     for (int g = 0; g < s.G; ++g) {
       if (g >= g_from && g < g_to) continue;
-      for (int c = threadIdx.x; c < a.bias.buckets; c += 64 * NW) part_bias[g * part_step + c] = 0.f;
+      for (int i = threadIdx.x; i < span; i += 64 * NW) part_bias[g * part_step + i] = 0.f;
     }
   }
 
@@ -403,16 +436,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
     auto g_at = [&](int i) { return i * a.gs.n; };
     int next_g = from / tiles, next_t = first + from - next_g * tiles;  // the tile that is fetched next
     const T *q_head = nullptr, *g_head = nullptr;
+    // waves 0 and 1 also move a tile's 64 (32) pairs of statistics, 4 bytes a lane
     const float* stat_head = nullptr;
+    const uint32_t* lone_head = nullptr;
     auto begin_head = [&] {
       const int head = hk * s.G + next_g;
       q_head = qb + head * a.qs.h;
       g_head = gb + head * a.gs.h;
       qt.start(q_head, next_t * BQ, d_units, q_at);
       gt.start(g_head, next_t * BQ, d_units, g_at);
-      stat_head = a.base + (static_cast<int64_t>(b) * s.H + head) * a.rows_pad + lane;
+      const int64_t at = (static_cast<int64_t>(b) * s.H + head) * a.rows_pad;
+      stat_head = (wave == 0 ? a.base : a.delta) + at + lane;
+      lone_head = a.lone + at / 32;
     };
-    const int64_t stat_step = static_cast<int64_t>(s.B) * s.H * a.rows_pad;  // base, delta and alive follow each other
+    uint64_t lone_now = 0, lone_next = 0;  // the tile's queries that see one frame alone
     auto fetch = [&](int stage) {
       const int row0 = next_t * BQ;
       if (DB < 512 && row0 + BQ <= s.N) {
@@ -422,13 +459,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
         qt.fetch_cut(lds[stage][0], q_head, row0, s.N, d_units, q_at);
         gt.fetch_cut(lds[stage][1], g_head, row0, s.N, d_units, g_at, reinterpret_cast<const T*>(zero_row));
       }
-#pragma unroll
-      for (int j = 0; j < 3; j += NW < 3 ? NW : 3) {
-        const int which = j + wave;
-        if (which < 3 && (BQ == 64 || lane < BQ)) {
-          dma4_m0(stat_head + which * stat_step + row0, __builtin_amdgcn_readfirstlane(lds_addr(stat[stage][0]) + 256 * which));
-        }
-      }
+      if (wave < 2 && (BQ == 64 || lane < BQ)) dma4_m0(stat_head + row0, __builtin_amdgcn_readfirstlane(lds_addr(stat[stage]) + 256 * wave));
+      lone_next = lone_head[row0 / 32];
+      if constexpr (BQ == 64) lone_next |= static_cast<uint64_t>(lone_head[row0 / 32 + 1]) << 32;
       if (++next_t == first + tiles) {
         next_t = first;
         ++next_g;
@@ -451,7 +484,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
       far_high = table[0];
       far_low = table[entries - 1];
     };
-    // a head's bins, summed by bucket
+    // a head's bins, over the waves
     auto end_table = [&](int g) {
       // past the table's ends, and the far tiles' sums: into the end bins
       const float above = group_sum(sum_high + bins[lane], kWave);
@@ -461,22 +494,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
         bins[entries - 1 - kPad] += under;
       }
       __syncthreads();
-      const int span = 2 * a.bias.distance + 1;
       const float unscale = kHalf ? v_scale * dp_unscale : 1.f;
-      for (int c = threadIdx.x; c < a.bias.buckets; c += 64 * NW) {
-        const int begin = max(0, a.bias.first[c]), end = min(span, a.bias.first[c + 1]);
+      for (int i = threadIdx.x; i < 2 * a.bias.distance + 1; i += 64 * NW) {
         float sum = 0.f;
-        for (int i = begin; i < end; ++i) {
-          const float* bin = table + 2 * entries - 1 - kPad - min(max(a.bias.order[i], 0), span - 1);
 #pragma unroll
-          for (int w = 0; w < NW; ++w) sum += bin[w * entries];
-        }
-        part_bias[g * part_step + c] = sum * unscale;
+        for (int w = 0; w < NW; ++w) sum += table[entries + kBinPad + w * (entries + 2 * kBinPad) + kPad + i];
+        part_bias[g * part_step + i] = sum * unscale;
       }
       __syncthreads();  // before the bins are cleared
     };
     if constexpr (BIAS) {
-      bins = table + entries * (1 + wave);
+      bins = table + entries + kBinPad + wave * (entries + 2 * kBinPad);
       begin_table(g_now);
       lane_table = table + (a.bias.distance + kPad + 8 * h - ki);
     }
@@ -498,8 +526,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
           begin_table(g_now);
         }
       }
-      const float* alive = stat[stage][2];
-      const uint64_t lone = __ballot((BQ == 64 || lane < BQ) && alive[BQ == 64 ? lane : lane & (BQ - 1)] == 0.f);
+      lone_now = lone_next;
       if (i + 1 < to) {
         if (next_t == first) begin_head();
         fetch(stage ^ 1);
@@ -548,10 +575,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
           p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base[row]));
           ds[r] = p[r] * fmaf(ds[r], dp_scale, -delta[row]);
         }
-        const uint32_t sub_lone = static_cast<uint32_t>(lone >> (32 * u));
+        const uint32_t sub_lone = static_cast<uint32_t>(lone_now >> (32 * u));
         if (sub_lone != 0) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) ds[r] *= alive[32 * u + reg_key(r) + 8 * h];
+          for (int r = 0; r < 16; ++r) ds[r] = where_bit(sub_lone >> (8 * h), reg_key(r), ds[r] * 0.f, ds[r]);
         }
         if constexpr (BIAS) {
           if (near) {
@@ -581,8 +608,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
       dv[dt] = f32x16_t{};
     }
   }
-  if (key_tile < a.sink_tiles) {
-    const int64_t at = ((static_cast<int64_t>(slot) * a.grid.pairs + pair) * a.sink_keys + ki) * s.D;
+  if (a.splits > 1 || key_tile < a.sink_tiles) {
+    const int64_t at = ((static_cast<int64_t>(slot) * a.grid.pairs + pair) * a.part_keys + ki) * s.D;
     store_cols_f32<T, DP>(a.part_k + at, dk, k_scale, s.D, h);
     store_cols_f32<T, DP>(a.part_v + at, dv, v_scale, s.D, h);
   } else {
@@ -592,9 +619,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
   }
 }
 
-// The sinks' keys: dk, dv = the sum of their blocks' parts.  A thread takes 4 columns; the grid's y is the gradient.
+// dk, dv of the keys that several blocks share = the sum of their parts.  A thread takes 4 columns; the grid's y is the
+// gradient.
 template <typename T>
-__global__ __launch_bounds__(256) void local_sink_sum_kernel(BwdArgs a, int keys) {
+__global__ __launch_bounds__(256) void local_parts_sum_kernel(BwdArgs a, int keys) {
   const Shape& s = a.s;
   const float* part = blockIdx.y != 0 ? a.part_v : a.part_k;
   T* out = static_cast<T*>(blockIdx.y != 0 ? a.dv : a.dk);
@@ -602,10 +630,11 @@ __global__ __launch_bounds__(256) void local_sink_sum_kernel(BwdArgs a, int keys
   if (i >= a.grid.pairs * keys * quads) return;
   const int64_t row = i / quads, quad = i - row * quads, pair = row / keys, key = row - pair * keys;
   const int64_t b = pair / s.Hk, hk = pair - b * s.Hk;
+  const uint32_t slots = a.splits + (key < a.sink_keys ? a.chunks : 0);
   float o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t c = 0; c <= a.chunks; ++c) {
+  for (uint32_t c = 0; c < slots; ++c) {
     float x[4];
-    load_pack<float, 4>(part + (((static_cast<int64_t>(c) * a.grid.pairs + pair) * a.sink_keys + key) * quads + quad) * 4, x);
+    load_pack<float, 4>(part + (((static_cast<int64_t>(c) * a.grid.pairs + pair) * a.part_keys + key) * quads + quad) * 4, x);
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] += x[j];
   }
@@ -616,42 +645,53 @@ __global__ __launch_bounds__(256) void local_sink_sum_kernel(BwdArgs a, int keys
 
 struct BwdPlan {
   int nw_q, nw_k;
-  int64_t row_tiles, key_tiles, sink_tiles, chunks, chunk_tiles;
+  int64_t row_tiles, key_tiles, splits, sink_tiles, chunks, chunk_tiles;
+  int64_t blocks() const { return key_tiles * splits + sink_tiles * chunks; }  // of a pair in local_dkv_kernel
+  int64_t sink_keys() const { return sink_tiles * 32 * nw_k; }
+  int64_t part_keys() const { return splits > 1 ? key_tiles * 32 * nw_k : sink_keys(); }
 };
 
+// The frames' blocks are split over their queries where they are
+// fewer than two a CU, into shares of at least two tiles.
 BwdPlan plan_backward(const Shape& s, const Window& w, int dtype) {
   const bool wide = padded_dim(s.D) * static_cast<int>(dtype_size(dtype)) == 512;
-  const int64_t bq = wide ? 32 : 64;
+  const int64_t bq = wide ? 32 : 64, want = 2 * num_cus(), pairs = int64_t{s.B} * s.Hk;
   BwdPlan p{};
   p.nw_q = s.N <= 64 && !wide ? 2 : 4;
   p.nw_k = s.M <= 64 && !wide ? 2 : 4;
   const int64_t block_keys = 32 * p.nw_k;
   p.row_tiles = (int64_t{s.N} + 32 * p.nw_q - 1) / (32 * p.nw_q);
   p.key_tiles = (int64_t{s.M} + block_keys - 1) / block_keys;
-  if (w.sinks > 0 && w.left >= 0) {
+  // row tiles of an ordinary block
+  const int64_t all = (int64_t{s.N} + bq - 1) / bq * s.G;
+  int64_t usual = all;
+  if (w.left >= 0 && w.right >= 0) usual = std::min(all, (int64_t{w.left} + w.right + block_keys + bq - 1) / bq * s.G);
+  const int64_t blocks = std::max<int64_t>(1, pairs * p.key_tiles);
+  p.splits = blocks < want ? std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, usual / 2)) : 1;
+  if (w.sinks > 0) {
     p.sink_tiles = std::min<int64_t>(p.key_tiles, (w.sinks + block_keys - 1) / block_keys);
-    // as many tiles a block as an ordinary one has, at least 8 (about 10 us)
-    const int64_t all = (int64_t{s.N} + bq - 1) / bq * s.G;
-    const int64_t usual = w.right < 0 ? all : (int64_t{w.left} + w.right + block_keys + bq - 1) / bq * s.G;
-    p.chunk_tiles = std::max<int64_t>(8, std::min(usual, all));
+    // as many tiles a block as an ordinary one has, at least 8 (about 10 us) where those are not split
+    p.chunk_tiles = std::max<int64_t>(p.splits > 1 ? 2 : 8, usual / p.splits);
     p.chunks = (all + p.chunk_tiles - 1) / p.chunk_tiles;
   }
   return p;
 }
 
 struct BwdSpace {
-  size_t stat, bound, part_k, part_bias, total;
+  size_t stat, bound, part_k, part_bias, sum_bias, total;
 };
 
-BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int64_t buckets, int dtype) {
+// span: distances of the bias, 0 without one
+BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int64_t span, int dtype) {
   const size_t pairs = static_cast<size_t>(s.B) * s.Hk;
   BwdSpace w;
   w.stat = static_cast<size_t>(s.B) * s.H * align_up(s.N, 64) * 4;
   w.bound = dtype == PMSST_F16 ? align_up(pairs * kParts * 4, 256) : 0;
-  const size_t sink_keys = p.sink_tiles * 32 * p.nw_k;
-  w.part_k = align_up((1 + p.chunks) * pairs * sink_keys * s.D * 4, 256);
-  w.part_bias = align_up(static_cast<size_t>(s.B) * s.H * (p.key_tiles + p.sink_tiles * p.chunks) * buckets * 4, 256);
-  w.total = align_up(3 * w.stat, 256) + 2 * w.bound + 2 * w.part_k + w.part_bias;
+  w.part_k = align_up(static_cast<size_t>(p.splits + p.chunks) * pairs * p.part_keys() * s.D * 4, 256);
+  const size_t blocks = static_cast<size_t>(s.B) * p.blocks();
+  w.part_bias = align_up(s.H * blocks * span * 4, 256);
+  w.sum_bias = align_up(s.H * ((blocks + kSumRows - 1) / kSumRows) * span * 4, 256);
+  w.total = align_up(2 * w.stat + w.stat / 32, 256) + 2 * w.bound + 2 * w.part_k + w.part_bias + w.sum_bias;
   return w;
 }
 
@@ -670,7 +710,7 @@ template <typename T, int DP, int NW>
 int launch_dkv(const BwdArgs& a, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
   if (a.bias.table) {
-    local_dkv_kernel<T, DP, NW, true><<<grid, 64 * NW, bias_entries(a.bias.distance) * 4 * (1 + NW), stream>>>(a);
+    local_dkv_kernel<T, DP, NW, true><<<grid, 64 * NW, (bias_entries(a.bias.distance) * (1 + NW) + 2 * kBinPad * NW) * 4, stream>>>(a);
   } else {
     local_dkv_kernel<T, DP, NW, false><<<grid, 64 * NW, 0, stream>>>(a);
   }
@@ -698,27 +738,35 @@ int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
     rc = launch_dq<T, DP, 4>(a, stream);
   }
   if (rc != PMSST_OK) return rc;
-  const int64_t per = p.key_tiles + p.sink_tiles * p.chunks;
+  const int64_t per = p.blocks();
   if (per > 0) {
     a.grid = make_grid(pairs, per);
     rc = launch_dkv<T, DP>(a, p, stream);
     if (rc != PMSST_OK) return rc;
   }
   if (a.bias.table) {
-    const dim3 grid(static_cast<uint32_t>(a.s.H), static_cast<uint32_t>((a.bias.buckets + 31) / 32));
-    const int64_t blocks = int64_t{a.s.B} * per;  // 0 without frames: zeros
+    const int span = 2 * a.bias.distance + 1;
+    const int64_t blocks = int64_t{a.s.B} * per, parts = (blocks + kSumRows - 1) / kSumRows;  // none without frames: zeros
+    if (parts > 0) {
+      const dim3 grid(static_cast<uint32_t>(a.s.H), static_cast<uint32_t>((span + 63) / 64), static_cast<uint32_t>(parts));
+      local_bins_sum_kernel<<<grid, 1024, 0, stream>>>(a.part_bias, a.sum_bias, blocks, span);
+      if ((rc = check_launch("local_bins_sum_kernel")) != PMSST_OK) return rc;
+    }
+    const dim3 grid(static_cast<uint32_t>(a.s.H), static_cast<uint32_t>((a.bias.buckets + 3) / 4));
     if (a.bias.f32) {
-      local_bias_sum_kernel<float><<<grid, 1024, 0, stream>>>(a.part_bias, static_cast<float*>(a.dbias), blocks, a.bias.buckets, a.s.H);
+      local_bias_sum_kernel<float><<<grid, 256, 0, stream>>>(a.sum_bias, static_cast<float*>(a.dbias), a.order, a.first,
+                                                             static_cast<int>(parts), span, a.cut, a.bias.buckets, a.s.H);
     } else {
-      local_bias_sum_kernel<T><<<grid, 1024, 0, stream>>>(a.part_bias, static_cast<T*>(a.dbias), blocks, a.bias.buckets, a.s.H);
+      local_bias_sum_kernel<T><<<grid, 256, 0, stream>>>(a.sum_bias, static_cast<T*>(a.dbias), a.order, a.first,
+                                                         static_cast<int>(parts), span, a.cut, a.bias.buckets, a.s.H);
     }
     if ((rc = check_launch("local_bias_sum_kernel")) != PMSST_OK) return rc;
   }
-  if (p.sink_tiles == 0) return rc;
-  const int keys = std::min(a.sink_keys, a.s.M);
+  const int keys = std::min(a.part_keys, a.s.M);
+  if (keys == 0) return rc;
   const int64_t blocks = (pairs * keys * (a.s.D / 4) + 255) / 256;
-  local_sink_sum_kernel<T><<<dim3(static_cast<uint32_t>(blocks), 2), 256, 0, stream>>>(a, keys);
-  return check_launch("local_sink_sum_kernel");
+  local_parts_sum_kernel<T><<<dim3(static_cast<uint32_t>(blocks), 2), 256, 0, stream>>>(a, keys);
+  return check_launch("local_parts_sum_kernel");
 }
 
 template <typename T>
@@ -733,15 +781,16 @@ extern "C" {
 
 size_t pmsst_local_attention_backward_workspace_size(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
                                                      int64_t head_dim, int64_t left, int64_t right, int64_t sinks,
-                                                     int has_starts, int64_t buckets, int dtype) {
+                                                     int has_starts, int64_t max_distance, int dtype) {
   using namespace pmsst::attn;
   LocalArgs l;
   static const int32_t some = 0;
   if (make_local("pmsst_local_attention_backward", batch, queries, keys, heads, kv_heads, head_dim, left, right, sinks,
                  has_starts ? &some : nullptr, nullptr, 0, nullptr, 0, 0, 1.0, dtype, l) != PMSST_OK ||
-      buckets < 0 || buckets > kMaxBuckets || l.s.B == 0 || l.s.N == 0)
+      max_distance > kMaxDistance || l.s.B == 0 || l.s.N == 0)
     return 0;
-  return pmsst::bwd_space(l.s, pmsst::plan_backward(l.s, l.w, dtype), buckets, dtype).total;
+  const int64_t span = max_distance < 0 ? 0 : 2 * reach_of(l.s, l.w, max_distance) + 1;
+  return pmsst::bwd_space(l.s, pmsst::plan_backward(l.s, l.w, dtype), span, dtype).total;
 }
 
 int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out_strides, const void* q, const int64_t* q_strides,
@@ -768,8 +817,9 @@ int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out
   a.s = l.s;
   a.w = l.w;
   a.bias = l.bias;
-  a.bias.order = bucket_order;
-  a.bias.first = bucket_first;
+  a.order = bucket_order;
+  a.first = bucket_first;
+  a.cut = l.cut;
   if ((rc = make_strides(what, grad_out, grad_out_strides, queries, heads, head_dim, dtype, a.gs)) != PMSST_OK) return rc;
   if ((rc = make_strides(what, out, nullptr, queries, heads, head_dim, dtype, a.os)) != PMSST_OK) return rc;
   if ((rc = make_strides(what, q, q_strides, queries, heads, head_dim, dtype, a.qs)) != PMSST_OK) return rc;
@@ -779,7 +829,7 @@ int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out
                  15) == 0,
                 "%s: gradients must be 16-byte aligned", what);
   const BwdPlan p = plan_backward(a.s, a.w, dtype);
-  const BwdSpace w = bwd_space(a.s, p, bias ? buckets : 0, dtype);
+  const BwdSpace w = bwd_space(a.s, p, bias ? 2 * a.bias.distance + 1 : 0, dtype);
   if (workspace == nullptr || workspace_bytes < w.total)
     return fail(PMSST_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, w.total, workspace_bytes);
   PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: workspace must be 16-byte aligned", what);
@@ -798,8 +848,8 @@ int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out
   a.rows_pad = static_cast<int32_t>(align_up(a.s.N, 64));
   a.base = reinterpret_cast<float*>(at);
   a.delta = reinterpret_cast<float*>(at + w.stat);
-  a.alive = reinterpret_cast<float*>(at + 2 * w.stat);
-  at += align_up(3 * w.stat, 256);
+  a.lone = reinterpret_cast<uint32_t*>(at + 2 * w.stat);
+  at += align_up(2 * w.stat + w.stat / 32, 256);
   a.vmax = reinterpret_cast<float*>(at);
   at += w.bound;
   a.l1 = reinterpret_cast<float*>(at);
@@ -809,16 +859,19 @@ int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out
   a.part_v = reinterpret_cast<float*>(at);
   at += w.part_k;
   a.part_bias = reinterpret_cast<float*>(at);
+  a.sum_bias = reinterpret_cast<float*>(at + w.part_bias);
   a.row_tiles = static_cast<uint32_t>(p.row_tiles);
   a.key_tiles = static_cast<uint32_t>(p.key_tiles);
   a.sink_tiles = static_cast<uint32_t>(p.sink_tiles);
   a.chunks = static_cast<uint32_t>(p.chunks);
   a.chunk_tiles = static_cast<int32_t>(p.chunk_tiles);
-  a.sink_keys = static_cast<int32_t>(p.sink_tiles * 32 * p.nw_k);
+  a.splits = static_cast<uint32_t>(p.splits);
+  a.sink_keys = static_cast<int32_t>(p.sink_keys());
+  a.part_keys = static_cast<int32_t>(p.part_keys());
   a.late_first = a.w.right >= 0 && a.w.left < 0;
-  const int64_t per = std::max(p.row_tiles * a.s.G, p.key_tiles + p.sink_tiles * p.chunks);
+  const int64_t per = std::max(p.row_tiles * a.s.G, p.blocks());
   PMSST_REQUIRE(grid_fits(batch * kv_heads, per), "%s: too many rows for one call", what);
-  PMSST_REQUIRE(batch * kv_heads * a.sink_keys * (head_dim / 4) < int64_t{1} << 31, "%s: too many sinks for one call", what);
+  PMSST_REQUIRE(batch * kv_heads * a.part_keys * (head_dim / 4) < int64_t{1} << 31, "%s: too many sinks for one call", what);
   a.scale = static_cast<float>(scale);
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   a.bias_unit = static_cast<float>(1.0 / scale);

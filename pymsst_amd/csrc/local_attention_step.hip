@@ -36,11 +36,55 @@ struct StepArgs {
   float scale_log2;
 };
 
-// 16 bytes as floats.
+// f of this lane's value and that of lane l ^ 16, the lower lane's first.
+template <typename F>
+__device__ __forceinline__ float rows_join(float v, F f) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a = r[0], b = r[1];
+  return f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+// Sum over the aligned groups of LPR lanes, by lane moves in the adder's own operand.
+template <int LPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += dpp_mov<0xB1>(v);                                    // quad_perm [1,0,3,2]
+  v += dpp_mov<0x4E>(v);                                    // quad_perm [2,3,0,1]
+  if constexpr (LPR >= 8) v += dpp_mov<0x141>(v);           // row_half_mirror
+  if constexpr (LPR >= 16) v += dpp_mov<0x140>(v);          // row_mirror
+  if constexpr (LPR >= 32) v = rows_join(v, [](float x, float y) { return x + y; });
+  return v;
+}
+
+// f over the lanes that share (lane % LPR).
+template <int LPR, typename F>
+__device__ __forceinline__ float groups_join(float v, F f) {
+  if constexpr (LPR <= 4) v = f(v, dpp_mov<0x124>(v));  // row_ror:4
+  if constexpr (LPR <= 8) v = f(v, dpp_mov<0x128>(v));  // row_ror:8
+  if constexpr (LPR <= 16) v = rows_join(v, f);
+  float lo, hi;
+  halves(v, lo, hi);
+  return f(lo, hi);
+}
+
+// Products of two 16-byte units, added to `sum` in fp32: 16-bit types two elements an instruction.
 template <typename T>
-struct Unit {
-  static constexpr int E = 16 / sizeof(T);
-};
+__device__ __forceinline__ float dot(const u32x4_t& a, const u32x4_t& b, float sum) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = a[i], y = b[i];
+    if constexpr (std::is_same<T, bf16>::value) {
+      typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, x), __builtin_bit_cast(v2, y), sum, false);
+    } else if constexpr (std::is_same<T, f16>::value) {
+      typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, x), __builtin_bit_cast(v2, y), sum, false);
+    } else {
+      sum = fmaf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y), sum);
+    }
+  }
+  return sum;
+}
 
 // What the lanes past a row's end multiply (with 0: nothing there may be infinite).
 static __device__ const u32x4_t zero_unit = {0, 0, 0, 0};
@@ -50,7 +94,7 @@ constexpr int kUnroll = 4;  // loads of K (and of V) on their way in a wave
 // LPR: lanes of a row (a power of two), RT: rows of the block.
 template <typename T, int LPR, int RT, bool BIAS>
 __global__ __launch_bounds__(256) void local_step_kernel(StepArgs a) {
-  constexpr int E = Unit<T>::E, KPW = 64 / LPR;
+  constexpr int E = 16 / sizeof(T), KPW = 64 / LPR;
   extern __shared__ float shared[];  // the bias of the rows' heads by distance back, then the waves' results
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   uint32_t pair, sub;
@@ -114,19 +158,18 @@ __global__ __launch_bounds__(256) void local_step_kernel(StepArgs a) {
   const int first = x0 + wave * KPW * kUnroll;
   if (first < x1) fetch(first);
 
-  // q in log2 units
-  float q[RT][E], o[RT][E], m[RT], l[RT];
+  u32x4_t q[RT];
+  float o[RT][E], m[RT], l[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     m[r] = -kInf;
     l[r] = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) q[r][i] = o[r][i] = 0.f;
+    for (int i = 0; i < E; ++i) o[r][i] = 0.f;
+    q[r] = u32x4_t{0, 0, 0, 0};
     if (r < rows && unit_ok) {
       const int row = r0 + r, n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(row))), head = hk * s.G + (row - n * s.G);
-      load_pack<T, E>(static_cast<const T*>(a.q) + b * a.qs.b + n * a.qs.n + head * a.qs.h + at, q[r]);
-#pragma unroll
-      for (int i = 0; i < E; ++i) q[r][i] *= a.scale_log2;
+      q[r] = *reinterpret_cast<const u32x4_t*>(static_cast<const T*>(a.q) + b * a.qs.b + n * a.qs.n + head * a.qs.h + at);
     }
   }
 
@@ -146,13 +189,16 @@ __global__ __launch_bounds__(256) void local_step_kernel(StepArgs a) {
     }
   }
 
+  // the query of a row, and where its head's bias begins
+  auto query_of = [&](int r) { return static_cast<int>(s.by_g.div(static_cast<uint32_t>(r0 + r))); };
   const int entries = a.bias.distance + 1;  // distances 0 .. back
+  auto table_of = [&](int r) { return min(s.G >= RT ? r : r % s.G, min(rows, s.G) - 1) * entries; };
   if constexpr (BIAS) {
     const int heads = min(rows, s.G);
     for (int i = threadIdx.x; i < heads * entries; i += blockDim.x) {
       const int g = i / entries, back = i - g * entries;
       const int head = hk * s.G + (r0 + g) % s.G;
-      shared[i] = bias_value(a.bias, dtype_code<T>(), s.H, head, -back, kLog2e);
+      shared[i] = bias_value(bias_entry(a.bias, dtype_code<T>(), s.H, head, a.bias.bucket_of[a.bias.distance - back]), kLog2e);
     }
     __syncthreads();
   }
@@ -168,30 +214,38 @@ __global__ __launch_bounds__(256) void local_step_kernel(StepArgs a) {
     float w[RT][kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      float x[E];
-      unpack<T>(kg[u], x);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        float sum = 0.f;
+      for (int r = 0; r < RT; ++r) w[r][u] = lanes_sum<LPR>(dot<T>(q[r], kg[u], 0.f)) * a.scale_log2;
+    }
+    // what every row sees whole: sinks, or window frames past those that the later queries have left behind
+    const int last = base + KPW * kUnroll;
+    const bool whole = last <= min(x1, old_frames) && (base >= sink_frames + s.N - 1 || last <= sink_frames);
+    if constexpr (BIAS) {
+      if (whole && base >= sink_frames && now - (window_first + last - 1 - sink_frames) >= a.bias.distance) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) sum = fmaf(q[r][i], x[i], sum);
-        w[r][u] = group_sum(sum, LPR);
+        for (int r = 0; r < RT; ++r) {
+          const float far = shared[table_of(r) + a.bias.distance];
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u) w[r][u] += far;
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int since = now - frame_of(base + u * KPW + slot_in_wave);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) w[r][u] += shared[table_of(r) + min(max(since + query_of(r), 0), a.bias.distance)];
+        }
       }
     }
+    if (!whole) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int x = base + u * KPW + slot_in_wave;
-      const int frame = frame_of(x);
+      for (int u = 0; u < kUnroll; ++u) {
+        const int x = base + u * KPW + slot_in_wave, frame = frame_of(x);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const int n = static_cast<int>(s.by_g.div(static_cast<uint32_t>(r0 + r)));
-        const int back = now + n - frame;
-        const bool seen = x < x1 && back >= 0 && (back <= a.left || frame < a.sinks);
-        if constexpr (BIAS) {
-          const int g = s.G >= RT ? r : r % s.G;
-          w[r][u] += shared[min(g, min(rows, s.G) - 1) * entries + min(max(back, 0), a.bias.distance)];
+        for (int r = 0; r < RT; ++r) {
+          const int back = now + query_of(r) - frame;
+          w[r][u] = x < x1 && back >= 0 && (back <= a.left || frame < a.sinks) ? w[r][u] : -kInf;
         }
-        w[r][u] = seen ? w[r][u] : -kInf;
       }
     }
 #pragma unroll
@@ -230,13 +284,12 @@ __global__ __launch_bounds__(256) void local_step_kernel(StepArgs a) {
   const int pitch = s.D + 2;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    float top = m[r];
-#pragma unroll
-    for (int off = LPR; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+    auto sum = [](float x, float y) { return x + y; };
+    const float top = groups_join<LPR>(m[r], [](float x, float y) { return fmaxf(x, y); });
     const float f = m[r] == -kInf ? 0.f : __builtin_amdgcn_exp2f(m[r] - top);
-    l[r] = cross_group_sum(l[r] * f, LPR);
+    l[r] = groups_join<LPR>(l[r] * f, sum);
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[r][i] = cross_group_sum(o[r][i] * f, LPR);
+    for (int i = 0; i < E; ++i) o[r][i] = groups_join<LPR>(o[r][i] * f, sum);
     float* to = shared + (wave * RT + r) * pitch;
     if (slot_in_wave == 0 && unit_ok) {
 #pragma unroll
@@ -311,7 +364,7 @@ StepPlan plan_step(const Shape& s, int64_t left, int64_t sinks, int dtype) {
   p.chunks = (int64_t{s.R} + p.rows - 1) / p.rows;
   const int64_t frames = left + s.N + sinks, per_wave = 64 / p.lanes * kUnroll;
   p.waves = 4;
-  const int64_t blocks = int64_t{s.B} * s.Hk * p.chunks, want = 2 * num_cus();
+  const int64_t blocks = int64_t{s.B} * s.Hk * p.chunks, want = num_cus();
   p.splits = 1;
   if (blocks < want) p.splits = std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, frames / (per_wave * p.waves * 4)));
   p.per_split = (frames + p.splits - 1) / p.splits;

@@ -811,7 +811,7 @@ class HipFusedExtension:
         with _DeviceGuard(q.device):
             size = self._lib.pmsst_local_attention_backward_workspace_size(
                 b, n, m, h, hk, d, left, right, sinks, query_starts is not None,
-                0 if bias is None else bias_plan.num_buckets, code)
+                -1 if bias is None else bias_plan.max_distance, code)
             ws = _workspace(size, q.device)
             rc = self._lib.pmsst_local_attention_backward(
                 _ptr(grad_out), gs, _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(out), _ptr(lse),

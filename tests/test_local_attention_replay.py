@@ -70,13 +70,13 @@ void forward(const Case& c, int rows) {
 }
 
 template <int BQ>
-void backward(const Case& c, int block, int group, int slots, int chunk) {
+void backward(const Case& c, int block, int group, int splits, int chunks, int chunk) {
   const int sink_tiles = c.w.sinks > 0 ? min((c.w.sinks + block - 1) / block, (c.frames + block - 1) / block) : 0;
   for (int tile = 0; tile * block < c.count; ++tile) {
     const int key0 = tile * block, end = min(key0 + block, c.count), all = (c.queries + BQ - 1) / BQ;
     std::vector<int> times(all * group);
-    for (int slot = 0; slot <= (tile < sink_tiles ? slots : 0); ++slot) {
-      const RowTiles r = rows_of<BQ>(c.w, c.start, c.queries, group, key0, end, slot, slots, chunk);
+    for (int slot = 0; slot < splits + (tile < sink_tiles ? chunks : 0); ++slot) {
+      const RowTiles r = rows_of<BQ>(c.w, c.start, c.queries, group, key0, end, slot, splits, chunks, chunk);
       CHECK(r.from >= 0 && r.from <= r.to && r.to <= r.tiles * group, "range %d %d of %d", r.from, r.to, r.tiles);
       for (int i = r.from; i < r.to; ++i) {
         const int g = i / r.tiles, t = r.first + i % r.tiles;
@@ -135,8 +135,8 @@ int main() {
     for (int rows : {64, 128}) {
       forward<32>(c, rows);
       forward<64>(c, rows);
-      backward<32>(c, rows, 1 + i % 3, 1 + below_n(4), 1 + below_n(9));
-      backward<64>(c, rows, 1 + i % 3, 1 + below_n(4), 1 + below_n(9));
+      backward<32>(c, rows, 1 + i % 3, 1 + below_n(5), 1 + below_n(4), 1 + below_n(9));
+      backward<64>(c, rows, 1 + i % 3, 1 + below_n(5), 1 + below_n(4), 1 + below_n(9));
     }
   }
   // the far ends of the documented ranges: no sum passes 32 bits
@@ -147,7 +147,7 @@ int main() {
         const int count = 1 << 28;
         const TileList l = tiles_of<64>(w, start, start + (1 << 28) - 1, count);
         CHECK(l.total >= 0 && (l.total == 0 || (l.at(0) >= 0 && l.at(l.total - 1) * int64_t{64} < count)), "far tiles");
-        const RowTiles r = rows_of<64>(w, start, 1 << 28, 1, count - 128, count, 0, 1, 8);
+        const RowTiles r = rows_of<64>(w, start, 1 << 28, 1, count - 128, count, 0, 1, 1, 8);
         CHECK(r.first >= 0 && r.first + r.tiles <= (1 << 22), "far rows");
       }
     }
