@@ -75,7 +75,8 @@ __device__ __forceinline__ float keep_bits(float x, uint32_t m) {
   return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & m);
 }
 
-// Adds the diagonals of x (lane l: frame l % 32, queries reg_key(i) + 8 (l / 32)) to bins[query - frame], this wave's alone.
+// Adds the diagonals of x (lane l: frame l % 32, queries reg_key(i) + 8 (l / 32)) to bins[query - frame], this wave's alone
+// (or with frames and queries exchanged, to bins[frame - query]).
 // The halves first exchange 8 registers, so that each holds 16 queries in a row.  A lower lane's query c at frame r
 // then ends in lane r + 15 - c: it moves up with each query after it, and the 15 places past lane 31 are free, as the
 // upper half's values are left out.  The upper half moves down likewise.
@@ -546,8 +547,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
         if (what == Sees::kNone) continue;
         hold(sizeof(T) == 4);
         const int at_lane = fresh<DB>(lane);
-        f32x16_t p;
+        f32x16_t p{}, ds{};
         bool near = false, upper = false;
+        // 16 bits: every fragment of the two products is on its way before the first of them (a read at a time leaves the
+        // matrix cores waiting for LDS; the registers are there, as two waves share a SIMD either way)
+        u32x4_t fq[sizeof(T) == 2 ? NS : 1], fg[sizeof(T) == 2 ? NS : 1];
+        if constexpr (sizeof(T) == 2) {
+          const int row = 32 * u + key_row(at_lane & 31);
+#pragma unroll
+          for (int i = 0; i < NS; ++i) fq[i] = row_frag<DB>(ql, row, i, at_lane >> 5);
+#pragma unroll
+          for (int i = 0; i < NS; ++i) fg[i] = row_frag<DB>(gl, row, i, at_lane >> 5);
+        }
         if constexpr (BIAS) {
           near = !bias_far(key0 - p0 - 31, a.bias.distance, upper);
           if (near) {
@@ -557,11 +568,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[r] = far;
           }
-          p = mma_rows_from<T, DP>(p, ql, u, kf, at_lane);
-        } else {
-          p = mma_rows<T, DP>(ql, u, kf, at_lane);
         }
-        f32x16_t ds = mma_rows<T, DP>(gl, u, vf, at_lane);
+        if constexpr (sizeof(T) == 2) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < NS; ++i) p = mma<T>(fq[i], kf[i], p);
+#pragma unroll
+          for (int i = 0; i < NS; ++i) ds = mma<T>(fg[i], vf[i], ds);
+        } else {
+          p = mma_rows_from<T, DP>(p, ql, u, kf, at_lane);
+          ds = mma_rows<T, DP>(gl, u, vf, at_lane);
+        }
         // (what lanes of unseen frames hold is dropped at the end, but for the bias's sums)
         if (what == Sees::kSome || (BIAS && any_unseen)) {
           uint32_t bits = queries_seeing(a.w, start, ki, row0) >> (8 * h);
@@ -619,6 +636,240 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
   }
 }
 
+// ---------------------------------------------------------------- up to 64 frames, 16 bits
+
+// All gradients in one pass where a tile holds every frame, as in the cross attention: a block of 2 waves keeps K and V of
+// a (batch row, key head) in LDS and passes over the query tiles of its heads; P and dS go through LDS to be the other
+// operand of dV and dK.  A wave's whole rows of P and dP are in registers, so D is their sum, in fp32.  5 products instead
+// of 7, and every tensor is moved once: 1032 x 62 queries over 62 frames with a bias, bf16, 8 heads of 64, see the figures at
+// plan_backward.
+template <typename T, int DP, bool BIAS>
+constexpr int few_waves() { return DP == 128 ? 1 : 2; }
+
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T, DP, BIAS>()))) void local_few_kernel(BwdArgs a) {
+  constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32, PB = 64 * sizeof(T);
+  constexpr bool kHalf = std::is_same<T, f16>::value;
+  __shared__ __attribute__((aligned(16))) char kv[2][64 * DB];
+  __shared__ __attribute__((aligned(16))) char rows[2][64 * DB];
+  __shared__ __attribute__((aligned(16))) char ps[2][64 * PB];
+  __shared__ float most[2];
+  extern __shared__ float table[];  // the bias by distance, then each wave's bins
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t pair, sub;
+  if (!locate(a.grid, pair, sub)) return;
+  const Shape& s = a.s;
+  const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk;
+  const int d_units = s.D * static_cast<int>(sizeof(T)) / 16;
+  const int count = key_count(a.km, b, s.M);
+  const int start = start_of(a.w, b);
+  uint64_t kept = range_bits(0, count);
+  if (a.km.mask) kept &= __ballot(a.km.mask[b * a.km.stride + min(lane, s.M - 1)] != 0);
+  const int entries = 2 * a.bias.distance + 1 + 2 * kPad;
+  float* bins = table + entries + kBinPad + wave * (entries + 2 * kBinPad);
+
+  Tile<T, DP, 64, 2> tile;  // no state: every move computes its addresses
+  tile.fetch_cut(kv[0], static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h, 0, s.M, d_units, [&](int i) { return i * a.ks.n; });
+  tile.fetch_cut(kv[1], static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h, 0, s.M, d_units, [&](int i) { return i * a.vs.n; });
+
+  f32x16_t dk[DT]{}, dv[DT]{};
+  constexpr int kNoSum = 101;  // above every exponent (scale_exponent's end at 100): nothing but zeros so far
+  int e_sum = kNoSum;          // dk is held at 2^e_sum
+  const int tiles = (s.N + 63) / 64;
+  for (int g = 0; g < s.G; ++g) {
+    const int head = hk * s.G + g;
+    float far_low = 0.f, far_high = 0.f, sum_low = 0.f, sum_high = 0.f;
+    for (int t = 0; t < tiles; ++t) {
+      if (g > 0 || t > 0) __syncthreads();  // the tiles of the rows before these have been read, and the table
+      tile.fetch_cut(rows[0], static_cast<const T*>(a.q) + b * a.qs.b + head * a.qs.h, t * 64, s.N, d_units, [&](int i) { return i * a.qs.n; });
+      tile.fetch_cut(rows[1], static_cast<const T*>(a.dout) + b * a.gs.b + head * a.gs.h, t * 64, s.N, d_units, [&](int i) { return i * a.gs.n; });
+      if constexpr (BIAS) {
+        if (t == 0) {
+          fill_bias<T, false>(table, a.bias, s.H, head, a.bias_unit, 128);
+          for (int i = lane; i < entries; i += 64) bins[i] = 0.f;
+        }
+      }
+      const int n0 = t * 64 + 32 * wave, n = n0 + (lane & 31), p0 = start + n0, pos = start + n;
+      const bool row_ok = n < s.N;
+      float base = -kInf;  // -lse in log2 units: a row that sees no frame (and one past the end) has no weight
+      if (row_ok) {
+        const float lse = a.lse[(static_cast<int64_t>(b) * s.H + head) * s.N + n];
+        base = lse == -kInf ? -kInf : -lse * kLog2e;
+      }
+      const int low = low_of(a.w, pos), high = high_of(a.w, pos, count);
+      uint32_t seen[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) seen[u] = static_cast<uint32_t>(kept >> (32 * u)) & frames_seen(low, high, a.w.sinks, 32 * u);
+      const bool lone = __popc(seen[0]) + __popc(seen[1]) == 1;
+      vm_wait<0>();
+      if (g == 0 && t == 0 && (kept != ~uint64_t{0} || d_units != tile.UNITS)) {
+        tile.clear(kv[0], kept, d_units);
+        tile.clear(kv[1], kept, d_units);
+      }
+      if (d_units != tile.UNITS) {
+        tile.clear(rows[0], ~uint64_t{0}, d_units);
+        tile.clear(rows[1], ~uint64_t{0}, d_units);
+      }
+      // rows past the end hold the last one again, whose infinities would meet their weights of 0
+      if (t * 64 + 64 > s.N) tile.clear_from(rows[1], s.N - t * 64);
+      __syncthreads();
+
+      const int at_lane = fresh<256>(lane);  // whatever DB: this kernel has no registers for addresses
+      if constexpr (BIAS) {
+        far_low = table[0];
+        far_high = table[entries - 1];
+      }
+      f32x16_t p[2], ds[2];
+      bool near[2] = {false, false}, upper[2] = {false, false};
+      {
+        u32x4_t f[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) f[i] = row_frag<DB>(rows[0], 32 * wave + (at_lane & 31), i, h);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if constexpr (BIAS) {
+            near[u] = !bias_far(32 * u - p0 - 31, a.bias.distance, upper[u]);
+            if (near[u]) {
+              p[u] = bias_tile(table + (a.bias.distance + kPad + 8 * h - pos + 32 * u));
+            } else {
+              const float far = upper[u] ? far_high : far_low;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) p[u][r] = far;
+            }
+            p[u] = mma_rows_from<T, DP>(p[u], kv[0], u, f, at_lane);
+          } else {
+            p[u] = mma_rows<T, DP>(kv[0], u, f, at_lane);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) f[i] = row_frag<DB>(rows[1], 32 * wave + (at_lane & 31), i, h);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) ds[u] = mma_rows<T, DP>(kv[1], u, f, at_lane);
+      }
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t bits = seen[u] >> (8 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float w = where_bit(bits, reg_key(i), __builtin_amdgcn_exp2f(fmaf(p[u][i], a.scale_log2, base)), 0.f);
+          sum[i & 1] = fmaf(w, ds[u][i], sum[i & 1]);
+          p[u][i] = w;
+        }
+      }
+      const float delta = half_sum(sum[0] + sum[1]), alive = lone ? 0.f : 1.f;
+      float top = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          ds[u][i] = p[u][i] * ((ds[u][i] - delta) * alive);
+          if constexpr (kHalf) top = fmaxf(top, fabsf(ds[u][i]));
+        }
+        if constexpr (BIAS) {
+          if (near[u]) {
+            add_diagonals(bins + (a.bias.distance + kPad + 32 * u - p0), ds[u], lane);
+          } else {
+            float far[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) far[i & 1] += ds[u][i];
+            const float both = far[0] + far[1];
+            sum_high += upper[u] ? both : 0.f;
+            sum_low += upper[u] ? 0.f : both;
+          }
+        }
+      }
+      int e = 0;
+      if constexpr (kHalf) {
+        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+        if (lane == 0) most[wave] = top;
+        __syncthreads();
+        top = fmaxf(most[0], most[1]);
+        e = top == 0.f ? kNoSum : scale_exponent(top, 15);
+        const float power = ldexpf(1.f, e);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            ds[u][i] *= power;
+            p[u][i] *= 16384.f;
+          }
+        }
+        // dk stays at the smaller power of two; this tile's dS are stored at it below
+        if (e < e_sum) {
+          const float down = e_sum == kNoSum ? 0.f : ldexpf(1.f, e - e_sum);
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dk[dt][i] *= down;
+          }
+          e_sum = e;
+        }
+      }
+
+      f32x16_t dq[DT]{};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) mma_cols<T, DP>(kv[0], u, ds[u], dq, at_lane);
+      const int row = 32 * wave + (at_lane & 31);
+      if (row_ok) {
+        const float dq_scale = kHalf ? ldexpf(a.scale, -e) : a.scale;
+        const int64_t to = (static_cast<int64_t>(b) * s.N + n) * s.H + head;
+        store_cols<T, DP>(static_cast<T*>(a.dq) + to * s.D, dq, dq_scale, s.D, h);
+      }
+
+      // [row][frame] tiles: a lane writes its row's frames, 8 consecutive ones a unit
+      const float shift = kHalf ? ldexpf(1.f, e_sum - e) : 1.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if constexpr (kHalf) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ds[u][i] *= shift;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int to = row * PB + 16 * ((4 * u + 2 * j + h) ^ swz<PB>(row));
+          *reinterpret_cast<u32x4_t*>(ps[0] + to) = pack8<T>(p[u], j);
+          *reinterpret_cast<u32x4_t*>(ps[1] + to) = pack8<T>(ds[u], j);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u32x4_t pf = col_frag<PB>(ps[0], 16 * k, wave, at_lane), sf = col_frag<PB>(ps[1], 16 * k, wave, at_lane);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          dv[dt] = mma<T>(col_frag<DB>(rows[1], 16 * k, dt, at_lane), pf, dv[dt]);
+          dk[dt] = mma<T>(col_frag<DB>(rows[0], 16 * k, dt, at_lane), sf, dk[dt]);
+        }
+      }
+    }
+    if constexpr (BIAS) {
+      // the head's bins, past the table's ends into the end ones, over the waves (the table's next fill waits at the
+      // head's first barrier, as does the clearing of the bins, which are a wave's own until then)
+      const float under = group_sum(sum_low + bins[lane], kWave);
+      const float above = group_sum(sum_high + bins[entries - kPad + lane], kWave);
+      if (lane == 0) {
+        bins[kPad] += under;
+        bins[entries - 1 - kPad] += above;
+      }
+      __syncthreads();
+      const int span = 2 * a.bias.distance + 1;
+      float* part = a.part_bias + (static_cast<int64_t>(head) * s.B + b) * span;
+      for (int i = threadIdx.x; i < span; i += 128) {  // by falling distance
+        const float* bin = table + entries + kBinPad + entries - 1 - kPad - i;
+        part[i] = bin[0] + bin[entries + 2 * kBinPad];
+      }
+    }
+  }
+  // a transposed read hands lane l the frame key_row(l % 32)
+  const int ki = 32 * wave + key_row(lane & 31);
+  if (ki >= s.M) return;
+  const float k_scale = kHalf ? ldexpf(a.scale, -e_sum) : a.scale, v_scale = kHalf ? 1.f / 16384.f : 1.f;
+  const int64_t to = ((static_cast<int64_t>(b) * s.M + ki) * s.Hk + hk) * s.D;
+  store_cols<T, DP>(static_cast<T*>(a.dk) + to, dk, k_scale, s.D, h);
+  store_cols<T, DP>(static_cast<T*>(a.dv) + to, dv, v_scale, s.D, h);
+}
+
 // dk, dv of the keys that several blocks share = the sum of their parts.  A thread takes 4 columns; the grid's y is the
 // gradient.
 template <typename T>
@@ -644,11 +895,12 @@ __global__ __launch_bounds__(256) void local_parts_sum_kernel(BwdArgs a, int key
 // ---------------------------------------------------------------- host
 
 struct BwdPlan {
+  bool few;  // local_few_kernel
   int nw_q, nw_k;
   int64_t row_tiles, key_tiles, splits, sink_tiles, chunks, chunk_tiles;
-  int64_t blocks() const { return key_tiles * splits + sink_tiles * chunks; }  // of a pair in local_dkv_kernel
+  int64_t blocks() const { return few ? 1 : key_tiles * splits + sink_tiles * chunks; }  // of a pair, that leave bins
   int64_t sink_keys() const { return sink_tiles * 32 * nw_k; }
-  int64_t part_keys() const { return splits > 1 ? key_tiles * 32 * nw_k : sink_keys(); }
+  int64_t part_keys() const { return few ? 0 : splits > 1 ? key_tiles * 32 * nw_k : sink_keys(); }
 };
 
 // The frames' blocks are split over their queries where they are
@@ -667,6 +919,8 @@ BwdPlan plan_backward(const Shape& s, const Window& w, int dtype) {
   int64_t usual = all;
   if (w.left >= 0 && w.right >= 0) usual = std::min(all, (int64_t{w.left} + w.right + block_keys + bq - 1) / bq * s.G);
   const int64_t blocks = std::max<int64_t>(1, pairs * p.key_tiles);
+  // (few pairs: a block each would leave CUs without any)
+  p.few = s.M > 0 && s.M <= 64 && dtype != PMSST_F32 && pairs >= num_cus();
   p.splits = blocks < want ? std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, usual / 2)) : 1;
   if (w.sinks > 0) {
     p.sink_tiles = std::min<int64_t>(p.key_tiles, (w.sinks + block_keys - 1) / block_keys);
@@ -685,8 +939,8 @@ struct BwdSpace {
 BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int64_t span, int dtype) {
   const size_t pairs = static_cast<size_t>(s.B) * s.Hk;
   BwdSpace w;
-  w.stat = static_cast<size_t>(s.B) * s.H * align_up(s.N, 64) * 4;
-  w.bound = dtype == PMSST_F16 ? align_up(pairs * kParts * 4, 256) : 0;
+  w.stat = p.few ? 0 : static_cast<size_t>(s.B) * s.H * align_up(s.N, 64) * 4;
+  w.bound = dtype == PMSST_F16 && !p.few ? align_up(pairs * kParts * 4, 256) : 0;
   w.part_k = align_up(static_cast<size_t>(p.splits + p.chunks) * pairs * p.part_keys() * s.D * 4, 256);
   const size_t blocks = static_cast<size_t>(s.B) * p.blocks();
   w.part_bias = align_up(s.H * blocks * span * 4, 256);
@@ -694,6 +948,9 @@ BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int64_t span, int dtype) {
   w.total = align_up(2 * w.stat + w.stat / 32, 256) + 2 * w.bound + 2 * w.part_k + w.part_bias + w.sum_bias;
   return w;
 }
+
+// LDS of a bias's table and the bins of `waves`.
+size_t bins_bytes(const BwdArgs& a, int waves) { return (bias_entries(a.bias.distance) * (1 + waves) + 2 * kBinPad * waves) * 4; }
 
 template <typename T, int DP, int NW>
 int launch_dq(const BwdArgs& a, hipStream_t stream) {
@@ -710,11 +967,19 @@ template <typename T, int DP, int NW>
 int launch_dkv(const BwdArgs& a, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
   if (a.bias.table) {
-    local_dkv_kernel<T, DP, NW, true><<<grid, 64 * NW, (bias_entries(a.bias.distance) * (1 + NW) + 2 * kBinPad * NW) * 4, stream>>>(a);
+    local_dkv_kernel<T, DP, NW, true><<<grid, 64 * NW, bins_bytes(a, NW), stream>>>(a);
   } else {
     local_dkv_kernel<T, DP, NW, false><<<grid, 64 * NW, 0, stream>>>(a);
   }
   return check_launch("local_dkv_kernel");
+}
+
+template <typename T, int DP>
+int launch_dq(const BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+  if constexpr (DP * sizeof(T) != 512) {
+    if (p.nw_q == 2) return launch_dq<T, DP, 2>(a, stream);
+  }
+  return launch_dq<T, DP, 4>(a, stream);
 }
 
 template <typename T, int DP>
@@ -728,21 +993,28 @@ int launch_dkv(const BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
 template <typename T, int DP>
 int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
   const int64_t pairs = int64_t{a.s.B} * a.s.Hk;
-  int rc = PMSST_OK;
-  if constexpr (std::is_same<T, f16>::value) rc = launch_bound<T>(a, pairs, stream);
-  if (rc != PMSST_OK) return rc;
-  a.grid = make_grid(pairs, p.row_tiles * a.s.G);
-  if constexpr (DP * sizeof(T) != 512) {
-    rc = p.nw_q == 2 ? launch_dq<T, DP, 2>(a, stream) : launch_dq<T, DP, 4>(a, stream);
-  } else {
-    rc = launch_dq<T, DP, 4>(a, stream);
-  }
-  if (rc != PMSST_OK) return rc;
   const int64_t per = p.blocks();
-  if (per > 0) {
-    a.grid = make_grid(pairs, per);
-    rc = launch_dkv<T, DP>(a, p, stream);
+  int rc = PMSST_OK;
+  if (p.few) {
+    if constexpr (sizeof(T) == 2) {
+      a.grid = make_grid(pairs, 1);
+      const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
+      if (a.bias.table) {
+        local_few_kernel<T, DP, true><<<grid, 128, bins_bytes(a, 2), stream>>>(a);
+      } else {
+        local_few_kernel<T, DP, false><<<grid, 128, 0, stream>>>(a);
+      }
+      if ((rc = check_launch("local_few_kernel")) != PMSST_OK) return rc;
+    }
+  } else {
+    if constexpr (std::is_same<T, f16>::value) rc = launch_bound<T>(a, pairs, stream);
     if (rc != PMSST_OK) return rc;
+    a.grid = make_grid(pairs, p.row_tiles * a.s.G);
+    if ((rc = launch_dq<T, DP>(a, p, stream)) != PMSST_OK) return rc;
+    if (per > 0) {
+      a.grid = make_grid(pairs, per);
+      if ((rc = launch_dkv<T, DP>(a, p, stream)) != PMSST_OK) return rc;
+    }
   }
   if (a.bias.table) {
     const int span = 2 * a.bias.distance + 1;

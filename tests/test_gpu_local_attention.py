@@ -96,6 +96,31 @@ def test_forward_and_backward(hip_ext, dtype, shape, rule, mask):
     check_attention(hip_ext, shape, dtype, *rule, mask=mask, bias_dtype=dtype if mask == "both" else torch.float32)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", _F)
+@pytest.mark.parametrize("shape", [(33, 62, 62, 8, 8, 64), (65, 70, 33, 8, 4, 32), (260, 5, 64, 2, 1, 128), (129, 130, 1, 2, 2, 40)])
+@pytest.mark.parametrize("rule", [(None, None, 0, 32, 24), (9, 12, 3, 16, 40), (20, 0, 2, 0, 0)])
+@pytest.mark.parametrize("mask", ["none", "both"])
+def test_few_frames_of_many_pairs(hip_ext, dtype, shape, rule, mask):
+    check_attention(hip_ext, shape, dtype, *rule, mask=mask, seed=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", _F)
+@pytest.mark.parametrize("shape,rule,starts", [
+    ((2, 40, 900, 2, 2, 64), (300, 0, 4, 32, 128), [860, 333]),   # a chunk over a longer cache: split forward
+    ((2, 3, 2000, 8, 2, 64), (None, 0, 0, 32, 64), [1997, -2]),
+    ((1, 513, 513, 4, 1, 64), (60, 11, 5, 16, 1000), None),       # the sinks' later queries in blocks of their own
+    ((2, 700, 640, 2, 2, 32), (130, 0, 140, 0, 0), [5, -100]),    # two tiles of sinks, split
+    ((3, 100, 90, 2, 1, 128), (30, 20, 2, 8, 9), [10**9, -(10**9), 80]),  # queries that see sinks alone, or nothing
+    ((1, 600, 600, 2, 2, 64), (0, 0, 0, 8, 6), None),             # a frame sees itself
+    ((1, 200, 200, 2, 2, 64), (None, None, 0, 8, 1024), None),    # distances beyond every pair
+])
+@pytest.mark.parametrize("mask", ["none", "lengths"])
+def test_windows_starts_and_splits(hip_ext, dtype, shape, rule, starts, mask):
+    check_attention(hip_ext, shape, dtype, *rule, mask=mask, starts=starts, seed=4)
+
+
 def _step_case(shape, dtype, slots, positions, seed=0):
     b, n, h, hk, d = shape
     g = torch.Generator().manual_seed(seed)
