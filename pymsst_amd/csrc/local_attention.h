@@ -139,6 +139,10 @@ __device__ __forceinline__ bool bias_far(int lo, int distance, bool& upper) {
   return upper || lo + 62 <= -distance;
 }
 
+// The first frame's distance to the first query of a tile, cut to where the table's ends begin: a tile beyond it reads
+// its end's entries, all alike.
+__device__ __forceinline__ int bias_gap(int gap, int distance) { return min(max(gap, -distance - 31), distance + 31); }
+
 // The accumulator of a score tile: `table` entries from this lane's first one on, in the order of the registers.
 __device__ __forceinline__ f32x16_t bias_tile(const float* first) {
   f32x16_t acc;

@@ -221,18 +221,31 @@ __global__ __launch_bounds__(256) void local_join_kernel(FwdArgs a, uint32_t qua
   const uint32_t row = by_quads.div(i), quad = i - row * quads_per_row;
   const Shape& s = a.s;
   const int64_t rows = static_cast<int64_t>(s.B) * s.H * s.N;
-  float top = -kInf;
-  for (int k = 0; k < a.splits; ++k) top = fmaxf(top, a.part_lse[k * rows + row]);
-  float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < a.splits; ++k) {
-    const float li = a.part_lse[k * rows + row];
-    // a split without frames (or, where none is seen, every one) has no weight; NaN stays NaN
-    const float w = li == -kInf ? 0.f : __builtin_amdgcn_exp2f((li - top) * kLog2e);
-    float x[4];
-    load_pack<float, 4>(a.part_o + (k * rows + row) * s.D + 4 * quad, x);
-    sum += w;
+  float top = -kInf, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < a.splits; k += 4) {  // four splits' loads at a time
+    float l[4], x[4][4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] = fmaf(w, x[c], o[c]);
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = min(k + j, a.splits - 1) * rows + row;
+      l[j] = a.part_lse[at];
+      load_pack<float, 4>(a.part_o + at * s.D + 4 * quad, x[j]);
+    }
+    float next = top;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) next = fmaxf(next, l[j]);
+    const float f = top == -kInf ? 0.f : __builtin_amdgcn_exp2f((top - next) * kLog2e);
+    top = next;
+    sum *= f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] *= f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // a split without frames (or, where none is seen, every one) has no weight; NaN stays NaN
+      const float w = k + j >= a.splits || l[j] == -kInf ? 0.f : __builtin_amdgcn_exp2f((l[j] - top) * kLog2e);
+      sum += w;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = w == 0.f ? o[c] : fmaf(w, x[j][c], o[c]);
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const uint32_t bh = row / static_cast<uint32_t>(s.N), n = row - bh * static_cast<uint32_t>(s.N);

@@ -11,13 +11,12 @@
 // has; the sums meet in fp32 in the workspace and a third kernel adds them.  So do the sums of blocks that are split over
 // their queries, where there are few of them.
 //
-// The bias's gradient sums dS along diagonals, in local_dkv_kernel.  A wave's 32 x 32 tile holds 63 of them.  With one
-// frame a lane and queries in a row in its registers, adding the registers one after the other while the sum moves on by a
-// lane in between brings every diagonal into one lane: 16 additions with a lane shift in the same instruction, for either
-// half of the wave.  The sums then go to the wave's own bins in LDS, one a distance.  Tiles beyond the table's distances
-// add up in registers.  Every block leaves its bins in the workspace, and a last kernel adds the blocks and the distances
-// of a bucket, in a fixed order.  (With the bins summed by bucket in every block, that sum took half of the kernel's time:
-// 16 x 2760 queries, window of 1024, 320 buckets, 1074 us against 552.)
+// The bias's gradient sums dS along diagonals, in local_dkv_kernel.  A wave's 32 x 32 tile holds 63 of them, with one
+// frame a lane and queries in registers: 31 additions with a lane move in the operand bring every diagonal into one lane
+// (add_diagonals), and two more add them to the wave's own bins in LDS, one a distance.  Tiles beyond the table's
+// distances add up in registers.  Every block leaves its bins in the workspace, and two small kernels add the blocks and the
+// distances of a bucket, in a fixed order.  (With the bins summed by bucket in every block, that sum took half of the
+// kernel's time: 16 x 2760 queries, window of 1024, 320 buckets, 1074 us against 552.)
 #include "attention_bwd.h"
 #include "local_attention.h"
 
@@ -64,46 +63,57 @@ __device__ __forceinline__ int pair_exponent(const BwdArgs& a, uint32_t pair) {
 // ---------------------------------------------------------------- diagonals
 constexpr int kBinPad = 16;  // places on either side of a wave's bins that add_diagonals adds zeros to
 
-// The value of the lane before (after) this one; 0 enters at the wave's end.
-__device__ __forceinline__ float from_before(float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x138, 0xF, 0xF, true));
-}
-__device__ __forceinline__ float from_after(float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x130, 0xF, 0xF, true));
+// x of lane l + N (l - N for N < 0) of the same row of 16 lanes; 0 past its ends.
+template <int N>
+__device__ __forceinline__ float row_moved(float x) {
+  if constexpr (N == 0) return x;
+  constexpr int kCtrl = N > 0 ? 0x100 + N : 0x110 - N;  // row_shl, row_shr
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kCtrl, 0xF, 0xF, true));
 }
 __device__ __forceinline__ float keep_bits(float x, uint32_t m) {
   return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & m);
 }
 
+// Adds 8 queries c = C .. 7 in a row over a row of 16 frames r: those with r >= c to lane r - c of `on`, the others to
+// lane r - c + 16 of `past`.
+template <int C>
+__device__ __forceinline__ void add_run(const float (&x)[8], float& on, float& past) {
+  on += row_moved<C>(x[C]);
+  if constexpr (C > 0) past += row_moved<C - 16>(x[C]);
+  if constexpr (C < 7) add_run<C + 1>(x, on, past);
+}
+
 // Adds the diagonals of x (lane l: frame l % 32, queries reg_key(i) + 8 (l / 32)) to bins[query - frame], this wave's alone
 // (or with frames and queries exchanged, to bins[frame - query]).
-// The halves first exchange 8 registers, so that each holds 16 queries in a row.  A lower lane's query c at frame r
-// then ends in lane r + 15 - c: it moves up with each query after it, and the 15 places past lane 31 are free, as the
-// upper half's values are left out.  The upper half moves down likewise.
+// A query's value moves to the lane of its diagonal inside its row of 16 lanes, in the operand of the addition; what
+// leaves the row's low end goes on 16 lanes up in the next sum.  With h = l / 32, p = l / 16 % 2 and i = l % 16, the three
+// sums then hold frame - query = 16 p - 8 h + i less 0, 16 and 32.  The rows' parts that mean the same are added, and
+// exchanging the halves leaves -32 + l of the lower half in one register and -40 + l of the upper half in another.
 __device__ __forceinline__ void add_diagonals(float* bins, const f32x16_t& x, int lane) {
-  uint32_t low = lane < 32 ? ~0u : 0u;
-  asm volatile("" : "+v"(low));  // a register's mask, not one of the few scalar pairs
-  float y[16];
+  float near[8], far[8];
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
-    const float near = x[c], far = x[8 + c];
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, near), __builtin_bit_cast(uint32_t, far), false, false);
-    const uint32_t first = r[0], second = r[1];  // queries c and 16 + c of the halves, 8 + c and 24 + c
-    y[c] = __builtin_bit_cast(float, first);
-    y[8 + c] = __builtin_bit_cast(float, second);
+    near[c] = x[c];
+    far[c] = x[8 + c];
   }
-  float up = keep_bits(y[0], low), down = keep_bits(y[15], ~low);
-#pragma unroll
-  for (int c = 1; c < 16; ++c) {
-    up = from_before(up) + keep_bits(y[c], low);
-    down = from_after(down) + keep_bits(y[15 - c], ~low);
-  }
-  // Every lane adds; those beyond the diagonals (from 47 on, below 17) add 0, up to 17 places past them.  A lane's places in
-  // the two additions differ, and the compiler may not read the second before it writes the first: they are other lanes'.
+  float a = 0.f, b = 0.f, c = 0.f;
+  add_run<0>(near, a, b);
+  add_run<0>(far, b, c);
+  uint32_t even = (lane & 16) ? 0u : ~0u;
+  asm volatile("" : "+v"(even));  // a register's mask, not one of the few scalar pairs
+  const uint32_t u = __builtin_bit_cast(uint32_t, b);
+  const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t of_even = rows[0], of_odd = rows[1];  // in odd rows the even ones' b, in even rows the odd ones'
+  a += keep_bits(__builtin_bit_cast(float, of_odd), even);
+  c += keep_bits(__builtin_bit_cast(float, of_even), ~even);
+  const auto halves = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, a), false, false);
+  const uint32_t first = halves[0], second = halves[1];
+  // Lanes beyond the diagonals add 0, up to 9 places past them.  A lane's places in the two additions differ, and the
+  // compiler may not read the second before it writes the first: they are other lanes'.
   asm volatile("" ::: "memory");
-  bins[15 - lane] += up;
+  bins[32 - lane] += __builtin_bit_cast(float, first);
   asm volatile("" ::: "memory");
-  bins[48 - lane] += down;
+  bins[40 - lane] += __builtin_bit_cast(float, second);
   asm volatile("" ::: "memory");
 }
 
@@ -435,24 +445,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
     Tile<T, DP, BQ, NW> qt, gt;
     auto q_at = [&](int i) { return i * a.qs.n; };
     auto g_at = [&](int i) { return i * a.gs.n; };
-    int next_g = from / tiles, next_t = first + from - next_g * tiles;  // the tile that is fetched next
     const T *q_head = nullptr, *g_head = nullptr;
     // waves 0 and 1 also move a tile's 64 (32) pairs of statistics, 4 bytes a lane
     const float* stat_head = nullptr;
     const uint32_t* lone_head = nullptr;
-    auto begin_head = [&] {
-      const int head = hk * s.G + next_g;
-      q_head = qb + head * a.qs.h;
-      g_head = gb + head * a.gs.h;
-      qt.start(q_head, next_t * BQ, d_units, q_at);
-      gt.start(g_head, next_t * BQ, d_units, g_at);
-      const int64_t at = (static_cast<int64_t>(b) * s.H + head) * a.rows_pad;
-      stat_head = (wave == 0 ? a.base : a.delta) + at + lane;
-      lone_head = a.lone + at / 32;
-    };
-    uint64_t lone_now = 0, lone_next = 0;  // the tile's queries that see one frame alone
-    auto fetch = [&](int stage) {
-      const int row0 = next_t * BQ;
+    uint32_t lone_next[2] = {0, 0};  // the tile's queries that see one frame alone
+    auto fetch = [&](int t, int stage) {
+      const int row0 = t * BQ;
       if (DB < 512 && row0 + BQ <= s.N) {
         qt.fetch(lds[stage][0], q_step);
         gt.fetch(lds[stage][1], g_step);
@@ -461,29 +460,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
         gt.fetch_cut(lds[stage][1], g_head, row0, s.N, d_units, g_at, reinterpret_cast<const T*>(zero_row));
       }
       if (wave < 2 && (BQ == 64 || lane < BQ)) dma4_m0(stat_head + row0, __builtin_amdgcn_readfirstlane(lds_addr(stat[stage]) + 256 * wave));
-      lone_next = lone_head[row0 / 32];
-      if constexpr (BQ == 64) lone_next |= static_cast<uint64_t>(lone_head[row0 / 32 + 1]) << 32;
-      if (++next_t == first + tiles) {
-        next_t = first;
-        ++next_g;
-      }
+#pragma unroll
+      for (int u = 0; u < SUBS; ++u) lone_next[u] = lone_head[row0 / 32 + u];
     };
     arrive(kf);
     arrive(vf);
-    int g_now = next_g, t_now = next_t;
-    begin_head();
-    fetch(0);
     const float* lane_table = nullptr;  // this lane's entry for a query at frame 0
-    float far_low = 0.f, far_high = 0.f, sum_low = 0.f, sum_high = 0.f;
+    float sum_low = 0.f, sum_high = 0.f;
     const int entries = 2 * a.bias.distance + 1 + 2 * kPad;
     float* bins = nullptr;
     auto begin_table = [&](int g) {
       fill_bias<T, true>(table, a.bias, s.H, hk * s.G + g, a.bias_unit, 64 * NW);
       for (int i = lane; i < entries; i += 64) bins[i] = 0.f;
       sum_low = sum_high = 0.f;
-      __syncthreads();
-      far_high = table[0];
-      far_low = table[entries - 1];
     };
     // a head's bins, over the waves
     auto end_table = [&](int g) {
@@ -502,119 +491,113 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
         for (int w = 0; w < NW; ++w) sum += table[entries + kBinPad + w * (entries + 2 * kBinPad) + kPad + i];
         part_bias[g * part_step + i] = sum * unscale;
       }
-      __syncthreads();  // before the bins are cleared
     };
     if constexpr (BIAS) {
       bins = table + entries + kBinPad + wave * (entries + 2 * kBinPad);
-      begin_table(g_now);
       lane_table = table + (a.bias.distance + kPad + 8 * h - ki);
     }
-    int stage = 0;
-    for (int i = from; i < to; ++i) {
-      char* ql = lds[stage][0];
-      char* gl = lds[stage][1];
-      const float* base = stat[stage][0];
-      const float* delta = stat[stage][1];
-      vm_wait<0>();  // this wave's moves of the tile have arrived
-      if (d_units != qt.UNITS) {
-        qt.clear(ql, ~uint64_t{0}, d_units);
-        gt.clear(gl, ~uint64_t{0}, d_units);
-      }
-      __syncthreads();
-      if constexpr (BIAS) {
-        if (i > from && t_now == first) {  // every wave is past the head before
-          end_table(g_now - 1);
-          begin_table(g_now);
+    // head by head: a loop over all tiles would hold what changes with the head in scalar registers that it does not have
+    for (int at = from; at < to;) {
+      const int g = at / tiles, head = hk * s.G + g, t0 = first + at - g * tiles, t1 = min(first + tiles, t0 + to - at);
+      if (at > from) __syncthreads();  // every wave is past the head before: its tiles, table and bins
+      at += t1 - t0;
+      q_head = qb + head * a.qs.h;
+      g_head = gb + head * a.gs.h;
+      qt.start(q_head, t0 * BQ, d_units, q_at);
+      gt.start(g_head, t0 * BQ, d_units, g_at);
+      const int64_t stat_at = (static_cast<int64_t>(b) * s.H + head) * a.rows_pad;
+      stat_head = (wave == 0 ? a.base : a.delta) + stat_at + lane;
+      lone_head = a.lone + stat_at / 32;
+      fetch(t0, 0);
+      if constexpr (BIAS) begin_table(g);
+      int stage = 0;
+      for (int t = t0; t < t1; ++t) {
+        char* ql = lds[stage][0];
+        char* gl = lds[stage][1];
+        const float* base = stat[stage][0];
+        const float* delta = stat[stage][1];
+        vm_wait<0>();  // this wave's moves of the tile have arrived
+        if (d_units != qt.UNITS) {
+          qt.clear(ql, ~uint64_t{0}, d_units);
+          gt.clear(gl, ~uint64_t{0}, d_units);
         }
-      }
-      lone_now = lone_next;
-      if (i + 1 < to) {
-        if (next_t == first) begin_head();
-        fetch(stage ^ 1);
-      }
-      stage ^= 1;
-      const int row_tile0 = t_now * BQ;
-      if (++t_now == first + tiles) {
-        t_now = first;
-        ++g_now;
-      }
-      if (idle) continue;
+        __syncthreads();
+        const uint32_t lone_now[2] = {lone_next[0], lone_next[1]};
+        if (t + 1 < t1) fetch(t + 1, stage ^ 1);
+        stage ^= 1;
+        const int row_tile0 = t * BQ;
+        if (idle) continue;
 #pragma unroll
-      for (int u = 0; u < SUBS; ++u) {
-        const int row0 = row_tile0 + 32 * u, p0 = start + row0;
-        if (row0 >= s.N) continue;
-        const Sees what = sees(a.w, p0, key0, count);
-        if (what == Sees::kNone) continue;
-        hold(sizeof(T) == 4);
-        const int at_lane = fresh<DB>(lane);
-        f32x16_t p{}, ds{};
-        bool near = false, upper = false;
-        // 16 bits: every fragment of the two products is on its way before the first of them (a read at a time leaves the
-        // matrix cores waiting for LDS; the registers are there, as two waves share a SIMD either way)
-        u32x4_t fq[sizeof(T) == 2 ? NS : 1], fg[sizeof(T) == 2 ? NS : 1];
-        if constexpr (sizeof(T) == 2) {
-          const int row = 32 * u + key_row(at_lane & 31);
+        for (int u = 0; u < SUBS; ++u) {
+          const int row0 = row_tile0 + 32 * u, p0 = start + row0;
+          if (row0 >= s.N) continue;
+          const Sees what = sees(a.w, p0, key0, count);
+          if (what == Sees::kNone) continue;
+          hold(sizeof(T) == 4);
+          const int at_lane = fresh<DB>(lane);
+          f32x16_t p{}, ds{};
+          bool near = false, upper = false;
+          // 16 bits: every fragment of the two products is on its way before the first of them (a read at a time leaves the
+          // matrix cores waiting for LDS; the registers are there, as two waves share a SIMD either way)
+          u32x4_t fq[sizeof(T) == 2 ? NS : 1], fg[sizeof(T) == 2 ? NS : 1];
+          if constexpr (sizeof(T) == 2) {
+            const int row = 32 * u + key_row(at_lane & 31);
 #pragma unroll
-          for (int i = 0; i < NS; ++i) fq[i] = row_frag<DB>(ql, row, i, at_lane >> 5);
+            for (int i = 0; i < NS; ++i) fq[i] = row_frag<DB>(ql, row, i, at_lane >> 5);
 #pragma unroll
-          for (int i = 0; i < NS; ++i) fg[i] = row_frag<DB>(gl, row, i, at_lane >> 5);
-        }
-        if constexpr (BIAS) {
-          near = !bias_far(key0 - p0 - 31, a.bias.distance, upper);
-          if (near) {
-            p = bias_tile(lane_table + p0);
+            for (int i = 0; i < NS; ++i) fg[i] = row_frag<DB>(gl, row, i, at_lane >> 5);
+          }
+          if constexpr (BIAS) {
+            near = !bias_far(key0 - p0 - 31, a.bias.distance, upper);
+            p = bias_tile(lane_table + (key0 - bias_gap(key0 - p0, a.bias.distance)));
+          }
+          if constexpr (sizeof(T) == 2) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) p = mma<T>(fq[i], kf[i], p);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) ds = mma<T>(fg[i], vf[i], ds);
           } else {
-            const float far = upper ? far_high : far_low;
+            p = mma_rows_from<T, DP>(p, ql, u, kf, at_lane);
+            ds = mma_rows<T, DP>(gl, u, vf, at_lane);
+          }
+          // (what lanes of unseen frames hold is dropped at the end, but for the bias's sums)
+          if (what == Sees::kSome || (BIAS && any_unseen)) {
+            uint32_t bits = queries_seeing(a.w, start, ki, row0) >> (8 * h);
+            if constexpr (BIAS) bits = seen ? bits : 0u;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = far;
+            for (int r = 0; r < 16; ++r) p[r] = where_bit(bits, reg_key(r), p[r], -kInf);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int row = 32 * u + reg_key(r) + 8 * h;
+            p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base[row]));
+            ds[r] = p[r] * fmaf(ds[r], dp_scale, -delta[row]);
+          }
+          const uint32_t sub_lone = lone_now[u];
+          if (sub_lone != 0) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = where_bit(sub_lone >> (8 * h), reg_key(r), ds[r] * 0.f, ds[r]);
+          }
+          hold(sizeof(T) == 4);
+          mma_cols<T, DP>(gl, u, p, dv, at_lane);
+          mma_cols<T, DP>(ql, u, ds, dk, at_lane);
+          if constexpr (BIAS) {
+            if (near) {
+              add_diagonals(bins + (a.bias.distance + kPad + p0 - key0), ds, lane);
+            } else {
+              float sum[2] = {0.f, 0.f};
+#pragma unroll
+              for (int r = 0; r < 16; ++r) sum[r & 1] += ds[r];
+              const float both = sum[0] + sum[1];
+              sum_high += upper ? both : 0.f;
+              sum_low += upper ? 0.f : both;
+            }
           }
         }
-        if constexpr (sizeof(T) == 2) {
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int i = 0; i < NS; ++i) p = mma<T>(fq[i], kf[i], p);
-#pragma unroll
-          for (int i = 0; i < NS; ++i) ds = mma<T>(fg[i], vf[i], ds);
-        } else {
-          p = mma_rows_from<T, DP>(p, ql, u, kf, at_lane);
-          ds = mma_rows<T, DP>(gl, u, vf, at_lane);
-        }
-        // (what lanes of unseen frames hold is dropped at the end, but for the bias's sums)
-        if (what == Sees::kSome || (BIAS && any_unseen)) {
-          uint32_t bits = queries_seeing(a.w, start, ki, row0) >> (8 * h);
-          if constexpr (BIAS) bits = seen ? bits : 0u;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) p[r] = where_bit(bits, reg_key(r), p[r], -kInf);
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = 32 * u + reg_key(r) + 8 * h;
-          p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base[row]));
-          ds[r] = p[r] * fmaf(ds[r], dp_scale, -delta[row]);
-        }
-        const uint32_t sub_lone = static_cast<uint32_t>(lone_now >> (32 * u));
-        if (sub_lone != 0) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) ds[r] = where_bit(sub_lone >> (8 * h), reg_key(r), ds[r] * 0.f, ds[r]);
-        }
-        if constexpr (BIAS) {
-          if (near) {
-            add_diagonals(bins + (a.bias.distance + kPad + p0 - key0), ds, lane);
-          } else {
-            float sum[2] = {0.f, 0.f};
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sum[r & 1] += ds[r];
-            const float both = sum[0] + sum[1];
-            sum_high += upper ? both : 0.f;
-            sum_low += upper ? 0.f : both;
-          }
-        }
-        hold(sizeof(T) == 4);
-        mma_cols<T, DP>(gl, u, p, dv, at_lane);
-        mma_cols<T, DP>(ql, u, ds, dk, at_lane);
       }
+      if constexpr (BIAS) end_table(g);
     }
-    if constexpr (BIAS) end_table(g_now - (t_now == first ? 1 : 0));
   }
   if (ki >= s.M) return;
   if (!seen) {
@@ -643,8 +626,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
 // operand of dV and dK.  A wave's whole rows of P and dP are in registers, so D is their sum, in fp32.  5 products instead
 // of 7, and every tensor is moved once: 1032 x 62 queries over 62 frames with a bias, bf16, 8 heads of 64, see the figures at
 // plan_backward.
+// (Waves that share a SIMD: fp16's scaling and a bias together pass the registers of two.)
 template <typename T, int DP, bool BIAS>
-constexpr int few_waves() { return DP == 128 ? 1 : 2; }
+constexpr int few_waves() { return DP == 128 || (DP == 64 && BIAS && std::is_same<T, f16>::value) ? 1 : 2; }
 
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T, DP, BIAS>()))) void local_few_kernel(BwdArgs a) {

@@ -594,6 +594,12 @@ class HipFusedExtension:
                 st = self._attention_strides(t)
         return t, (ctypes.c_int64 * 3)(*st[:3])
 
+    def _local_operand(self, t):
+        """:meth:`_attention_operand`, without strides where ``t`` is dense."""
+        if t.is_contiguous() and t.data_ptr() % 16 == 0:
+            return t, None
+        return self._attention_operand(t)
+
     @staticmethod
     def _attention_strides(t):
         # an axis of one element is never stepped along; torch lets it carry any stride, and calls it contiguous
@@ -765,7 +771,7 @@ class HipFusedExtension:
         left, right, sinks, bias, key_mask, mask_stride, key_lengths, query_starts, scale = self._local_check(
             q, k, v, left, right, sinks, bias, bias_plan, key_mask, key_lengths, query_starts, scale)
         code = dtype_code(q.dtype)
-        (q, qs), (k, ks), (v, vs) = self._attention_operand(q), self._attention_operand(k), self._attention_operand(v)
+        (q, qs), (k, ks), (v, vs) = self._local_operand(q), self._local_operand(k), self._local_operand(v)
         b, n, h, d = q.shape
         m, hk = k.shape[1], k.shape[2]
         out = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
@@ -805,9 +811,9 @@ class HipFusedExtension:
             grads.append(torch.empty_like(bias))
         if n == 0 or b == 0:
             return [t.zero_() for t in grads]
-        (q, qs), (k, ks), (v, vs) = self._attention_operand(q), self._attention_operand(k), self._attention_operand(v)
-        grad_out, gs = self._attention_operand(grad_out)
-        (out, _), lse = self._attention_operand(out.contiguous()), lse.contiguous()
+        (q, qs), (k, ks), (v, vs) = self._local_operand(q), self._local_operand(k), self._local_operand(v)
+        grad_out, gs = self._local_operand(grad_out)
+        (out, _), lse = self._local_operand(out.contiguous()), lse.contiguous()
         with _DeviceGuard(q.device):
             size = self._lib.pmsst_local_attention_backward_workspace_size(
                 b, n, m, h, hk, d, left, right, sinks, query_starts is not None,
@@ -840,19 +846,18 @@ class HipFusedExtension:
         b, n, h, d = q.shape
         hk = k.shape[2]
         _req(0 <= left <= 2**28 and 0 <= sinks <= 2**28, "left and sinks must lie in [0, 2**28]")
-        strides = []
-        for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-            _req(t.device == q.device and t.dtype == q.dtype and t.dim() == 4 and t.shape[0] == b and t.shape[2:] == k.shape[2:],
-                 f"{name} must have shape [B, slots, Hk, D] and q's dtype and device")
-            strides.append(self._cache_strides(t, name))
+        _req(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[0] == b and k_cache.shape[2:] == k.shape[2:],
+             "k_cache and v_cache must have shape [B, slots, Hk, D]")
+        _req(k_cache.device == q.device and v_cache.device == q.device and k_cache.dtype == q.dtype and v_cache.dtype == q.dtype,
+             "k_cache and v_cache must have q's dtype and device")
+        strides = self._cache_strides(k_cache, "k_cache"), self._cache_strides(v_cache, "v_cache")
         slots = k_cache.shape[1]
-        _req(v_cache.shape == k_cache.shape, "k_cache and v_cache must have one shape")
         _req(slots - sinks >= left + n, "the caches must have at least sinks + left + N slots")
         _req(positions.device == q.device and positions.dtype == torch.int32 and positions.shape == (b,),
              "positions must be an int32 tensor of shape [B] on q's device")
         bias = self._bias_check(q, bias, bias_plan, scale)
         code = dtype_code(q.dtype)
-        (q, qs), (k, ks), (v, vs) = self._attention_operand(q), self._attention_operand(k), self._attention_operand(v)
+        (q, qs), (k, ks), (v, vs) = self._local_operand(q), self._local_operand(k), self._local_operand(v)
         positions = positions.contiguous()
         out = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
         with _DeviceGuard(q.device):
@@ -868,6 +873,8 @@ class HipFusedExtension:
 
     def _cache_strides(self, t, name):
         """A cache's strides: it is written in place, so its rows must lie apart and cannot be copied."""
+        if t.is_contiguous() and t.data_ptr() % 16 == 0:
+            return None
         unit = 16 // t.element_size()
         st = self._attention_strides(t)
         apart, extent = True, t.shape[3]
