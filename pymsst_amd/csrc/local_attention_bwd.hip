@@ -44,7 +44,8 @@ struct BwdArgs {
   float* sum_bias;      // [H, groups of kSumRows of those, span]
   Shape s;
   Grid grid;
-  uint32_t row_tiles, key_tiles, splits, sink_tiles, chunks;
+  uint32_t row_begin, row_end;  // the row tiles of a launch of local_dq_kernel
+  uint32_t key_tiles, splits, sink_tiles, chunks;
   int32_t chunk_tiles, sink_keys, part_keys;
   bool late_first;
   float scale, scale_log2, bias_unit;
@@ -119,8 +120,10 @@ __device__ __forceinline__ void add_diagonals(float* bins, const f32x16_t& x, in
 
 // ---------------------------------------------------------------- dQ
 
-template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 ? 1 : 2))) void local_dq_kernel(BwdArgs a) {
+// TWICE: a pass for D before the one for dQ (16 bits; see the loop).
+template <typename T, int DP, int NW, bool BIAS, bool TWICE>
+__global__ __launch_bounds__(64 * NW)
+__attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 || (TWICE && DP == 128) ? 1 : 2))) void local_dq_kernel(BwdArgs a) {
   constexpr int DB = DP * sizeof(T), NS = DB / 32, DT = DP / 32;
   constexpr int BK = local_tile<T, DP>(), SUBS = BK / 32;
   constexpr bool kHalf = std::is_same<T, f16>::value;
@@ -131,7 +134,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
   if (!locate(a.grid, pair, sub_block)) return;
   const Shape& s = a.s;
   const uint32_t tile_up = s.by_g.div(sub_block), g = sub_block - tile_up * static_cast<uint32_t>(s.G);
-  const uint32_t row_tile = a.late_first ? a.row_tiles - 1 - tile_up : tile_up;
+  const uint32_t row_tile = a.late_first ? a.row_end - 1 - tile_up : a.row_begin + tile_up;
   const int b = static_cast<int>(pair) / s.Hk, hk = static_cast<int>(pair) - b * s.Hk, head = hk * s.G + static_cast<int>(g);
   const int d_units = s.D * static_cast<int>(sizeof(T)) / 16;
   const int64_t bh = static_cast<int64_t>(b) * s.H + head;
@@ -213,8 +216,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
   auto k_at = [&](int i) { return i * a.ks.n; };
   auto v_at = [&](int i) { return i * a.vs.n; };
   const int64_t k_step = BK * static_cast<int64_t>(sizeof(T)) * a.ks.n, v_step = BK * static_cast<int64_t>(sizeof(T)) * a.vs.n;
-  kt.start(kb, list.at(0) * BK, d_units, k_at);
-  vt.start(vb, list.at(0) * BK, d_units, v_at);
   uint8_t byte_now = 1, byte_next = 1;  // this lane's key of the mask
   auto fetch = [&](int i, int stage) {
     const int key0 = list.at(i) * BK;
@@ -233,8 +234,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
   arrive(qf);
   arrive(gf);
   asm volatile("" : "+v"(base), "+v"(delta));
-  if (mask && list.total > 0) byte_next = mask_byte(list.at(0));
-  if (list.total > 0) fetch(0, 0);
+  auto begin = [&] {
+    if (list.total == 0) return;
+    kt.start(kb, list.at(0) * BK, d_units, k_at);
+    vt.start(vb, list.at(0) * BK, d_units, v_at);
+    if (mask) byte_next = mask_byte(list.at(0));
+    fetch(0, 0);
+  };
+  begin();
   const float* lane_table = nullptr;  // this lane's entry for frame 0
   float far_low = 0.f, far_high = 0.f, rest[2] = {0.f, 0.f};
   if constexpr (BIAS) {
@@ -244,70 +251,85 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
     far_high = table[2 * a.bias.distance + 2 * kPad];
     lane_table = table + (a.bias.distance + kPad + 8 * h - pos);
   }
-  int stage = 0;
-  for (int i = 0; i < list.total; ++i) {
-    const int t = list.at(i);
-    char* kl = lds[stage][0];
-    char* vl = lds[stage][1];
-    uint64_t seen = range_bits(t * BK, count);
-    if (mask) {
-      byte_now = byte_next;
-      seen &= __ballot(byte_now != 0);
-      if (i + 1 < list.total) byte_next = mask_byte(list.at(i + 1));
-    }
-    seen &= kAll;
-    vm_wait<0>();  // this wave's moves of the tile have arrived
-    if (seen != kAll || d_units != kt.UNITS) {
-      kt.clear(kl, seen, d_units);
-      vt.clear(vl, seen, d_units);
-    }
-    __syncthreads();
-    if (i + 1 < list.total) fetch(i + 1, stage ^ 1);
-    stage ^= 1;
-    if (idle) continue;
+  // What a row's dS adds up to is 0 but for D's error (out is rounded, and so were the weights it is a sum of); with it, D is
+  // rowsum(P o dP) to fp32's precision.  Of 16-bit rows that see few frames, D's error would be as large as the roundings
+  // of dS and dQ together (windows of 39 frames: dQ 1.53 times one rounding's error, with the pass 1.42), so their
+  // blocks pass over the tiles once for D alone; where many are seen it is lost among them.  (A kernel of its own: the two
+  // passes hold the registers of a third wave, 456 us against 620 for 124 x 948 queries.)
+#pragma unroll 1
+  for (bool first_pass = TWICE;; first_pass = false) {
+    int stage = 0;
+    for (int i = 0; i < list.total; ++i) {
+      const int t = list.at(i);
+      char* kl = lds[stage][0];
+      char* vl = lds[stage][1];
+      uint64_t seen = range_bits(t * BK, count);
+      if (mask) {
+        byte_now = byte_next;
+        seen &= __ballot(byte_now != 0);
+        if (i + 1 < list.total) byte_next = mask_byte(list.at(i + 1));
+      }
+      seen &= kAll;
+      vm_wait<0>();  // this wave's moves of the tile have arrived
+      if (seen != kAll || d_units != kt.UNITS) {
+        kt.clear(kl, seen, d_units);
+        vt.clear(vl, seen, d_units);
+      }
+      __syncthreads();
+      if (i + 1 < list.total) fetch(i + 1, stage ^ 1);
+      stage ^= 1;
+      if (idle) continue;
 #pragma unroll
-    for (int u = 0; u < SUBS; ++u) {
-      const int key0 = t * BK + 32 * u;
-      const uint32_t sub_seen = static_cast<uint32_t>(seen >> (32 * u));
-      const Sees what = sees(a.w, p0, key0, count);
-      if (sub_seen == 0 || what == Sees::kNone) continue;
-      const int at_lane = fresh<DB>(lane);
-      f32x16_t p;
-      if constexpr (BIAS) {
-        bool upper;
-        if (bias_far(key0 - p0 - 31, a.bias.distance, upper)) {
-          const float far = upper ? far_high : far_low;
+      for (int u = 0; u < SUBS; ++u) {
+        const int key0 = t * BK + 32 * u;
+        const uint32_t sub_seen = static_cast<uint32_t>(seen >> (32 * u));
+        const Sees what = sees(a.w, p0, key0, count);
+        if (sub_seen == 0 || what == Sees::kNone) continue;
+        const int at_lane = fresh<DB>(lane);
+        f32x16_t p;
+        if constexpr (BIAS) {
+          bool upper;
+          if (bias_far(key0 - p0 - 31, a.bias.distance, upper)) {
+            const float far = upper ? far_high : far_low;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) p[r] = far;
+            for (int r = 0; r < 16; ++r) p[r] = far;
+          } else {
+            p = bias_tile(lane_table + key0);
+          }
+          p = mma_rows_from<T, DP>(p, kl, u, qf, at_lane);
         } else {
-          p = bias_tile(lane_table + key0);
+          p = mma_rows<T, DP>(kl, u, qf, at_lane);
         }
-        p = mma_rows_from<T, DP>(p, kl, u, qf, at_lane);
-      } else {
-        p = mma_rows<T, DP>(kl, u, qf, at_lane);
-      }
-      const f32x16_t dp = mma_rows<T, DP>(vl, u, gf, at_lane);
-      if (what == Sees::kSome || sub_seen != 0xFFFFFFFFu) {
-        uint32_t bits = sub_seen;
-        if (what == Sees::kSome) bits &= frames_seen(low, high, a.w.sinks, key0);
-        bits >>= 8 * h;
+        const f32x16_t dp = mma_rows<T, DP>(vl, u, gf, at_lane);
+        if (what == Sees::kSome || sub_seen != 0xFFFFFFFFu) {
+          uint32_t bits = sub_seen;
+          if (what == Sees::kSome) bits &= frames_seen(low, high, a.w.sinks, key0);
+          bits >>= 8 * h;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = where_bit(bits, reg_key(r), p[r], -kInf);
-      }
+          for (int r = 0; r < 16; ++r) p[r] = where_bit(bits, reg_key(r), p[r], -kInf);
+        }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base)) * (dp[r] - delta);
-      }
-      if (lone != 0) {
+        for (int r = 0; r < 16; ++r) {
+          p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base)) * (dp[r] - delta);
+        }
+        if (lone != 0) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] *= alive;
-      }
-      if constexpr (BIAS) {
+          for (int r = 0; r < 16; ++r) p[r] *= alive;
+        }
+        if constexpr (BIAS || TWICE) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) rest[r & 1] += p[r];
+          for (int r = 0; r < 16; ++r) rest[r & 1] += p[r];
+        }
+        if (TWICE && first_pass) continue;
+        mma_cols<T, DP>(kl, u, p, acc, at_lane);
       }
-      mma_cols<T, DP>(kl, u, p, acc, at_lane);
     }
+    if (!TWICE || !first_pass) break;
+    const float total = half_sum(rest[0] + rest[1]);
+    delta += kHalf ? ldexpf(total, -e) : total;
+    rest[0] = rest[1] = 0.f;
+    __syncthreads();  // every wave has read the last tile
+    begin();
   }
   if (row_ok) {
     const float out_scale = kHalf ? ldexpf(a.scale, -e) : a.scale;
@@ -316,8 +338,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP * si
   }
   // for the other kernel, in the form it takes them; rows past the end have no weight
   if constexpr (BIAS) {
-    // What a row's dS adds up to, 0 but for D's error (out is rounded, and so were the weights it is a sum of): with it, D
-    // is rowsum(P o dP) to fp32's precision, which the bias's gradient needs (with D from out it is 3e-4 off).
+    // the bias's gradient needs D to fp32's precision (with D from out it is 3e-4 off)
     const float total = half_sum(rest[0] + rest[1]);
     delta += kHalf ? ldexpf(total, -e) : total;
   }
@@ -881,6 +902,7 @@ __global__ __launch_bounds__(256) void local_parts_sum_kernel(BwdArgs a, int key
 struct BwdPlan {
   bool few;  // local_few_kernel
   int nw_q, nw_k;
+  int64_t twice_tiles;  // the first row tiles, whose queries see few frames: local_dq_kernel passes twice
   int64_t row_tiles, key_tiles, splits, sink_tiles, chunks, chunk_tiles;
   int64_t blocks() const { return few ? 1 : key_tiles * splits + sink_tiles * chunks; }  // of a pair, that leave bins
   int64_t sink_keys() const { return sink_tiles * 32 * nw_k; }
@@ -898,6 +920,11 @@ BwdPlan plan_backward(const Shape& s, const Window& w, int dtype) {
   const int64_t block_keys = 32 * p.nw_k;
   p.row_tiles = (int64_t{s.N} + 32 * p.nw_q - 1) / (32 * p.nw_q);
   p.key_tiles = (int64_t{s.M} + block_keys - 1) / block_keys;
+  if (s.M <= 96 || (w.left >= 0 && w.right >= 0 && int64_t{w.left} + w.right + w.sinks < 96)) {
+    p.twice_tiles = p.row_tiles;
+  } else if (w.starts == nullptr && w.right >= 0 && w.right < 32) {
+    p.twice_tiles = std::min<int64_t>(p.row_tiles, 256 / (32 * p.nw_q));  // a past that grows
+  }
   // row tiles of an ordinary block
   const int64_t all = (int64_t{s.N} + bq - 1) / bq * s.G;
   int64_t usual = all;
@@ -936,15 +963,29 @@ BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int64_t span, int dtype) {
 // LDS of a bias's table and the bins of `waves`.
 size_t bins_bytes(const BwdArgs& a, int waves) { return (bias_entries(a.bias.distance) * (1 + waves) + 2 * kBinPad * waves) * 4; }
 
-template <typename T, int DP, int NW>
-int launch_dq(const BwdArgs& a, hipStream_t stream) {
+template <typename T, int DP, int NW, bool TWICE>
+int launch_dq(BwdArgs& a, int64_t begin, int64_t end, hipStream_t stream) {
+  if (begin == end) return PMSST_OK;
+  a.row_begin = static_cast<uint32_t>(begin);
+  a.row_end = static_cast<uint32_t>(end);
+  a.grid = make_grid(int64_t{a.s.B} * a.s.Hk, (end - begin) * a.s.G);
   const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
   if (a.bias.table) {
-    local_dq_kernel<T, DP, NW, true><<<grid, 64 * NW, bias_entries(a.bias.distance) * 4, stream>>>(a);
+    local_dq_kernel<T, DP, NW, true, TWICE><<<grid, 64 * NW, bias_entries(a.bias.distance) * 4, stream>>>(a);
   } else {
-    local_dq_kernel<T, DP, NW, false><<<grid, 64 * NW, 0, stream>>>(a);
+    local_dq_kernel<T, DP, NW, false, TWICE><<<grid, 64 * NW, 0, stream>>>(a);
   }
   return check_launch("local_dq_kernel");
+}
+
+template <typename T, int DP, int NW>
+int launch_dq(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    const int rc = launch_dq<T, DP, NW, true>(a, 0, p.twice_tiles, stream);
+    return rc != PMSST_OK ? rc : launch_dq<T, DP, NW, false>(a, p.twice_tiles, p.row_tiles, stream);
+  } else {
+    return launch_dq<T, DP, NW, false>(a, 0, p.row_tiles, stream);
+  }
 }
 
 template <typename T, int DP, int NW>
@@ -959,11 +1000,11 @@ int launch_dkv(const BwdArgs& a, hipStream_t stream) {
 }
 
 template <typename T, int DP>
-int launch_dq(const BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
+int launch_dq(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
   if constexpr (DP * sizeof(T) != 512) {
-    if (p.nw_q == 2) return launch_dq<T, DP, 2>(a, stream);
+    if (p.nw_q == 2) return launch_dq<T, DP, 2>(a, p, stream);
   }
-  return launch_dq<T, DP, 4>(a, stream);
+  return launch_dq<T, DP, 4>(a, p, stream);
 }
 
 template <typename T, int DP>
@@ -993,7 +1034,6 @@ int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
   } else {
     if constexpr (std::is_same<T, f16>::value) rc = launch_bound<T>(a, pairs, stream);
     if (rc != PMSST_OK) return rc;
-    a.grid = make_grid(pairs, p.row_tiles * a.s.G);
     if ((rc = launch_dq<T, DP>(a, p, stream)) != PMSST_OK) return rc;
     if (per > 0) {
       a.grid = make_grid(pairs, per);
@@ -1116,7 +1156,6 @@ int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out
   at += w.part_k;
   a.part_bias = reinterpret_cast<float*>(at);
   a.sum_bias = reinterpret_cast<float*>(at + w.part_bias);
-  a.row_tiles = static_cast<uint32_t>(p.row_tiles);
   a.key_tiles = static_cast<uint32_t>(p.key_tiles);
   a.sink_tiles = static_cast<uint32_t>(p.sink_tiles);
   a.chunks = static_cast<uint32_t>(p.chunks);
