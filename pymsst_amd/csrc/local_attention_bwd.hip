@@ -35,7 +35,7 @@ struct BwdArgs {
   int32_t cut;                   // indexes cut off on either side of the bias's table
   const float* lse;  // [B, H, N]
   void *dq, *dk, *dv, *dbias;
-  float *base, *delta;  // [B * H, rows_pad]: -lse in log2 units (- inf: no weight), D
+  float *base, *delta;  // [B * H, rows_pad]: -lse in log2 units (- inf: no weight), -D
   uint32_t* lone;       // [B * H, rows_pad / 32]: a bit for each query that sees one frame alone
   int32_t rows_pad;     // N rounded up to 64
   float *vmax, *l1;     // fp16: [pairs, kParts] maxima of |V| over the seen frames and of |dO row|_1
@@ -343,10 +343,9 @@ __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 || (TWICE && DP == 128) 
     delta += kHalf ? ldexpf(total, -e) : total;
   }
   if (h == 0 && n < a.rows_pad) {
-    if constexpr (kHalf) delta = ldexpf(delta, pair_exponent(a, pair));
     const int64_t at = bh * a.rows_pad + n;
     a.base[at] = row_base + (kHalf ? 14.f : 0.f);
-    a.delta[at] = delta;
+    a.delta[at] = -delta;
     if (lane == 0) a.lone[at / 32] = lone;
   }
 }
@@ -354,19 +353,20 @@ __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 || (TWICE && DP == 128) 
 // The blocks' bins become the buckets' sums in two steps, each in a fixed order: `rows` blocks' at a time by distance,
 // then those sums by bucket.
 constexpr int kSumRows = 256;
-__global__ __launch_bounds__(1024) void local_bins_sum_kernel(const float* parts, float* sums, int64_t blocks, int span) {
+__global__ __launch_bounds__(1024) void local_bins_sum_kernel(const float* bins, float* sums, int64_t blocks, int64_t parts, int span) {
   __shared__ float red[16][64];
   const int x = threadIdx.x & 63, y = threadIdx.x >> 6, at = static_cast<int>(blockIdx.y) * 64 + x;
-  const int64_t head = blockIdx.x, from = int64_t{blockIdx.z} * kSumRows, to = from + kSumRows < blocks ? from + kSumRows : blocks;
+  const int64_t head = blockIdx.x / parts, part = blockIdx.x - head * parts, from = part * kSumRows;
+  const int64_t to = from + kSumRows < blocks ? from + kSumRows : blocks;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   if (at < span) {
-    const float* part = parts + head * blocks * span + at;
+    const float* bin = bins + head * blocks * span + at;
     int64_t k = from + y;
     for (; k + 48 < to; k += 64) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] += part[(k + 16 * j) * span];
+      for (int j = 0; j < 4; ++j) sum[j] += bin[(k + 16 * j) * span];
     }
-    for (; k < to; k += 16) sum[0] += part[k * span];
+    for (; k < to; k += 16) sum[0] += bin[k * span];
   }
   red[y][x] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
   __syncthreads();
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(1024) void local_bins_sum_kernel(const float* parts
   float t = 0.f;
 #pragma unroll
   for (int j = 0; j < 16; ++j) t += red[j][x];
-  sums[(head * gridDim.z + blockIdx.z) * span + at] = t;
+  sums[blockIdx.x * static_cast<int64_t>(span) + at] = t;
 }
 
 // dbias[bucket, head]; a wave a bucket.  `order` and `first` are by the whole table's indexes, of which `cut` lie off
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
   constexpr int BQ = local_tile<T, DP>(), SUBS = BQ / 32;
   constexpr bool kHalf = std::is_same<T, f16>::value;
   __shared__ __attribute__((aligned(16))) char lds[kStages][2][BQ * DB];
-  __shared__ __attribute__((aligned(16))) float stat[kStages][2][64];  // -lse (log2 units), D
+  __shared__ __attribute__((aligned(16))) float stat[kStages][2][64];  // -lse (log2 units), -D
   extern __shared__ float table[];  // the bias by falling distance, then each wave's bins
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t pair, sub_block;
@@ -557,6 +557,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
           hold(sizeof(T) == 4);
           const int at_lane = fresh<DB>(lane);
           f32x16_t p{}, ds{};
+          if constexpr (sizeof(T) == 2) {  // dP - D as one sum
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = delta[32 * u + reg_key(r) + 8 * h];
+          }
           bool near = false, upper = false;
           // 16 bits: every fragment of the two products is on its way before the first of them (a read at a time leaves the
           // matrix cores waiting for LDS; the registers are there, as two waves share a SIMD either way)
@@ -593,7 +597,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
           for (int r = 0; r < 16; ++r) {
             const int row = 32 * u + reg_key(r) + 8 * h;
             p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base[row]));
-            ds[r] = p[r] * fmaf(ds[r], dp_scale, -delta[row]);
+            ds[r] = p[r] * (sizeof(T) == 4 ? ds[r] + delta[row] : kHalf ? ds[r] * dp_scale : ds[r]);
           }
           const uint32_t sub_lone = lone_now[u];
           if (sub_lone != 0) {
@@ -1044,8 +1048,8 @@ int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
     const int span = 2 * a.bias.distance + 1;
     const int64_t blocks = int64_t{a.s.B} * per, parts = (blocks + kSumRows - 1) / kSumRows;  // none without frames: zeros
     if (parts > 0) {
-      const dim3 grid(static_cast<uint32_t>(a.s.H), static_cast<uint32_t>((span + 63) / 64), static_cast<uint32_t>(parts));
-      local_bins_sum_kernel<<<grid, 1024, 0, stream>>>(a.part_bias, a.sum_bias, blocks, span);
+      const dim3 grid(static_cast<uint32_t>(a.s.H * parts), static_cast<uint32_t>((span + 63) / 64));
+      local_bins_sum_kernel<<<grid, 1024, 0, stream>>>(a.part_bias, a.sum_bias, blocks, parts, span);
       if ((rc = check_launch("local_bins_sum_kernel")) != PMSST_OK) return rc;
     }
     const dim3 grid(static_cast<uint32_t>(a.s.H), static_cast<uint32_t>((a.bias.buckets + 3) / 4));

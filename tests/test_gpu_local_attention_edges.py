@@ -310,6 +310,15 @@ def test_own_buckets_and_many_of_them(hip_ext, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", _F)
+@pytest.mark.parametrize("d", [64, 128])
+def test_the_largest_distance(hip_ext, dtype, d):
+    """1024 frames either way: the most that the tables in LDS hold, beside the largest tiles; and steps over as many."""
+    check_attention(hip_ext, (1, 1100, 1100, 1, 1, d), dtype, buckets=64, distance=1024)
+    check_step(hip_ext, (2, 4, 8, 2, d), dtype, 1500, 3, 1504, [5000, 900], 64, 1024)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", _F)
 def test_large_scores_scales_and_magnitudes(hip_ext, dtype):
     for shape in ((1, 100, 300, 2, 2, 64), (65, 62, 62, 4, 4, 64)):
         rule = dict(left=80, right=30, sinks=2, buckets=16, distance=50)
