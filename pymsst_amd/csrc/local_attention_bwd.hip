@@ -35,7 +35,7 @@ struct BwdArgs {
   int32_t cut;                   // indexes cut off on either side of the bias's table
   const float* lse;  // [B, H, N]
   void *dq, *dk, *dv, *dbias;
-  float *base, *delta;  // [B * H, rows_pad]: -lse in log2 units (- inf: no weight), -D
+  float *base, *delta;  // [B * H, rows_pad]: -lse in log2 units (- inf: no weight), D
   uint32_t* lone;       // [B * H, rows_pad / 32]: a bit for each query that sees one frame alone
   int32_t rows_pad;     // N rounded up to 64
   float *vmax, *l1;     // fp16: [pairs, kParts] maxima of |V| over the seen frames and of |dO row|_1
@@ -343,9 +343,10 @@ __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 || (TWICE && DP == 128) 
     delta += kHalf ? ldexpf(total, -e) : total;
   }
   if (h == 0 && n < a.rows_pad) {
+    if constexpr (kHalf) delta = ldexpf(delta, pair_exponent(a, pair));
     const int64_t at = bh * a.rows_pad + n;
     a.base[at] = row_base + (kHalf ? 14.f : 0.f);
-    a.delta[at] = -delta;
+    a.delta[at] = delta;
     if (lane == 0) a.lone[at / 32] = lone;
   }
 }
@@ -408,7 +409,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
   constexpr int BQ = local_tile<T, DP>(), SUBS = BQ / 32;
   constexpr bool kHalf = std::is_same<T, f16>::value;
   __shared__ __attribute__((aligned(16))) char lds[kStages][2][BQ * DB];
-  __shared__ __attribute__((aligned(16))) float stat[kStages][2][64];  // -lse (log2 units), -D
+  __shared__ __attribute__((aligned(16))) float stat[kStages][2][64];  // -lse (log2 units), D
   extern __shared__ float table[];  // the bias by falling distance, then each wave's bins
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t pair, sub_block;
@@ -557,10 +558,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
           hold(sizeof(T) == 4);
           const int at_lane = fresh<DB>(lane);
           f32x16_t p{}, ds{};
-          if constexpr (sizeof(T) == 2) {  // dP - D as one sum
-#pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = delta[32 * u + reg_key(r) + 8 * h];
-          }
           bool near = false, upper = false;
           // 16 bits: every fragment of the two products is on its way before the first of them (a read at a time leaves the
           // matrix cores waiting for LDS; the registers are there, as two waves share a SIMD either way)
@@ -597,7 +594,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
           for (int r = 0; r < 16; ++r) {
             const int row = 32 * u + reg_key(r) + 8 * h;
             p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], a.scale_log2, base[row]));
-            ds[r] = p[r] * (sizeof(T) == 4 ? ds[r] + delta[row] : kHalf ? ds[r] * dp_scale : ds[r]);
+            // (not as one sum with the product, begun at -D: the matrix cores' roundings then lean to D's side, and the bias's
+            // gradient of 124 x 948 queries is 1e-5 off instead of 6e-7)
+            ds[r] = p[r] * fmaf(ds[r], dp_scale, -delta[row]);
           }
           const uint32_t sub_lone = lone_now[u];
           if (sub_lone != 0) {

@@ -310,6 +310,23 @@ def test_own_buckets_and_many_of_them(hip_ext, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", _F)
+@pytest.mark.parametrize("rule", [dict(), dict(left=120, right=0, sinks=2)])
+def test_an_fp32_bias_gradient_of_many_pairs(hip_ext, dtype, rule):
+    """The bars bound every rounding at its worst; what leans to one side adds up long before that.  A row's weights are off
+    by at most about 40 roundings of 2^-24 (scores of 5, lse of 7, sums of 258), 2.4e-6, each row to its own side: over the
+    6192 rows of a head the sums' errors fall below a tenth of that, and the fp32 sums of a bin's up to 2 10^5 terms add
+    their square root in roundings, 2.7e-5 / sqrt(terms) of a sum of |dS| that is sqrt(terms) times the signed sum's
+    size or less: 2e-6 of the gradient's norm holds both with room, the 3e-4 of a D from a rounded output does not."""
+    b, n, h = 24, 258, 4
+    q, k, v, do, _, _ = _inputs((b, n, n, h, h, 64), dtype, seed=21)
+    bias, plan = _bias(hip_ext, h, 32, 128, rule.get("right") != 0, torch.float32)
+    db = _run(hip_ext, q, k, v, do, bias=bias, bias_plan=plan, **rule)[5]
+    want = oa.local_attention_backward(*map(to_np, (do, q, k, v)), bias=to_np(bias), bucket_of=plan.bucket_of.cpu().numpy(), **rule)[3]
+    assert np.linalg.norm(to_np(db) - want) <= 2e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", _F)
 @pytest.mark.parametrize("d", [64, 128])
 def test_the_largest_distance(hip_ext, dtype, d):
     """1024 frames either way: the most that the tables in LDS hold, beside the largest tiles; and steps over as many."""
