@@ -12,6 +12,11 @@
 //
 // The slots that are written hold frames that no query of the call sees (slots - sinks >= left + frames), and the new
 // frames are read from k and v, not from the caches: no block waits for another.
+//
+// One row: HBM and the launch; 8 rows of a shared key head: the same (200 MB of fp16 keys and values of 128 in 46 us, 4.3
+// TB/s).  Four rows with a bias: the vector unit, whose lookups by distance come on top (219 MB in 57 us, 3.8 TB/s).  The
+// smallest call's kernel is 5 us and its enqueue 14.  Waves of a block: 8 in place of 4 took 50 us for 47, 2 took 80; loads in
+// flight a lane: kUnroll of 2 and 8 took 48 and 50.
 #include "local_attention.h"
 
 namespace pmsst {
@@ -356,6 +361,9 @@ struct StepPlan {
   int64_t chunks, splits, per_split;
 };
 
+// A lane group holds a row of K, a block the rows of a key head up to 8, rounded up to the next instance.  Blocks are split
+// over the frames, into shares of four rounds of loads or more, where there are fewer than CUs: one stream, 8 heads of 64 on
+// one key head over 60000 frames, 65 us against 1089; with 8 key heads over 4000, 20 us against 30.
 StepPlan plan_step(const Shape& s, int64_t left, int64_t sinks, int dtype) {
   StepPlan p;
   const int units = s.D * static_cast<int>(dtype_size(dtype)) / 16;
