@@ -471,6 +471,7 @@ int pmsst_local_attention_step(const void* q, const int64_t* q_strides, const vo
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(PMSST_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
   PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0 || need == 0, "%s: workspace must be 16-byte aligned", what);
+  PMSST_REQUIRE(k_cache != v_cache, "%s: the caches lie in one place", what);
   a.q = q;
   a.k = k;
   a.v = v;

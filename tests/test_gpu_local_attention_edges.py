@@ -151,6 +151,15 @@ def test_c_abi_refusals():
     assert fwd(b=0) == 0 and fwd(n=0) == 0 and step(b=0) == 0 and step(n=0) == 0  # nothing to do
 
 
+def test_one_cache_for_keys_and_values_is_refused():
+    """Each would be written over the other."""
+    lib = _lib.load_library()
+    one = ctypes.c_void_p(4096)  # never dereferenced
+    rc = lib.pmsst_local_attention_step(one, None, one, None, one, None, one, None, one, None, one, 9, 4, None, 0, None, 0, 0, one,
+                                        2, 1, 20, 4, 2, 64, 1.0, 2, None, 0, None)
+    assert rc == -1 and b"one place" in lib.pmsst_last_error()
+
+
 def test_calls_past_the_grid_are_refused():
     lib = _lib.load_library()
     one = ctypes.c_void_p(4096)  # never dereferenced
