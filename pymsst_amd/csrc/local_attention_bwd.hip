@@ -378,7 +378,7 @@ __global__ __launch_bounds__(1024) void local_bins_sum_kernel(const float* bins,
   sums[blockIdx.x * static_cast<int64_t>(span) + at] = t;
 }
 
-// dbias[bucket, head]; a wave a bucket.  `order` and `first` are by the whole table's indexes, of which `cut` lie off
+// dbias[bucket, head]; a wave a bucket (16 x 2760 queries, one side of 800 distances in one bucket: 12.7 -> 6.7 us with four at a time).  `order` and `first` are by the whole table's indexes, of which `cut` lie off
 // either end; the sums are by falling distance.
 template <typename B>
 __global__ __launch_bounds__(256) void local_bias_sum_kernel(const float* sums, B* out, const int32_t* order, const int32_t* first,
@@ -388,10 +388,17 @@ __global__ __launch_bounds__(256) void local_bias_sum_kernel(const float* sums, 
   const float* from = sums + static_cast<int64_t>(blockIdx.x) * parts * span;
   const int begin = max(0, first[c]), end = min(all, first[c + 1]);
   float sum = 0.f;
-  for (int i = begin + x; i < end; i += 64) {
-    const int at = span - 1 - (order[i] - cut);
-    if (at < 0 || at >= span) continue;
-    for (int z = 0; z < parts; ++z) sum += from[static_cast<int64_t>(z) * span + at];
+  for (int base = begin + x; base < end; base += 4 * 64) {  // two loads, one waiting for the other: four at a time
+    int at[4];
+    float value[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) at[j] = span - 1 - (order[min(base + j * 64, end - 1)] - cut);
+    for (int z = 0; z < parts; ++z) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) value[j] = from[static_cast<int64_t>(z) * span + min(max(at[j], 0), span - 1)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += base + j * 64 < end && at[j] >= 0 && at[j] < span ? value[j] : 0.f;
+    }
   }
   sum = group_sum(sum, kWave);
   if (x == 0) out[static_cast<int64_t>(c) * heads + blockIdx.x] = from_f32<B>(sum);
