@@ -378,8 +378,8 @@ __global__ __launch_bounds__(1024) void local_bins_sum_kernel(const float* bins,
   sums[blockIdx.x * static_cast<int64_t>(span) + at] = t;
 }
 
-// dbias[bucket, head]; a wave a bucket (16 x 2760 queries, one side of 800 distances in one bucket: 12.7 -> 6.7 us with four at a time).  `order` and `first` are by the whole table's indexes, of which `cut` lie off
-// either end; the sums are by falling distance.
+// dbias[bucket, head]; a wave a bucket (one with 800 distances: 6.7 us, 12.7 without four loads at a time).  `order` and
+// `first` are by the whole table's indexes, of which `cut` lie off either end; the sums are by falling distance.
 template <typename B>
 __global__ __launch_bounds__(256) void local_bias_sum_kernel(const float* sums, B* out, const int32_t* order, const int32_t* first,
                                                              int parts, int span, int cut, int buckets, int heads) {
@@ -927,8 +927,8 @@ struct BwdPlan {
 };
 
 // The frames' blocks are split over their queries where they are fewer than two a CU, into shares of at least two tiles:
-// fp32, 4 x 317 queries and frames, 8 heads on 2, local_dkv_kernel 38 us and a sum of 8 against 186 and 5.  The sinks'
-// rows in blocks of their own: 16 x 2760 queries, window of 1024, 4 sinks, 339 us and a sum of 8 against 357 and 6 (more
+// fp32, 4 x 317 queries and frames, 8 heads on 2, local_dkv_kernel 38 us and a sum of 5 against 186 and 4.  The sinks'
+// rows in blocks of their own: 16 x 2760 queries, window of 1024, 4 sinks, 339 us and a sum of 5 against 357 and 4 (more
 // with narrower windows, where a sinks' block passes over more times as many rows as another).
 BwdPlan plan_backward(const Shape& s, const Window& w, int dtype) {
   const bool wide = padded_dim(s.D) * static_cast<int>(dtype_size(dtype)) == 512;

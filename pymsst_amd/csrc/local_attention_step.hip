@@ -14,8 +14,8 @@
 // frames are read from k and v, not from the caches: no block waits for another.
 //
 // One row: HBM and the launch; 8 rows of a shared key head: the same (200 MB of fp16 keys and values of 128 in 46 us, 4.3
-// TB/s).  Four rows with a bias: the vector unit, whose lookups by distance come on top (219 MB in 57 us, 3.8 TB/s).  The
-// smallest call's kernel is 5 us and its enqueue 14.  Waves of a block: 8 in place of 4 took 50 us for 47, 2 took 80; loads in
+// TB/s).  Four rows with a bias: the vector unit (219 MB in 57 us, 3.8 TB/s; a padded table that saves the lookups' cuts changes
+// nothing).  The smallest call's kernel is 5 us and its enqueue 14.  Waves of a block: 8 in place of 4 took 50 us for 47, 2 took 80; loads in
 // flight a lane: kUnroll of 2 and 8 took 48 and 50.
 #include "local_attention.h"
 
