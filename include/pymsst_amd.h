@@ -473,7 +473,8 @@ int pmsst_local_attention_forward(const void* q, const int64_t* q_strides, const
                                   double scale, int dtype, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
-/* Bytes of workspace of the backward on the current device (max_distance: -1 without a bias). */
+/* Bytes of workspace of the backward on the current device (max_distance: -1 without a bias; 0 where up to 64 frames of
+ * 16 bits meet many batch rows without one, and workspace may then be NULL). */
 size_t pmsst_local_attention_backward_workspace_size(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
                                                      int64_t kv_heads, int64_t head_dim, int64_t left, int64_t right,
                                                      int64_t sinks, int has_starts, int64_t max_distance, int dtype);

@@ -1145,9 +1145,9 @@ int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out
                 "%s: gradients must be 16-byte aligned", what);
   const BwdPlan p = plan_backward(a.s, a.w, dtype);
   const BwdSpace w = bwd_space(a.s, p, bias ? 2 * a.bias.distance + 1 : 0, dtype);
-  if (workspace == nullptr || workspace_bytes < w.total)
+  if (w.total > 0 && (workspace == nullptr || workspace_bytes < w.total))  // few frames without a bias: none is needed
     return fail(PMSST_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, w.total, workspace_bytes);
-  PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: workspace must be 16-byte aligned", what);
+  PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0 || w.total == 0, "%s: workspace must be 16-byte aligned", what);
   a.q = q;
   a.k = k;
   a.v = v;
