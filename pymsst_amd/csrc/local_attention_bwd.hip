@@ -39,14 +39,15 @@ struct BwdArgs {
   uint32_t* lone;       // [B * H, rows_pad / 32]: a bit for each query that sees one frame alone
   int32_t rows_pad;     // N rounded up to 64
   float *vmax, *l1;     // fp16: [pairs, kParts] maxima of |V| over the seen frames and of |dO row|_1
-  float *part_k, *part_v;  // [splits + chunks, pairs, part_keys, D]: of the keys that several blocks share
+  // of the keys that several blocks share: [splits, pairs, part_keys, D], then the sinks' later rows' [chunks, pairs, sink_rows, D]
+  float *part_k, *part_v;
   float* part_bias;     // [H, B * blocks of a pair in local_dkv_kernel, span]: sums by falling distance
   float* sum_bias;      // [H, groups of kSumRows of those, span]
   Shape s;
   Grid grid;
   uint32_t row_begin, row_end;  // the row tiles of a launch of local_dq_kernel
   uint32_t key_tiles, splits, sink_tiles, chunks;
-  int32_t chunk_tiles, part_keys;
+  int32_t chunk_tiles, part_keys, sink_rows;
   bool late_first;
   float scale, scale_log2, bias_unit;
   struct { float factor; } drop;  // what attn_bound_kernel's bound is multiplied by: no dropout here
@@ -640,8 +641,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
     }
   }
   if (a.splits > 1 || key_tile < a.sink_tiles) {
-    if (slot >= a.splits && ki >= a.w.sinks) return;  // no row past the window sees this frame
-    const int64_t at = ((static_cast<int64_t>(slot) * a.grid.pairs + pair) * a.part_keys + ki) * s.D;
+    if (slot >= a.splits && ki >= a.sink_rows) return;  // no row past the window sees this frame
+    int64_t row = (static_cast<int64_t>(min(slot, a.splits)) * a.grid.pairs + (slot < a.splits ? pair : 0u)) * a.part_keys + ki;
+    if (slot >= a.splits) row += (static_cast<int64_t>(slot - a.splits) * a.grid.pairs + pair) * a.sink_rows;
+    const int64_t at = row * s.D;
     store_cols_f32<T, DP>(a.part_k + at, dk, k_scale, s.D, h);
     store_cols_f32<T, DP>(a.part_v + at, dv, v_scale, s.D, h);
   } else {
@@ -897,17 +900,23 @@ __global__ __launch_bounds__(256) void local_parts_sum_kernel(BwdArgs a, uint32_
   const int64_t key = by_quads.div(i), quad = i - static_cast<uint32_t>(key) * quads;
   const float* from = (blockIdx.y != 0 ? a.part_v : a.part_k) + ((static_cast<int64_t>(pair) * a.part_keys + key) * quads + quad) * 4;
   const int64_t step = static_cast<int64_t>(a.grid.pairs) * a.part_keys * s.D;
-  const int slots = static_cast<int>(a.splits + (key < a.w.sinks ? a.chunks : 0));
+  const int64_t sink_step = static_cast<int64_t>(a.grid.pairs) * a.sink_rows * s.D;
   float o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int c = 0; c < slots; c += 4) {
-    float x[4][4];
+  auto add = [&](const float* first, int64_t apart, int parts) {
+    for (int c = 0; c < parts; c += 4) {
+      float x[4][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) load_pack<float, 4>(from + min(c + k, slots - 1) * step, x[k]);
+      for (int k = 0; k < 4; ++k) load_pack<float, 4>(first + min(c + k, parts - 1) * apart, x[k]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 4; ++k) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] += c + k < slots ? x[k][j] : 0.f;
+        for (int j = 0; j < 4; ++j) o[j] += c + k < parts ? x[k][j] : 0.f;
+      }
     }
+  };
+  add(from, step, static_cast<int>(a.splits));
+  if (key < a.sink_rows) {
+    add(from + a.splits * step + static_cast<int64_t>(pair) * (a.sink_rows - a.part_keys) * s.D, sink_step, static_cast<int>(a.chunks));
   }
   const uint32_t b = pair / static_cast<uint32_t>(s.Hk), hk = pair - b * static_cast<uint32_t>(s.Hk);
   T* out = static_cast<T*>(blockIdx.y != 0 ? a.dv : a.dk);
@@ -924,6 +933,7 @@ struct BwdPlan {
   int64_t blocks() const { return few ? 1 : key_tiles * splits + sink_tiles * chunks; }  // of a pair, that leave bins
   int64_t sink_keys() const { return sink_tiles * 32 * nw_k; }
   int64_t part_keys() const { return few ? 0 : splits > 1 ? key_tiles * 32 * nw_k : sink_keys(); }
+  static int64_t sink_rows(const Shape& s, const Window& w) { return std::min(w.sinks, s.M); }
 };
 
 // The frames' blocks are split over their queries where they are fewer than two a CU, into shares of at least two tiles:
@@ -954,8 +964,15 @@ BwdPlan plan_backward(const Shape& s, const Window& w, int dtype) {
   p.splits = blocks < want ? std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, usual / 2)) : 1;
   if (w.sinks > 0) {
     p.sink_tiles = std::min<int64_t>(p.key_tiles, (w.sinks + block_keys - 1) / block_keys);
-    // as many tiles a block as an ordinary one has, at least 8 (about 10 us) where those are not split
+    // as many tiles a block as an ordinary one has, at least 8 (about 10 us) where those are not split; past 64 MB, no
+    // more parts than the frames' own gradients would take in fp32 (16 x 8192 queries, windows of 128 either way, 2048
+    // sinks, 4 parts in place of 16: the backward takes 2382 us in place of 2969, and 0.7 GB in place of 2.2)
     p.chunk_tiles = std::max<int64_t>(p.splits > 1 ? 2 : 8, usual / p.splits);
+    const int64_t sinks = p.sink_rows(s, w), part_bytes = 8 * pairs * sinks * s.D;
+    if (part_bytes > 0) {
+      const int64_t most = std::max<int64_t>({1, (int64_t{64} << 20) / part_bytes, s.M / sinks});
+      p.chunk_tiles = std::max(p.chunk_tiles, (all + most - 1) / most);
+    }
     p.chunks = (all + p.chunk_tiles - 1) / p.chunk_tiles;
   }
   return p;
@@ -966,12 +983,13 @@ struct BwdSpace {
 };
 
 // span: distances of the bias, 0 without one
-BwdSpace bwd_space(const Shape& s, const BwdPlan& p, int64_t span, int dtype) {
+BwdSpace bwd_space(const Shape& s, const Window& win, const BwdPlan& p, int64_t span, int dtype) {
   const size_t pairs = static_cast<size_t>(s.B) * s.Hk;
   BwdSpace w;
   w.stat = p.few ? 0 : static_cast<size_t>(s.B) * s.H * align_up(s.N, 64) * 4;
   w.bound = dtype == PMSST_F16 && !p.few ? align_up(pairs * kParts * 4, 256) : 0;
-  w.part_k = align_up(static_cast<size_t>(p.splits + p.chunks) * pairs * p.part_keys() * s.D * 4, 256);
+  const int64_t sink_parts = p.few ? 0 : p.chunks * p.sink_rows(s, win);
+  w.part_k = align_up(pairs * (p.splits * p.part_keys() + sink_parts) * s.D * 4, 256);
   const size_t blocks = static_cast<size_t>(s.B) * p.blocks();
   w.part_bias = align_up(s.H * blocks * span * 4, 256);
   w.sum_bias = align_up(s.H * ((blocks + kSumRows - 1) / kSumRows) * span * 4, 256);
@@ -1105,7 +1123,7 @@ size_t pmsst_local_attention_backward_workspace_size(int64_t batch, int64_t quer
       max_distance > kMaxDistance || l.s.B == 0 || l.s.N == 0)
     return 0;
   const int64_t span = max_distance < 0 ? 0 : 2 * reach_of(l.s, l.w, max_distance) + 1;
-  return pmsst::bwd_space(l.s, pmsst::plan_backward(l.s, l.w, dtype), span, dtype).total;
+  return pmsst::bwd_space(l.s, l.w, pmsst::plan_backward(l.s, l.w, dtype), span, dtype).total;
 }
 
 int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out_strides, const void* q, const int64_t* q_strides,
@@ -1144,7 +1162,7 @@ int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out
                  15) == 0,
                 "%s: gradients must be 16-byte aligned", what);
   const BwdPlan p = plan_backward(a.s, a.w, dtype);
-  const BwdSpace w = bwd_space(a.s, p, bias ? 2 * a.bias.distance + 1 : 0, dtype);
+  const BwdSpace w = bwd_space(a.s, a.w, p, bias ? 2 * a.bias.distance + 1 : 0, dtype);
   if (w.total > 0 && (workspace == nullptr || workspace_bytes < w.total))  // few frames without a bias: none is needed
     return fail(PMSST_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, w.total, workspace_bytes);
   PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0 || w.total == 0, "%s: workspace must be 16-byte aligned", what);
@@ -1181,6 +1199,7 @@ int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out
   a.chunk_tiles = static_cast<int32_t>(p.chunk_tiles);
   a.splits = static_cast<uint32_t>(p.splits);
   a.part_keys = static_cast<int32_t>(p.part_keys());
+  a.sink_rows = static_cast<int32_t>(p.sink_rows(a.s, a.w));
   a.late_first = a.w.right >= 0 && a.w.left < 0;
   const int64_t per = std::max(p.row_tiles * a.s.G, p.blocks());
   PMSST_REQUIRE(grid_fits(batch * kv_heads, per), "%s: too many rows for one call", what);
