@@ -480,8 +480,8 @@ size_t pmsst_local_attention_backward_workspace_size(int64_t batch, int64_t quer
                                                      int64_t sinks, int has_starts, int64_t max_distance, int dtype);
 /* Gradients of the forward (same masks, limits, bias and scale) from its dense out and its lse: grad_q[batch, queries,
  * heads, head_dim], grad_k and grad_v[batch, keys, kv_heads, head_dim], and with a bias grad_bias[buckets, heads] in
- * the bias's dtype, all dense and fully written (exact zeros in grad_q and grad_k where a query sees one frame).
- * An fp32 grad_bias of 16-bit tensors is summed from unrounded fp32 values.
+ * the bias's dtype, all dense and fully written (exact zeros in grad_q and grad_k where a query sees one
+ * frame that neither window, masks nor bias hide).  An fp32 grad_bias of 16-bit tensors is summed from unrounded fp32 values.
  * bucket_order, bucket_first: device int32[2 max_distance + 1] and [buckets + 1], the indexes of bucket_of in the order
  * of their buckets, and where each bucket's begin. */
 int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out_strides, const void* q,

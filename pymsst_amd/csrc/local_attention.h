@@ -112,10 +112,11 @@ __device__ __forceinline__ float bias_value(float v, float unit) {
 }
 
 // Fills `table` by distance, kPad + distance entries on either side of 0 (falling distances if DOWN).  Two loads, one
-// waiting for the other, make an entry: four are on their way at once.
+// waiting for the other, make an entry: four are on their way at once.  True if one of this thread's hides its frames.
 template <typename T, bool DOWN>
-__device__ __forceinline__ void fill_bias(float* table, const BiasArgs& t, int heads, int head, float unit, int threads) {
+__device__ __forceinline__ bool fill_bias(float* table, const BiasArgs& t, int heads, int head, float unit, int threads) {
   const int entries = 2 * t.distance + 1 + 2 * kPad;
+  bool hides = false;
   for (int base = threadIdx.x; base < entries; base += 4 * threads) {
     int bucket[4];
     float value[4];
@@ -128,9 +129,23 @@ __device__ __forceinline__ void fill_bias(float* table, const BiasArgs& t, int h
     for (int j = 0; j < 4; ++j) value[j] = bias_entry(t, dtype_code<T>(), heads, head, bucket[j]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (base + j * threads < entries) table[base + j * threads] = bias_value(value[j], unit);
+      const float v = bias_value(value[j], unit);
+      hides |= v == -kInf;
+      if (base + j * threads < entries) table[base + j * threads] = v;
     }
   }
+  return hides;
+}
+
+// Bits of the 32 frames from key0 on that the bias (a table by rising distance) does not hide from a query at frame `pos`.
+__device__ __forceinline__ uint32_t bias_shows(const float* table, int distance, int pos, int key0) {
+  uint32_t bits = 0;
+#pragma unroll 4
+  for (int i = 0; i < 32; ++i) {
+    const int d = min(max(key0 + i - pos, -distance), distance);
+    bits |= (table[d + distance + kPad] != -kInf ? 1u : 0u) << i;
+  }
+  return bits;
 }
 
 // Whether the distances lo .. lo + 62 of a tile are all on one end of the table (that end's entry), or not.

@@ -129,7 +129,7 @@ __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 || (TWICE && DP == 128) 
   constexpr int BK = local_tile<T, DP>(), SUBS = BK / 32;
   constexpr bool kHalf = std::is_same<T, f16>::value;
   __shared__ __attribute__((aligned(16))) char lds[kStages][2][BK * DB];
-  extern __shared__ float table[];  // the bias by distance
+  extern __shared__ float table[];  // the bias by distance, then for each wave whether it saw an entry that hides
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t pair, sub_block;
   if (!locate(a.grid, pair, sub_block)) return;
@@ -186,7 +186,7 @@ __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 || (TWICE && DP == 128) 
   constexpr uint64_t kAll = BK == 64 ? ~uint64_t{0} : 0xFFFFFFFFu;
 
   // Where a query sees one frame alone, P is 1 whatever the score: dS, and with it dQ and dK, is zero exactly, while P
-  // from lse and D from O would leave their rounding errors.
+  // from lse and D from O would leave their rounding errors.  (What the bias hides is taken off below, with its table.)
   int found = 0;
   if (mask == nullptr) {
     found = max(0, high - low) + max(0, min(sinks, low));
@@ -202,8 +202,8 @@ __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 || (TWICE && DP == 128) 
       if (!__any(row_ok && found < 2)) break;
     }
   }
-  const uint32_t lone = static_cast<uint32_t>(__ballot(found == 1));
-  const float alive = found == 1 ? 0.f : 1.f;
+  uint32_t lone = static_cast<uint32_t>(__ballot(found == 1));
+  float alive = found == 1 ? 0.f : 1.f;
 
   const float row_base = base;
   int e = 0;
@@ -246,11 +246,33 @@ __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) > 256 || (TWICE && DP == 128) 
   const float* lane_table = nullptr;  // this lane's entry for frame 0
   float far_low = 0.f, far_high = 0.f, rest[2] = {0.f, 0.f};
   if constexpr (BIAS) {
-    fill_bias<T, false>(table, a.bias, s.H, head, a.bias_unit, 64 * NW);
+    const int entries = 2 * a.bias.distance + 1 + 2 * kPad;
+    const bool own = __any(fill_bias<T, false>(table, a.bias, s.H, head, a.bias_unit, 64 * NW));
+    if (lane == 0) table[entries + wave] = own ? 1.f : 0.f;
     __syncthreads();
     far_low = table[0];
-    far_high = table[2 * a.bias.distance + 2 * kPad];
+    far_high = table[entries - 1];
     lane_table = table + (a.bias.distance + kPad + 8 * h - pos);
+    float hides = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) hides += table[entries + w];
+    if (hides != 0.f) {
+      // frames that the bias hides are not seen: counted again, until every query has two
+      found = 0;
+      for (int i = 0; i < list.total && __any(row_ok && found < 2); ++i) {
+        const int key0 = list.at(i) * BK;
+        uint64_t seen = range_bits(key0, count) & kAll;
+        if (mask) seen &= __ballot(mask_byte(list.at(i)) != 0);
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) {
+          const int at = key0 + 32 * u;
+          found += __popc(static_cast<uint32_t>(seen >> (32 * u)) & frames_seen(low, high, a.w.sinks, at) &
+                          bias_shows(table, a.bias.distance, pos, at));
+        }
+      }
+      lone = static_cast<uint32_t>(__ballot(found == 1));
+      alive = found == 1 ? 0.f : 1.f;
+    }
   }
   // What a row's dS adds up to is 0 but for D's error (out is rounded, and so were the weights it is a sum of); with it, D is
   // rowsum(P o dP) to fp32's precision.  Of 16-bit rows that see few frames, D's error would be as large as the roundings
@@ -673,7 +695,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
   __shared__ __attribute__((aligned(16))) char rows[2][64 * DB];
   __shared__ __attribute__((aligned(16))) char ps[2][64 * PB];
   __shared__ float most[2];
-  extern __shared__ float table[];  // the bias by distance, then each wave's bins
+  extern __shared__ float table[];  // the bias by distance, each wave's bins, and whether it saw an entry that hides
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t pair, sub;
   if (!locate(a.grid, pair, sub)) return;
@@ -686,6 +708,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
   if (a.km.mask) kept &= __ballot(a.km.mask[b * a.km.stride + min(lane, s.M - 1)] != 0);
   const int entries = 2 * a.bias.distance + 1 + 2 * kPad;
   float* bins = table + entries + kBinPad + wave * (entries + 2 * kBinPad);
+  float* hides = table + 3 * entries + 4 * kBinPad;  // of 2 waves
 
   Tile<T, DP, 64, 2> tile;  // no state: every move computes its addresses
   tile.fetch_cut(kv[0], static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h, 0, s.M, d_units, [&](int i) { return i * a.ks.n; });
@@ -702,24 +725,27 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
       if (g > 0 || t > 0) __syncthreads();  // the tiles of the rows before these have been read, and the table
       tile.fetch_cut(rows[0], static_cast<const T*>(a.q) + b * a.qs.b + head * a.qs.h, t * 64, s.N, d_units, [&](int i) { return i * a.qs.n; });
       tile.fetch_cut(rows[1], static_cast<const T*>(a.dout) + b * a.gs.b + head * a.gs.h, t * 64, s.N, d_units, [&](int i) { return i * a.gs.n; });
-      if constexpr (BIAS) {
-        if (t == 0) {
-          fill_bias<T, false>(table, a.bias, s.H, head, a.bias_unit, 128);
-          for (int i = lane; i < entries; i += 64) bins[i] = 0.f;
-        }
-      }
       const int n0 = t * 64 + 32 * wave, n = n0 + (lane & 31), p0 = start + n0, pos = start + n;
       const bool row_ok = n < s.N;
-      float base = -kInf;  // -lse in log2 units: a row that sees no frame (and one past the end) has no weight
+      // -lse in log2 units: a row that sees no frame (and one past the end) has no weight.  (On its way before the bias:
+      // 1032 x 62, 137 us against 142.)
+      float base = -kInf;
       if (row_ok) {
         const float lse = a.lse[(static_cast<int64_t>(b) * s.H + head) * s.N + n];
         base = lse == -kInf ? -kInf : -lse * kLog2e;
+      }
+      if constexpr (BIAS) {
+        if (t == 0) {
+          const bool own = __any(fill_bias<T, false>(table, a.bias, s.H, head, a.bias_unit, 128));
+          hides[wave] = own ? 1.f : 0.f;
+          for (int i = lane; i < entries; i += 64) bins[i] = 0.f;
+        }
       }
       const int low = low_of(a.w, pos), high = high_of(a.w, pos, count);
       uint32_t seen[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) seen[u] = static_cast<uint32_t>(kept >> (32 * u)) & frames_seen(low, high, a.w.sinks, 32 * u);
-      const bool lone = __popc(seen[0]) + __popc(seen[1]) == 1;
+      int found = __popc(seen[0]) + __popc(seen[1]);
       vm_wait<0>();
       if (g == 0 && t == 0 && (kept != ~uint64_t{0} || d_units != tile.UNITS)) {
         tile.clear(kv[0], kept, d_units);
@@ -737,6 +763,11 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
       if constexpr (BIAS) {
         far_low = table[0];
         far_high = table[entries - 1];
+        if (hides[0] + hides[1] != 0.f) {  // frames that the bias hides are not seen
+          found = 0;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) found += __popc(seen[u] & bias_shows(table, a.bias.distance, pos, 32 * u));
+        }
       }
       f32x16_t p[2], ds[2];
       bool near[2] = {false, false}, upper[2] = {false, false};
@@ -776,7 +807,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
           p[u][i] = w;
         }
       }
-      const float delta = half_sum(sum[0] + sum[1]), alive = lone ? 0.f : 1.f;
+      const float delta = half_sum(sum[0] + sum[1]), alive = found == 1 ? 0.f : 1.f;
       float top = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -1008,7 +1039,7 @@ int launch_dq(BwdArgs& a, int64_t begin, int64_t end, hipStream_t stream) {
   a.grid = make_grid(int64_t{a.s.B} * a.s.Hk, (end - begin) * a.s.G);
   const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
   if (a.bias.table) {
-    local_dq_kernel<T, DP, NW, true, TWICE><<<grid, 64 * NW, bias_entries(a.bias.distance) * 4, stream>>>(a);
+    local_dq_kernel<T, DP, NW, true, TWICE><<<grid, 64 * NW, (bias_entries(a.bias.distance) + NW) * 4, stream>>>(a);
   } else {
     local_dq_kernel<T, DP, NW, false, TWICE><<<grid, 64 * NW, 0, stream>>>(a);
   }
@@ -1062,7 +1093,7 @@ int run_bwd(BwdArgs& a, const BwdPlan& p, hipStream_t stream) {
       a.grid = make_grid(pairs, 1);
       const dim3 grid(static_cast<uint32_t>(grid_blocks(a.grid)));
       if (a.bias.table) {
-        local_few_kernel<T, DP, true><<<grid, 128, bins_bytes(a, 2), stream>>>(a);
+        local_few_kernel<T, DP, true><<<grid, 128, bins_bytes(a, 2) + 8, stream>>>(a);
       } else {
         local_few_kernel<T, DP, false><<<grid, 128, 0, stream>>>(a);
       }
