@@ -380,6 +380,73 @@ StepPlan plan_step(const Shape& s, int64_t left, int64_t sinks, int dtype) {
   return p;
 }
 
+// The rows of a [batch, positions, heads] tensor: dense, `bytes` each, where they begin and how far apart they lie.
+struct RowSet {
+  uintptr_t at;
+  int64_t size[3], apart[3], bytes;
+};
+
+// Whether two sets of rows share a byte: whether a's row - b's row, a sum of strides times indexes, can lie within their
+// bytes of each other.  The largest strides' multiples are tried first, and of each only those that the smaller ones can
+// still make up for; sets that take more than 2^16 trials count as sharing one.
+bool rows_meet(const RowSet& a, const RowSet& b) {
+  typedef __int128 wide;
+  struct Term { int64_t apart, lo, hi; } terms[6];
+  int count = 0;
+  auto add = [&](int64_t apart, int64_t lo, int64_t hi) {
+    if (apart < 0) { apart = -apart; const int64_t t = lo; lo = -hi; hi = -t; }
+    if (apart == 0 || lo == hi) return;
+    int i = 0;
+    while (i < count && terms[i].apart > apart) ++i;
+    if (i < count && terms[i].apart == apart) {
+      terms[i].lo += lo;
+      terms[i].hi += hi;
+      return;
+    }
+    for (int j = count++; j > i; --j) terms[j] = terms[j - 1];
+    terms[i] = {apart, lo, hi};
+  };
+  for (int i = 0; i < 3; ++i) {
+    if (a.size[i] == 0 || b.size[i] == 0) return false;
+    add(a.apart[i], 0, a.size[i] - 1);
+    add(b.apart[i], 1 - b.size[i], 0);
+  }
+  wide lo[7], hi[7];  // what the terms from i on can sum up to
+  lo[count] = hi[count] = 0;
+  for (int i = count; i-- > 0;) {
+    lo[i] = lo[i + 1] + static_cast<wide>(terms[i].apart) * terms[i].lo;
+    hi[i] = hi[i + 1] + static_cast<wide>(terms[i].apart) * terms[i].hi;
+  }
+  // the sum has to lie in (from, to), of those before i less what they have
+  int64_t x[6], last[6];
+  wide from[7], to[7];
+  from[0] = static_cast<wide>(b.at) - a.at - a.bytes;
+  to[0] = static_cast<wide>(b.at) - a.at + b.bytes;
+  auto up = [](wide n, wide d) { return n >= 0 ? (n + d - 1) / d : -(-n / d); };
+  auto down = [&](wide n, wide d) { return -up(-n, d); };
+  auto open = [&](int i) {
+    const wide first = up(from[i] + 1 - hi[i + 1], terms[i].apart), end = down(to[i] - 1 - lo[i + 1], terms[i].apart);
+    x[i] = static_cast<int64_t>(first < terms[i].lo ? terms[i].lo : first > terms[i].hi ? terms[i].hi + wide{1} : first);
+    last[i] = static_cast<int64_t>(end > terms[i].hi ? terms[i].hi : end < terms[i].lo ? terms[i].lo - wide{1} : end);
+  };
+  if (from[0] >= hi[0] || to[0] <= lo[0]) return false;
+  if (count == 0) return true;
+  int i = 0;
+  open(0);
+  for (int trials = 0; trials < 1 << 16; ++trials) {
+    while (x[i] > last[i]) {
+      if (--i < 0) return false;
+      ++x[i];
+    }
+    const wide step = static_cast<wide>(terms[i].apart) * x[i];
+    from[i + 1] = from[i] - step;
+    to[i + 1] = to[i] - step;
+    if (i + 1 == count) return true;  // (the last term's multiples are those that fit)
+    open(++i);
+  }
+  return true;
+}
+
 size_t step_workspace(const Shape& s, const StepPlan& p) {
   if (p.splits == 1) return 0;
   const size_t rows = static_cast<size_t>(p.splits) * s.B * s.Hk * s.R;
@@ -472,6 +539,17 @@ int pmsst_local_attention_step(const void* q, const int64_t* q_strides, const vo
     return fail(PMSST_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
   PMSST_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0 || need == 0, "%s: workspace must be 16-byte aligned", what);
   PMSST_REQUIRE(k_cache != v_cache, "%s: the caches lie in one place", what);
+  // the kernel reads what other blocks of it write, were the caches not apart from each other and from q, k and v
+  auto rows_of = [&](const void* at, const Strides& st, int64_t positions_, int64_t heads_) {
+    const int64_t size = dtype_size(dtype);
+    return RowSet{reinterpret_cast<uintptr_t>(at), {batch, positions_, heads_}, {st.b * size, st.n * size, st.h * size}, head_dim * size};
+  };
+  const RowSet caches[2] = {rows_of(k_cache, a.kcs, slots, kv_heads), rows_of(v_cache, a.vcs, slots, kv_heads)};
+  const RowSet read[3] = {rows_of(q, a.qs, frames, heads), rows_of(k, a.ks, frames, kv_heads), rows_of(v, a.vs, frames, kv_heads)};
+  PMSST_REQUIRE(!rows_meet(caches[0], caches[1]), "%s: the caches share memory", what);
+  for (const RowSet& cache : caches) {
+    for (const RowSet& rows : read) PMSST_REQUIRE(!rows_meet(cache, rows), "%s: q, k or v lies in a cache", what);
+  }
   a.q = q;
   a.k = k;
   a.v = v;

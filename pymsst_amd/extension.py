@@ -839,8 +839,8 @@ class HipFusedExtension:
         stream is idle, its caches stay and its ``out`` is 0.  Frame ``f`` lies in slot ``f`` if ``f < sinks``, else
         in ``sinks + (f - sinks) % (slots - sinks)``.  A query at frame ``p`` sees the frames ``p - left .. p`` and the
         first ``sinks``; the caches must have at least ``sinks + left + N`` slots, and hold what was written for the
-        frames that are seen.  Caches: rows dense and whole 16 bytes apart, no two in one place, none of them ``k`` or
-        ``v``.  Bias and scale as in :meth:`local_attention_forward`."""
+        frames that are seen.  Caches: rows dense and whole 16 bytes apart, no two in one place, and none where ``q``,
+        ``k`` or ``v`` lies.  Bias and scale as in :meth:`local_attention_forward`."""
         _req(k.dim() == 4 and q.dim() == 4 and k.shape[1] == q.shape[1], "q, k and v must have as many new frames")
         _, _, _, scale = self._attention_check(q, k, v, None, None, scale, 0.0, None)
         b, n, h, d = q.shape
