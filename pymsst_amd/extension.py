@@ -840,7 +840,8 @@ class HipFusedExtension:
         in ``sinks + (f - sinks) % (slots - sinks)``.  A query at frame ``p`` sees the frames ``p - left .. p`` and the
         first ``sinks``; the caches must have at least ``sinks + left + N`` slots, and hold what was written for the
         frames that are seen.  Caches: rows dense and whole 16 bytes apart, no two in one place, and none where ``q``,
-        ``k`` or ``v`` lies.  Bias and scale as in :meth:`local_attention_forward`."""
+        ``k`` or ``v`` lies.  Bias and scale as in :meth:`local_attention_forward`.  A step has no derivative: ``out`` requires
+        no gradient, and the caches may not (outside ``torch.no_grad()``)."""
         _req(k.dim() == 4 and q.dim() == 4 and k.shape[1] == q.shape[1], "q, k and v must have as many new frames")
         _, _, _, scale = self._attention_check(q, k, v, None, None, scale, 0.0, None)
         b, n, h, d = q.shape
@@ -850,6 +851,8 @@ class HipFusedExtension:
              "k_cache and v_cache must have shape [B, slots, Hk, D]")
         _req(k_cache.device == q.device and v_cache.device == q.device and k_cache.dtype == q.dtype and v_cache.dtype == q.dtype,
              "k_cache and v_cache must have q's dtype and device")
+        _req(not (k_cache.requires_grad or v_cache.requires_grad) or not torch.is_grad_enabled(),
+             "k_cache and v_cache are written in place and may not require a gradient")
         strides = self._cache_strides(k_cache, "k_cache"), self._cache_strides(v_cache, "v_cache")
         slots = k_cache.shape[1]
         _req(slots - sinks >= left + n, "the caches must have at least sinks + left + N slots")
@@ -869,6 +872,8 @@ class HipFusedExtension:
                 code, _ptr(ws), size, _stream(q.device),
             )
         check(rc, "pmsst_local_attention_step")
+        # as after torch's own writes in place: a backward that has saved a cache is an error now, not a wrong gradient
+        torch.autograd.graph.increment_version((k_cache, v_cache))
         return out
 
     def _cache_strides(self, t, name):
