@@ -499,12 +499,12 @@ int pmsst_local_attention_backward(const void* grad_out, const int64_t* grad_out
 size_t pmsst_local_attention_step_workspace_size(int64_t batch, int64_t frames, int64_t heads, int64_t kv_heads,
                                                  int64_t head_dim, int64_t left, int64_t sinks, int dtype);
 /* Frame by frame: `frames` new frames of each stream are written into its caches and attended to with what the caches
- * hold.  Stream b stands at frame positions[b] (device int32), which q, k, v[b, 0] are; frame f lies in slot f of the
- * caches if f < sinks, else in slot sinks + (f - sinks) % (slots - sinks).  A query at frame p sees the frames from
- * p - left to p and the first `sinks`; slots - sinks must be at least left + frames.  positions[b] < 0: the stream is
- * idle, its caches stay as they are and its out is 0.  k_cache, v_cache: [batch, slots, kv_heads, head_dim] with
- * strides as elsewhere (no two elements in one place, of either), apart from q, k and v (caches that share memory with
- * each other or with them are refused); bias as in the forward. */
+ * hold.  Stream b stands at frame positions[b] (device int32, at most 2^31 - frames), which q, k, v[b, 0] are; frame f
+ * lies in slot f of the caches if f < sinks, else in slot sinks + (f - sinks) % (slots - sinks).  A query at frame p sees
+ * the frames from p - left to p and the first `sinks`; slots - sinks must be at least left + frames.  positions[b] < 0:
+ * the stream is idle, its caches stay as they are and its out is 0.  k_cache, v_cache: [batch, slots, kv_heads, head_dim]
+ * with strides as elsewhere (no two elements in one place, of either), apart from q, k and v (caches that share memory
+ * with each other or with them are refused); bias as in the forward. */
 int pmsst_local_attention_step(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                const void* v, const int64_t* v_strides, void* k_cache, const int64_t* k_cache_strides,
                                void* v_cache, const int64_t* v_cache_strides, const int32_t* positions, int64_t left,

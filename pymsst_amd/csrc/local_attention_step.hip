@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void local_step_kernel(StepArgs a) {
 
   // the stream's frames in the order they are visited: the sinks' (their slots are their frames), the window's, the new
   const int sink_frames = now < 0 ? 0 : min(a.sinks, now);
-  const int window_first = max(sink_frames, now - a.left);
+  const int window_first = max(sink_frames, max(now, 0) - a.left);
   const int window_frames = now < 0 ? 0 : now - window_first;
   const int old_frames = sink_frames + window_frames;
   const int total = now < 0 ? 0 : old_frames + s.N;
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256) void local_step_kernel(StepArgs a) {
     const int last = base + KPW * kUnroll;
     const bool whole = last <= min(x1, old_frames) && (base >= sink_frames + s.N - 1 || last <= sink_frames);
     if constexpr (BIAS) {
-      if (whole && base >= sink_frames && now - (window_first + last - 1 - sink_frames) >= a.bias.distance) {
+      if (whole && base >= sink_frames && now - (window_first + (last - 1 - sink_frames)) >= a.bias.distance) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           const float far = shared[table_of(r) + a.bias.distance];

@@ -835,13 +835,13 @@ class HipFusedExtension:
         written into its caches ``[B, slots, Hk, D]`` (in place) and ``q[B, N, H, D]`` attends to what they hold; returns
         ``out[B, N, H, D]``.
 
-        ``positions`` (int32 ``[B]``, read when the kernel runs): the frame of each stream's first new one; below 0 the
-        stream is idle, its caches stay and its ``out`` is 0.  Frame ``f`` lies in slot ``f`` if ``f < sinks``, else
-        in ``sinks + (f - sinks) % (slots - sinks)``.  A query at frame ``p`` sees the frames ``p - left .. p`` and the
-        first ``sinks``; the caches must have at least ``sinks + left + N`` slots, and hold what was written for the
-        frames that are seen.  Caches: rows dense and whole 16 bytes apart, no two in one place, and none where ``q``,
-        ``k`` or ``v`` lies.  Bias and scale as in :meth:`local_attention_forward`.  A step has no derivative: ``out`` requires
-        no gradient, and the caches may not (outside ``torch.no_grad()``)."""
+        ``positions`` (int32 ``[B]``, read when the kernel runs): the frame of each stream's first new one, at most
+        ``2**31 - N``; below 0 the stream is idle, its caches stay and its ``out`` is 0.  Frame ``f`` lies in slot ``f``
+        if ``f < sinks``, else in ``sinks + (f - sinks) % (slots - sinks)``.  A query at frame ``p`` sees the frames
+        ``p - left .. p`` and the first ``sinks``; the caches must have at least ``sinks + left + N`` slots, and hold what
+        was written for the frames that are seen (finite numbers).  Caches: rows dense and whole 16 bytes apart, no two in
+        one place, and none where ``q``, ``k`` or ``v`` lies.  Bias and scale as in :meth:`local_attention_forward`.  A
+        step has no derivative: ``out`` requires no gradient, and the caches may not (outside ``torch.no_grad()``)."""
         _req(k.dim() == 4 and q.dim() == 4 and k.shape[1] == q.shape[1], "q, k and v must have as many new frames")
         _, _, _, scale = self._attention_check(q, k, v, None, None, scale, 0.0, None)
         b, n, h, d = q.shape
