@@ -681,8 +681,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
 // All gradients in one pass where a tile holds every frame, as in the cross attention: a block of 2 waves keeps K and V of
 // a (batch row, key head) in LDS and passes over the query tiles of its heads; P and dS go through LDS to be the other
 // operand of dV and dK.  A wave's whole rows of P and dP are in registers, so D is their sum, in fp32.  5 products instead
-// of 7, and every tensor is moved once: 1032 x 62 queries over 62 frames with a bias, bf16, 8 heads of 64, 132 us (HBM, 3.5
-// TB/s at 6 waves a CU: 48 KB of LDS a block) against 119 + 116 of the two kernels.
+// of 7, and every tensor is moved once: 1032 x 62 queries over 62 frames with a bias, bf16, 8 heads of 64, 131 us (HBM, 3.5
+// TB/s at 6 waves a CU: 48 KB of LDS a block) against 119 + 116 of the two kernels.  The same holds with many queries, which a
+// block takes in turn (the whole backward, over 64 frames): 256 x 512, 8 heads, 147 us against 285; 256 x 4096, one head,
+// 239 against 294; 64 x 2100 over 50, 4 heads, no bias, 86 against 137.
 // (Waves that share a SIMD: fp16's scaling and a bias together pass the registers of two.)
 template <typename T, int DP, bool BIAS>
 constexpr int few_waves() { return DP == 128 || (DP == 64 && BIAS && std::is_same<T, f16>::value) ? 1 : 2; }
@@ -721,31 +723,40 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
   for (int g = 0; g < s.G; ++g) {
     const int head = hk * s.G + g;
     float far_low = 0.f, far_high = 0.f, sum_low = 0.f, sum_high = 0.f;
+    bool some_hidden = false;
     for (int t = 0; t < tiles; ++t) {
       if (g > 0 || t > 0) __syncthreads();  // the tiles of the rows before these have been read, and the table
       tile.fetch_cut(rows[0], static_cast<const T*>(a.q) + b * a.qs.b + head * a.qs.h, t * 64, s.N, d_units, [&](int i) { return i * a.qs.n; });
       tile.fetch_cut(rows[1], static_cast<const T*>(a.dout) + b * a.gs.b + head * a.gs.h, t * 64, s.N, d_units, [&](int i) { return i * a.gs.n; });
       const int n0 = t * 64 + 32 * wave, n = n0 + (lane & 31), p0 = start + n0, pos = start + n;
       const bool row_ok = n < s.N;
-      // -lse in log2 units: a row that sees no frame (and one past the end) has no weight.  (On its way before the bias:
-      // 1032 x 62, 137 us against 142.)
-      float base = -kInf;
-      if (row_ok) {
-        const float lse = a.lse[(static_cast<int64_t>(b) * s.H + head) * s.N + n];
-        base = lse == -kInf ? -kInf : -lse * kLog2e;
-      }
+      // -lse in log2 units: a row that sees no frame (and one past the end) has no weight.  (On its way before the bias.)
+      float lse = -kInf;
+      if (row_ok) lse = a.lse[(static_cast<int64_t>(b) * s.H + head) * s.N + n];
       if constexpr (BIAS) {
         if (t == 0) {
           const bool own = __any(fill_bias<T, false>(table, a.bias, s.H, head, a.bias_unit, 128));
           hides[wave] = own ? 1.f : 0.f;
           for (int i = lane; i < entries; i += 64) bins[i] = 0.f;
+          __syncthreads();
+          some_hidden = __builtin_amdgcn_readfirstlane(hides[0] + hides[1] != 0.f);
         }
       }
+      const float base = lse == -kInf ? -kInf : -lse * kLog2e;
       const int low = low_of(a.w, pos), high = high_of(a.w, pos, count);
       uint32_t seen[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) seen[u] = static_cast<uint32_t>(kept >> (32 * u)) & frames_seen(low, high, a.w.sinks, 32 * u);
       int found = __popc(seen[0]) + __popc(seen[1]);
+      if constexpr (BIAS) {
+        // frames that the bias hides are not seen (here, before the wait for the tiles: behind it 256 x 4096 queries take
+        // 250 us, not 239)
+        if (some_hidden) {
+          found = 0;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) found += __popc(seen[u] & bias_shows(table, a.bias.distance, pos, 32 * u));
+        }
+      }
       vm_wait<0>();
       if (g == 0 && t == 0 && (kept != ~uint64_t{0} || d_units != tile.UNITS)) {
         tile.clear(kv[0], kept, d_units);
@@ -763,11 +774,6 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(few_waves<T
       if constexpr (BIAS) {
         far_low = table[0];
         far_high = table[entries - 1];
-        if (hides[0] + hides[1] != 0.f) {  // frames that the bias hides are not seen
-          found = 0;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) found += __popc(seen[u] & bias_shows(table, a.bias.distance, pos, 32 * u));
-        }
       }
       f32x16_t p[2], ds[2];
       bool near[2] = {false, false}, upper[2] = {false, false};
