@@ -10,9 +10,9 @@
 //
 // What bounds it.  Heads of 64 in 16 bits, all frames seen: the cross attention's pass (products, exponentials and the
 // tiles' LDS reads share a clock of 1.7 GHz) and, with a bias, 16 LDS reads a sub-tile more: 124 x 948, 8 heads, fp16,
-// 376 us, 608 TFLOP/s.  Windows of a tile or two: HBM, and the tiles at the window's ends that are partly seen: 248 x 258
-// queries, 8 heads, windows of 64 either way, bf16, 74 us, 3.5 TB/s.  Long rows with a window of 1024 (16 x 2760 queries, 8
-// heads, bias, bf16): 149 us, 507 TFLOP/s of the pairs that are seen.  Few blocks: the latency of the tiles a block takes
+// 366 us, 623 TFLOP/s.  Windows of a tile or two: HBM, and the tiles at the window's ends that are partly seen: 248 x 258
+// queries, 8 heads, windows of 64 either way, bf16, 71 us, 3.7 TB/s.  Long rows with a window of 1024 (16 x 2760 queries, 8
+// heads, bias, bf16): 151 us, 500 TFLOP/s of the pairs that are seen.  Few blocks: the latency of the tiles a block takes
 // in turn.
 #include "local_attention.h"
 

@@ -681,7 +681,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(dkv_wav
 // All gradients in one pass where a tile holds every frame, as in the cross attention: a block of 2 waves keeps K and V of
 // a (batch row, key head) in LDS and passes over the query tiles of its heads; P and dS go through LDS to be the other
 // operand of dV and dK.  A wave's whole rows of P and dP are in registers, so D is their sum, in fp32.  5 products instead
-// of 7, and every tensor is moved once: 1032 x 62 queries over 62 frames with a bias, bf16, 8 heads of 64, 131 us (HBM, 3.5
+// of 7, and every tensor is moved once: 1032 x 62 queries over 62 frames with a bias, bf16, 8 heads of 64, 132 us (HBM, 3.5
 // TB/s at 6 waves a CU: 48 KB of LDS a block) against 119 + 116 of the two kernels.  The same holds with many queries, which a
 // block takes in turn (the whole backward, over 64 frames): 256 x 512, 8 heads, 147 us against 285; 256 x 4096, one head,
 // 239 against 294; 64 x 2100 over 50, 4 heads, no bias, 86 against 137.

@@ -1,5 +1,5 @@
 // Local attention frame by frame: a few new frames of each stream are written into its ring caches and attended to with
-// the first frames (sinks) and the last ones that the caches hold, in one launch.
+// the first frames (sinks) and the last ones that the caches hold, in one launch, or two where blocks are split.
 //
 // The bytes of the keys and values bound it, so there are no matrix instructions and no LDS tiles: a row of K is
 // spread over the lanes of a group, 16 bytes each, and a wave's load takes 64 / group rows.  Every lane keeps the
@@ -13,9 +13,9 @@
 // The slots that are written hold frames that no query of the call sees (slots - sinks >= left + frames), and the new
 // frames are read from k and v, not from the caches: no block waits for another.
 //
-// One row: HBM and the launch; 8 rows of a shared key head: the same (200 MB of fp16 keys and values of 128 in 46 us, 4.3
-// TB/s).  Four rows with a bias: the vector unit (219 MB in 57 us, 3.8 TB/s; a padded table that saves the lookups' cuts changes
-// nothing).  The smallest call's kernel is 5 us and its enqueue 14.  Waves of a block: 8 in place of 4 took 50 us for 47, 2 took 80; loads in
+// One row: HBM and the launch; 8 rows of a shared key head: the same (200 MB of fp16 keys and values of 128 in 47 us, 4.3
+// TB/s).  Four rows with a bias: the vector unit (219 MB in 58 us, 3.8 TB/s; a padded table that saves the lookups' cuts changes
+// nothing).  The smallest call's kernel is 5 us and its enqueue 15.  Waves of a block: 8 in place of 4 took 50 us for 47, 2 took 80; loads in
 // flight a lane: kUnroll of 2 and 8 took 48 and 50.
 #include "local_attention.h"
 
